@@ -406,6 +406,74 @@ int ins_scan_part(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int
 int ins_merge_parts(ins_cache *cache, int32_t B, int32_t n_parts, const void *parts, int64_t *out,
                     ins_stats *stats, void *stream);
 
+/* Page operations (the reference's cache only appends, resets and loads,
+ * cache/base.py:29-81). Pages full of rows can be held by several sequences;
+ * a page that rows are written to is always one sequence's own, so an ingress
+ * after any of these calls needs no check. Each call takes B sequences, moves
+ * each row at most once, and is one launch (two when its descriptors exceed
+ * 3,840 bytes, or for ins_cache_put_rows). A call that is refused (EBADLEN,
+ * EINVAL) has changed nothing. ins_cache_reset frees pages too, but blocks;
+ * ins_cache_truncate to 0 does not.
+ *
+ * fork: sequence dst[i], which must be empty, becomes the first lengths[i]
+ * rows of src[i] (all of them when lengths is NULL). Full pages are shared, a
+ * page that is not full is copied.
+ *
+ * compact: of sequence seq_ids[i], rows below base[i] stay, and of those from
+ * base[i] on the counts[i] rows base[i] + keep[..] stay, moved together after
+ * them; the length becomes base[i] + counts[i]. keep holds the sequences'
+ * offsets one after another (host; each sequence's distinct and rising). A
+ * page that is written and that another sequence holds too is replaced by a
+ * new one. Accepting a drafted tree's path is base = the context's length and
+ * keep = the path's nodes.
+ *
+ * truncate: keep the first lengths[i] rows, free the pages after them.
+ *
+ * rows: copy rows [t0[i], t0[i] + n[i]) of seq_ids[i], one sequence after
+ * another, to `rows` (device, [sum n][n_kv][bytes_per_token], the bytes of
+ * CompressedCache.buf, 4-byte aligned); the device form of ins_cache_export.
+ *
+ * put_rows: append n[i] such rows (device) to seq_ids[i]; the device form of
+ * ins_cache_import. */
+int64_t ins_cache_free_pages(const ins_cache *cache);
+int ins_cache_fork(ins_cache *cache, int32_t B, const int32_t *src, const int32_t *dst,
+                   const int64_t *lengths, void *stream);
+int ins_cache_compact(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int64_t *base,
+                      const int64_t *counts, const int64_t *keep, void *stream);
+int ins_cache_truncate(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int64_t *lengths,
+                       void *stream);
+int ins_cache_rows(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int64_t *t0,
+                   const int64_t *n, uint8_t *rows, void *stream);
+int ins_cache_put_rows(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int64_t *n,
+                       const uint8_t *rows, void *stream);
+
+/* Element types of ins_sample's logits. */
+enum { INS_F32 = 0, INS_F16 = 1, INS_BF16 = 2 };
+
+/* One sampled token per row of logits (no reference counterpart: its driver
+ * takes the argmax on the host). With z_i = x_i / temperature and w_i =
+ * exp(z_i - max z): keep the top_k largest x_i (ties: the lowest indexes), of
+ * those the shortest leading run in falling order whose mass reaches top_p of
+ * theirs, of those the ones with w_i >= min_p; the token is the kept i with
+ * the largest z_i - log(-log u_i) (ties: the lowest index), a draw from the
+ * kept tokens' probabilities when u is uniform in [0, 1) and independent.
+ *
+ * logits: device, rows x vocab of `dtype`, row_stride elements from one row to
+ * the next (0: the same row again), each element adjacent to the one before;
+ * uniform: device float, likewise. vocab in [1, 262144]. temperature, top_k, top_p, min_p: device,
+ * one value a row, each may be NULL (1, no cut, no cut, no cut). A temperature
+ * that is not above 0 takes the largest logit; top_k <= 0 or >= vocab, top_p
+ * >= 1 and min_p <= 0 cut nothing. A NaN logit counts as -inf, and a logit of
+ * -inf is never chosen; a row with nothing else gives token -1 and
+ * log-probability -inf. tokens: device int64 [rows]; logprobs: device float
+ * [rows] or NULL, the token's log-probability among the kept ones (0 for a
+ * row taken by its largest logit). Runs on the device of the current context,
+ * stream-ordered. */
+int ins_sample(int32_t rows, int32_t vocab, const void *logits, int32_t dtype, int64_t row_stride,
+               const float *uniform, int64_t uniform_stride, const float *temperature,
+               const int32_t *top_k, const float *top_p, const float *min_p, int64_t *tokens,
+               float *logprobs, void *stream);
+
 /* The last error message recorded on this thread ("" if none). */
 const char *ins_last_error(void);
 

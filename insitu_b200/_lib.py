@@ -15,12 +15,21 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB_PATH = os.path.join(HERE, "libinsitu_b200.so")
-SOURCES = ("csrc/insitu.cu", "csrc/common.cuh", "csrc/kernels.cuh", "csrc/scan_chunked.cuh",
-           "csrc/scan_fused.cuh", "csrc/project.cuh")
+# translation units, each with the headers it is rebuilt for
+COMMON = ("csrc/common.cuh", "csrc/cache.h")
+UNITS = {
+    "csrc/insitu.cu": COMMON + ("csrc/kernels.cuh", "csrc/scan_chunked.cuh", "csrc/scan_fused.cuh",
+                                "csrc/project.cuh"),
+    "csrc/pages.cu": COMMON + ("csrc/plan.cuh",),
+    "csrc/sample.cu": COMMON,
+}
+SOURCES = tuple(dict.fromkeys(s for unit, headers in UNITS.items() for s in (unit, *headers)))
 HEADER = os.path.join(ROOT, "include", "insitu_b200.h")
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-Xcompiler", "-fPIC", "-shared", "-Xlinker", "-soname=libinsitu_b200.so"]
+              "-Xcompiler", "-fPIC"]
+LINK_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-Xlinker",
+              "-soname=libinsitu_b200.so"]
 
 # status codes (insitu_b200.h)
 INS_OK, INS_EBADLEN, INS_ETIMEOUT, INS_ERANGE, INS_EINVAL, INS_ENOMEM, INS_ECUDA = 0, 4, 5, 7, 8, 9, 10
@@ -99,7 +108,8 @@ SYMBOLS = ("ins_abi_version", "ins_bytes_per_token", "ins_cache_create", "ins_ca
            "ins_cache_ddr_image", "ins_seam", "ins_seam_device_positions",
            "ins_cache_launches", "ins_finalize", "ins_exp_lut",
            "ins_scan_recomputed_total", "ins_cache_set_scan_kernel", "ins_cache_set_wait_test",
-           "ins_project")
+           "ins_project", "ins_cache_free_pages", "ins_cache_fork", "ins_cache_compact",
+           "ins_cache_truncate", "ins_cache_rows", "ins_cache_put_rows", "ins_sample")
 
 
 def nvcc() -> str:
@@ -110,14 +120,33 @@ def nvcc() -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile ``libinsitu_b200.so`` in-tree for sm_100a."""
-    srcs = [os.path.join(HERE, s) for s in SOURCES] + [HEADER]
-    if not force and os.path.exists(LIB_PATH):
-        newest = max(os.path.getmtime(s) for s in srcs)
-        if os.path.getmtime(LIB_PATH) >= newest:
-            return LIB_PATH
+    """Compile ``libinsitu_b200.so`` in-tree for sm_100a: the translation units
+    that changed, side by side, then the link."""
+    def mtime(path):
+        return os.path.getmtime(path) if os.path.exists(path) else -1.0
+
+    objdir = os.path.join(HERE, "build")
+    os.makedirs(objdir, exist_ok=True)
+    running, objects = [], []
+    for unit, headers in UNITS.items():
+        obj = os.path.join(objdir, os.path.basename(unit) + ".o")
+        objects.append(obj)
+        newest = max(mtime(os.path.join(HERE, s)) for s in (unit, *headers))
+        if not force and mtime(obj) >= max(newest, mtime(HEADER)):
+            continue
+        cmd = [nvcc(), *NVCC_FLAGS, "-c", "-o", obj + ".tmp", os.path.join(HERE, unit)]
+        if verbose:
+            print(" ".join(cmd))
+        running.append((subprocess.Popen(cmd, cwd=HERE), cmd, obj))
+    failed = [cmd for proc, cmd, _ in running if proc.wait()]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    for _, _, obj in running:
+        os.replace(obj + ".tmp", obj)
+    if not running and mtime(LIB_PATH) >= max(mtime(o) for o in objects):
+        return LIB_PATH
     tmp = LIB_PATH + ".tmp"
-    cmd = [nvcc(), *NVCC_FLAGS, "-o", tmp, os.path.join(HERE, "csrc", "insitu.cu")]
+    cmd = [nvcc(), *LINK_FLAGS, "-o", tmp, *objects]
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True, cwd=HERE)
@@ -233,6 +262,14 @@ def lib():
     L.ins_project.argtypes = [i32, i32, i32, vp, vp, vp, vp, vp]
     L.ins_cache_launches.argtypes = [vp]
     L.ins_cache_launches.restype = i64
+    L.ins_cache_free_pages.argtypes = [vp]
+    L.ins_cache_free_pages.restype = i64
+    L.ins_cache_fork.argtypes = [vp, i32, vp, vp, vp, vp]
+    L.ins_cache_compact.argtypes = [vp, i32, vp, vp, vp, vp, vp]
+    L.ins_cache_truncate.argtypes = [vp, i32, vp, vp, vp]
+    L.ins_cache_rows.argtypes = [vp, i32, vp, vp, vp, vp, vp]
+    L.ins_cache_put_rows.argtypes = [vp, i32, vp, vp, vp, vp]
+    L.ins_sample.argtypes = [i32, i32, vp, i32, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp]
     L.ins_last_error.restype = C.c_char_p
     _lib = L
     return L

@@ -13,6 +13,7 @@
 #include <mutex>
 #include <vector>
 
+#include "cache.h"
 #include "common.cuh"
 #include "kernels.cuh"
 #include "scan_chunked.cuh"
@@ -21,119 +22,15 @@
 
 using namespace ins;
 
-namespace {
+static thread_local std::string g_err;
 
-thread_local std::string g_err;
-
-int fail(int code, const std::string &msg) {
+int ins::fail(int code, const std::string &msg) {
     g_err = msg;
     return code;
 }
 
-#define CK(call)                                                                       \
-    do {                                                                               \
-        cudaError_t e_ = (call);                                                       \
-        if (e_ != cudaSuccess)                                                         \
-            return fail(INS_ECUDA, std::string(#call " failed: ") + cudaGetErrorString(e_)); \
-    } while (0)
-
-struct DeviceGuard {
-    int prev = -1;
-    explicit DeviceGuard(int dev) {
-        cudaGetDevice(&prev);
-        if (prev != dev) cudaSetDevice(dev);
-    }
-    ~DeviceGuard() {
-        int cur = -1;
-        cudaGetDevice(&cur);
-        if (prev >= 0 && cur != prev) cudaSetDevice(prev);
-    }
-};
-
-// Per-call uploads (sequence ids, slots, plans, positions) go through a ring
-// of pinned host / device buffer pairs. reserve() moves to the next slot and
-// waits only for that slot's previous copy, so the host can run NSLOT calls
-// ahead of the GPU rather than one; host writes into a slot wait on that
-// slot's last copy, so an enqueued copy never reads a half-rewritten area. A
-// slot that must grow takes the whole ring with it, so that steady-state
-// calls never allocate.
-struct Staging {
-    static constexpr int NSLOT = 4;
-    struct Slot {
-        void *h = nullptr;
-        void *d = nullptr;
-        cudaEvent_t done = nullptr;
-    };
-    Slot ring[NSLOT];
-    size_t cap = 0;                     // every slot's size
-    int cur = NSLOT - 1;
-    void *h = nullptr;                  // the current slot's buffers
-    void *d = nullptr;
-    int64_t *launches = nullptr;        // the cache's kernel count (an upload may be a launch)
-
-    int reserve(size_t bytes) {
-        cur = (cur + 1) % NSLOT;
-        Slot &sl = ring[cur];
-        if (!sl.done) CK(cudaEventCreateWithFlags(&sl.done, cudaEventDisableTiming));
-        CK(cudaEventSynchronize(sl.done));
-        if (bytes > cap) {
-            size_t want = cap ? cap : 4096;
-            while (want < bytes) want *= 2;
-            for (Slot &o : ring) {
-                if (o.done) CK(cudaEventSynchronize(o.done));
-                if (o.h) cudaFreeHost(o.h);
-                if (o.d) cudaFree(o.d);
-                o.h = o.d = nullptr;
-            }
-            cap = 0;
-            for (Slot &o : ring) {
-                CK(cudaHostAlloc(&o.h, want, cudaHostAllocDefault));
-                CK(cudaMalloc(&o.d, want));
-            }
-            cap = want;
-        }
-        h = sl.h;
-        d = sl.d;
-        return INS_OK;
-    }
-    int upload(size_t bytes, cudaStream_t s) {
-        int launched = 0;
-        CK(small_upload(d, h, bytes, s, &launched));
-        if (launched && launches) *launches += 1;
-        CK(cudaEventRecord(ring[cur].done, s));
-        return INS_OK;
-    }
-    void release() {
-        for (Slot &o : ring) {
-            if (o.done) cudaEventSynchronize(o.done), cudaEventDestroy(o.done);
-            if (o.h) cudaFreeHost(o.h);
-            if (o.d) cudaFree(o.d);
-            o = Slot();
-        }
-        h = d = nullptr;
-        cap = 0;
-    }
-};
-
-}  // namespace
-
-struct ins_cache {
-    ins_config cfg;
-    Geo g;
-    int device = 0;
-    DevTables *d_tables = nullptr;
-    uint8_t *d_pool = nullptr;
-    int32_t *d_page_table = nullptr;   // [max_seqs, max_pages]
-    int32_t *d_status = nullptr;
+struct ins_cache : ins::CacheBase {
     unsigned long long *d_redo_total = nullptr;   // items the sequential kernel recomputed, running
-    // host mirrors (pinned, so their copies can be asynchronous)
-    int32_t *h_page_table = nullptr;
-    int32_t *h_seq_lens = nullptr;
-    cudaEvent_t mirror_done = nullptr;
-    std::vector<int32_t> free_pages;
-    Staging stage_a;                    // per-call index uploads
-    Staging stage_b;
-    Staging stage_c;                    // positions of ins_seam
     ChunkScratch chunk;                 // scratch of the context-parallel scan
     uint64_t gen = 0;                   // bumped by every call that rewrites `chunk`
     struct {                            // context split: phase 1 waiting for phase 2
@@ -147,6 +44,8 @@ struct ins_cache {
         ChunkArgs a{};
     } split;
 };
+
+ins::CacheBase *ins::cache_base(ins_cache *c) { return c; }
 
 namespace {
 
@@ -230,7 +129,7 @@ int push_mirrors(ins_cache *c, cudaStream_t s, int32_t seq_lo, int32_t seq_hi) {
 }
 
 int64_t capacity_of(const ins_cache *c) {
-    return (int64_t)c->cfg.max_pages_per_seq * c->cfg.page_tokens;
+    return c->capacity();
 }
 
 // Reserve slots for n tokens appended to their sequences in order. On
@@ -273,8 +172,7 @@ int reserve_slots(ins_cache *c, int32_t n, const int32_t *seq_ids, int64_t *slot
         const size_t at = (size_t)s * row + (size_t)(pos / P);
         int32_t &pg = c->h_page_table[at];
         if (pos % P == 0) {
-            pg = c->free_pages.back();
-            c->free_pages.pop_back();
+            pg = c->open_page();
             if (pt_new) pt_new[(*n_new)++] = make_int2((int32_t)at, pg);
         }
         slots[i] = (int64_t)pg * P + pos % P;
@@ -402,10 +300,12 @@ int ins_cache_create(const ins_config *cfg, const ins_tables *tb, int32_t device
     if (cudaEventCreateWithFlags(&c->mirror_done, cudaEventDisableTiming) != cudaSuccess)
         return cleanup(fail(INS_ECUDA, "event creation failed"));
     c->chunk.redo_total = c->d_redo_total;
-    c->stage_a.launches = c->stage_b.launches = c->stage_c.launches = &c->chunk.launches;
+    c->launches = &c->chunk.launches;
+    c->stage_a.launches = c->stage_b.launches = c->stage_c.launches = c->stage_p.launches = c->launches;
     std::memset(c->h_page_table, 0xff, sizeof(int32_t) * pt);
     std::memset(c->h_seq_lens, 0, sizeof(int32_t) * cfg->max_seqs);
     c->free_pages.reserve((size_t)cfg->n_pages);
+    c->page_refs.assign((size_t)cfg->n_pages, 0);
     for (int64_t p = cfg->n_pages - 1; p >= 0; --p) c->free_pages.push_back((int32_t)p);
     if (cudaMemcpy(c->d_tables, &ht, sizeof(ht), cudaMemcpyHostToDevice) != cudaSuccess ||
         cudaMemcpy(c->d_page_table, c->h_page_table, sizeof(int32_t) * pt, cudaMemcpyHostToDevice) !=
@@ -426,6 +326,7 @@ int ins_cache_destroy(ins_cache *c) {
     c->stage_a.release();
     c->stage_b.release();
     c->stage_c.release();
+    c->stage_p.release();
     c->chunk.release();
     if (c->mirror_done) cudaEventDestroy(c->mirror_done);
     cudaFree(c->d_tables);
@@ -485,7 +386,7 @@ int ins_cache_reset(ins_cache *c, int32_t seq) {
     for (int32_t s = lo; s < hi; ++s) {
         for (size_t p = 0; p < row; ++p) {
             int32_t &pg = c->h_page_table[(size_t)s * row + p];
-            if (pg >= 0) c->free_pages.push_back(pg);
+            if (pg >= 0) c->release_page(pg);
             pg = -1;
         }
         c->h_seq_lens[s] = 0;

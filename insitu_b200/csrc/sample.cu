@@ -1,0 +1,473 @@
+// Sampling one token per row of logits: temperature, top-k, top-p, min-p, and
+// the draw itself from given uniform random numbers.
+//
+// With z_i = x_i / t and w_i = exp(z_i - max z), a row keeps the k largest x
+// (ties: the lowest indexes), of those the shortest leading run, in falling
+// order of x, whose mass reaches top_p of theirs, of those the ones with
+// w_i >= min_p; the token is the kept i with the largest z_i - log(-log u_i),
+// which is distributed as the kept w_i normalised.
+//
+// No sort: both cuts are order statistics (by count, by mass), found by
+// histograms that narrow a range of values. The row's logits are read from
+// memory once, into the shared memory of a thread-block cluster (each CTA a
+// contiguous slice of the vocabulary); the later passes read them there, and
+// the CTAs exchange histograms through distributed shared memory. A cut needs
+// the exact order of the values, so the histograms' last levels work on the
+// values' bits, and on the indexes where equal values are split.
+//
+// Masses are summed as integers, w_i rounded to 2^-31 (64-bit totals): the
+// result then does not depend on the order of the atomics, and the rounding
+// (2^-32 a token at most, against a largest w of 1) moves the total of
+// 128,000 tokens by some 1e-8 of it.
+//
+// Bound: one read of the logits (and of the random numbers, where a row is
+// not filtered); at a few rows the passes' latency.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <climits>
+
+#include "cache.h"
+
+namespace ins {
+namespace cg = cooperative_groups;
+
+constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32, SMP_BINS = 256;
+constexpr int SMP_MAX_VOCAB = 1 << 18;
+constexpr int SMP_WINDOWS = 4;               // first-level windows of 8 nats each, the last one open
+
+struct SampleArgs {
+    const void *logits;
+    int64_t stride;
+    const float *uniform;
+    int64_t u_stride;
+    const float *temperature, *top_p, *min_p;
+    const int32_t *top_k;
+    int64_t *tokens;
+    float *logprobs;
+    int32_t vocab, slice;
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// Logits as the order sees them: NaN counts as masked (-inf), -0 as 0.
+__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
+
+// Unsigned integers in the order of the floats.
+__device__ __forceinline__ uint32_t order_key(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+// What a CTA publishes to its cluster; two copies, used in turn, so that one
+// cluster barrier a step is enough.
+struct SampleShared {
+    uint32_t cnt[2][SMP_BINS], lo[2][SMP_BINS], hi[2][SMP_BINS];
+    unsigned long long sum[2];
+    float val[2];
+    int32_t idx[2];
+    // this CTA only
+    unsigned long long wsum[SMP_WARPS];
+    float wval[SMP_WARPS];
+    int32_t widx[SMP_WARPS];
+    uint32_t scan_c[SMP_BINS / 32];
+    unsigned long long scan_m[SMP_BINS / 32];
+    int32_t hit_bin;
+    uint32_t hit_cnt, hit_before_c;
+    unsigned long long hit_mass, hit_before_m;
+    uint32_t key_lo, key_hi;
+};
+
+template <typename T>
+struct Row {
+    SampleShared &sm;
+    cg::cluster_group cl;
+    const T *slice;                          // this CTA's logits, in shared memory
+    int n, first, parity, C;
+    float xmax, z0, t;
+    // kept so far: value key above thr_key, or equal to it at an index up to thr_idx
+    uint32_t thr_key;
+    int32_t thr_idx;
+
+    __device__ __forceinline__ float x_at(int i) const { return clean(to_f32(slice[i])); }
+    __device__ __forceinline__ float z_of(float x) const {
+        const float z = __fsub_rn(__fdiv_rn(x, t), z0);
+        return x == xmax ? 0.0f : z == z ? z : -INFINITY;   // both quotients beyond the float range: NaN
+    }
+    __device__ __forceinline__ bool kept(float x, uint32_t key, int i) const {
+        return x > -INFINITY && (key > thr_key || (key == thr_key && first + i <= thr_idx));
+    }
+    // w in units of 2^-31
+    __device__ __forceinline__ uint32_t mass_of(float x) const {
+        return __float2uint_rn(expf(z_of(x)) * 2147483648.0f);
+    }
+    // First-level bin: the distance below the maximum in 1/32 of t. Rounding
+    // is monotone, so the bins are ranges of values.
+    __device__ __forceinline__ int bin_of(float x) const {
+        const float d = x == xmax ? 0.0f : xmax - x;
+        return min(__float2int_rz(d * __fdiv_rn(32.0f, t)), SMP_WINDOWS * SMP_BINS - 1);
+    }
+
+    // Sums of the cluster, for every thread.
+    __device__ unsigned long long cluster_sum(unsigned long long v) {
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+        if (threadIdx.x % 32 == 0) sm.wsum[threadIdx.x / 32] = v;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            unsigned long long s = 0;
+            for (int w = 0; w < SMP_WARPS; ++w) s += sm.wsum[w];
+            sm.sum[parity] = s;
+        }
+        cl.sync();
+        unsigned long long s = 0;
+        for (int r = 0; r < C; ++r) s += *cl.map_shared_rank(&sm.sum[parity], r);
+        parity ^= 1;
+        return s;
+    }
+    // The largest value of the cluster and the lowest index that has it.
+    __device__ void cluster_best(float &v, int &i) {
+        auto better = [](float a, int ai, float b, int bi) { return a > b || (a == b && ai < bi); };
+        for (int o = 16; o; o >>= 1) {
+            const float ov = __shfl_xor_sync(FULL, v, o);
+            const int oi = __shfl_xor_sync(FULL, i, o);
+            if (better(ov, oi, v, i)) v = ov, i = oi;
+        }
+        if (threadIdx.x % 32 == 0) sm.wval[threadIdx.x / 32] = v, sm.widx[threadIdx.x / 32] = i;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < SMP_WARPS; ++w)
+                if (better(sm.wval[w], sm.widx[w], v, i)) v = sm.wval[w], i = sm.widx[w];
+            sm.val[parity] = v;
+            sm.idx[parity] = i;
+        }
+        cl.sync();
+        v = -INFINITY, i = INT_MAX;
+        for (int r = 0; r < C; ++r) {
+            const float ov = *cl.map_shared_rank(&sm.val[parity], r);
+            const int oi = *cl.map_shared_rank(&sm.idx[parity], r);
+            if (better(ov, oi, v, i)) v = ov, i = oi;
+        }
+        parity ^= 1;
+    }
+
+    __device__ void clear() {
+        __syncthreads();
+        for (int b = threadIdx.x; b < SMP_BINS; b += SMP_THREADS)
+            sm.cnt[parity][b] = sm.lo[parity][b] = sm.hi[parity][b] = 0;
+        __syncthreads();
+    }
+    __device__ __forceinline__ void count(int b, uint32_t mass) {
+        atomicAdd(&sm.cnt[parity][b], 1u);
+        if (mass) {
+            atomicAdd(&sm.lo[parity][b], mass & 0xffffu);
+            atomicAdd(&sm.hi[parity][b], mass >> 16);
+        }
+    }
+    // Adds the cluster's histograms up and finds the first bin at which the
+    // running count reaches need_c (BY_MASS: the running mass need_m).
+    // Returns it (SMP_BINS: none) with the bin's own count and the totals
+    // before it (all of them where there is none).
+    template <bool BY_MASS>
+    __device__ int crossing(uint32_t need_c, unsigned long long need_m, uint32_t &before_c,
+                            unsigned long long &before_m, uint32_t &in_c) {
+        cl.sync();
+        uint32_t c = 0, ic = 0;
+        unsigned long long m = 0, im = 0;
+        const int b = threadIdx.x, lane = b % 32;
+        if (b < SMP_BINS) {
+            for (int r = 0; r < C; ++r) {
+                c += cl.map_shared_rank(&sm.cnt[parity][0], r)[b];
+                if (BY_MASS)
+                    m += cl.map_shared_rank(&sm.lo[parity][0], r)[b] +
+                         ((unsigned long long)cl.map_shared_rank(&sm.hi[parity][0], r)[b] << 16);
+            }
+            ic = c, im = m;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t pc = __shfl_up_sync(FULL, ic, o);
+                const unsigned long long pm = __shfl_up_sync(FULL, im, o);
+                if (lane >= o) ic += pc, im += pm;
+            }
+            if (lane == 31) sm.scan_c[b / 32] = ic, sm.scan_m[b / 32] = im;
+        }
+        if (b == 0) sm.hit_bin = SMP_BINS;
+        __syncthreads();
+        if (b < SMP_BINS) {
+            for (int w = 0; w < b / 32; ++w) ic += sm.scan_c[w], im += sm.scan_m[w];
+            const bool before = BY_MASS ? im - m < need_m : ic - c < need_c;
+            const bool after = BY_MASS ? im >= need_m : ic >= need_c;
+            if (before && after) sm.hit_bin = b, sm.hit_cnt = c, sm.hit_before_c = ic - c, sm.hit_before_m = im - m;
+            if (b == SMP_BINS - 1 && !after) sm.hit_before_c = ic, sm.hit_before_m = im, sm.hit_cnt = 0;
+        }
+        __syncthreads();
+        before_c = sm.hit_before_c;
+        before_m = sm.hit_before_m;
+        in_c = sm.hit_cnt;
+        parity ^= 1;
+        return sm.hit_bin;
+    }
+
+    // The smallest (LOW) or largest key whose value lies in first-level bin
+    // `bin`, by a 32-way search of one warp over all keys of non-masked values.
+    template <bool LOW>
+    __device__ uint32_t bin_edge(int bin) const {
+        uint32_t a = order_key(-INFINITY) + 1, b = order_key(xmax);   // the answer lies in [a, b]
+        const int lane = threadIdx.x % 32;
+        while (a < b) {
+            const uint32_t step = (b - a) / 32 + 1;
+            // bins fall as keys rise: LOW wants the first key at or below `bin`
+            // (as a bin number), the other the last one at or above it
+            const uint64_t at = LOW ? (uint64_t)a + (uint64_t)step * (lane + 1) - 1 : (uint64_t)a + (uint64_t)step * lane;
+            const bool in = at <= b;
+            const int v = bin_of(key_value(in ? (uint32_t)at : b));
+            if (LOW) {
+                const unsigned ok = __ballot_sync(FULL, !in || v <= bin);
+                const int l = __ffs(ok) - 1;             // lane 31's `at` is b or beyond: always ok
+                const uint64_t hi = (uint64_t)a + (uint64_t)step * (l + 1) - 1;
+                const uint64_t lo = (uint64_t)a + (uint64_t)step * l;
+                b = (uint32_t)(hi < b ? hi : b);
+                a = (uint32_t)lo;
+            } else {
+                const unsigned ok = __ballot_sync(FULL, in && v >= bin);
+                const int l = 31 - __clz(ok);            // lane 0's `at` is a: always ok
+                const uint64_t hi = (uint64_t)a + (uint64_t)step * (l + 1) - 1;
+                a = (uint32_t)((uint64_t)a + (uint64_t)step * l);
+                b = (uint32_t)(hi < b ? hi : b);
+            }
+        }
+        return a;
+    }
+
+    // Narrows the kept set to its first need_c tokens (BY_MASS: the shortest
+    // run whose mass reaches need_m), in falling order of value, ties by index.
+    template <bool BY_MASS>
+    __device__ void cut(uint32_t need_c, unsigned long long need_m) {
+        uint32_t before_c, in_c;
+        unsigned long long before_m;
+        int bin = SMP_BINS, win = 0;
+        for (; win < SMP_WINDOWS; ++win) {
+            clear();
+            for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
+                const float x = x_at(i);
+                if (!kept(x, order_key(x), i)) continue;
+                const int b = bin_of(x) - win * SMP_BINS;
+                if (b >= 0 && b < SMP_BINS) count(b, BY_MASS ? mass_of(x) : 0u);
+            }
+            bin = crossing<BY_MASS>(need_c, need_m, before_c, before_m, in_c);
+            need_c -= before_c;
+            need_m -= before_m;
+            if (bin < SMP_BINS) break;
+        }
+        if (bin == SMP_BINS) return;                    // fewer tokens than asked for: all stay
+        if (threadIdx.x < 32) {
+            const uint32_t e = bin_edge<true>(win * SMP_BINS + bin);
+            if (threadIdx.x == 0) sm.key_lo = e;
+        } else if (threadIdx.x < 64) {
+            const uint32_t e = bin_edge<false>(win * SMP_BINS + bin);
+            if (threadIdx.x == 32) sm.key_hi = e;
+        }
+        __syncthreads();
+        uint32_t a = max(sm.key_lo, thr_key), b = sm.key_hi;
+        // the run ends inside [a, b], in_c tokens of which need_c (need_m) are wanted
+        auto whole = [&] { return BY_MASS ? in_c == 1 : in_c == need_c; };
+        while (a < b && !whole()) {
+            const int sh = max(0, 32 - __clz(b - a) - 8);
+            clear();
+            for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
+                const float x = x_at(i);
+                const uint32_t key = order_key(x);
+                if (key < a || key > b || !kept(x, key, i)) continue;
+                count((int)((b - key) >> sh), BY_MASS ? mass_of(x) : 0u);
+            }
+            const int c = crossing<BY_MASS>(need_c, need_m, before_c, before_m, in_c);
+            need_c -= before_c;
+            need_m -= before_m;
+            b -= (uint32_t)c << sh;
+            a = max(a, b - min(b, (1u << sh) - 1u));
+        }
+        int ties = INT_MAX;
+        if (!whole()) {
+            // a == b: equal values, of which the first `need` indexes stay
+            uint32_t need = need_c;
+            if (BY_MASS) {
+                const uint32_t q = max(1u, mass_of(key_value(a)));
+                need = (uint32_t)min((unsigned long long)in_c, (need_m + q - 1) / q);
+            }
+            int ia = 0, ib = SMP_MAX_VOCAB - 1;
+            while (need != in_c && ia < ib) {
+                const int sh = max(0, 32 - __clz(ib - ia) - 8);
+                clear();
+                for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
+                    const float x = x_at(i);
+                    if (order_key(x) != a || first + i < ia || first + i > ib || !kept(x, a, i)) continue;
+                    count((first + i - ia) >> sh, 0u);
+                }
+                const int c = crossing<false>(need, 0, before_c, before_m, in_c);
+                need -= before_c;
+                ia += c << sh;
+                ib = min(ib, ia + (1 << sh) - 1);
+            }
+            ties = ib;
+        }
+        // an earlier cut may have split the same ties
+        thr_idx = a == thr_key ? min(thr_idx, ties) : ties;
+        thr_key = a;
+    }
+};
+
+// Copies n elements from global memory into shared memory at the same
+// alignment within 16 bytes; returns where they start.
+template <typename T>
+__device__ __forceinline__ const T *stage_slice(uint8_t *smem, const T *src, int n) {
+    constexpr int V = 16 / sizeof(T);
+    const int shift = (int)(((uintptr_t)src & 15u) / sizeof(T));
+    T *dst = reinterpret_cast<T *>(smem) + shift;
+    const int head = min(n, (V - shift) % V), body = (n - head) / V;
+    for (int i = threadIdx.x; i < head; i += SMP_THREADS) dst[i] = src[i];
+    const uint4 *vs = reinterpret_cast<const uint4 *>(src + head);
+    uint4 *vd = reinterpret_cast<uint4 *>(dst + head);
+#pragma unroll 8
+    for (int i = threadIdx.x; i < body; i += SMP_THREADS) vd[i] = __ldcs(vs + i);
+    for (int i = head + body * V + threadIdx.x; i < n; i += SMP_THREADS) dst[i] = src[i];
+    __syncthreads();
+    return dst;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SMP_THREADS) k_sample(const SampleArgs a) {
+    extern __shared__ __align__(16) uint8_t dyn[];
+    __shared__ SampleShared sm;
+    wait_prior_grid();
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    const int64_t row = blockIdx.x / C;
+    const int first = min(rank * a.slice, a.vocab), n = min(a.slice, a.vocab - first);
+    const T *src = reinterpret_cast<const T *>(a.logits) + row * a.stride + first;
+    Row<T> R{sm, cl, stage_slice<T>(dyn, src, n), n, first, 0, C, 0.0f, 0.0f, 1.0f, 0u, INT_MAX};
+
+    float best = -INFINITY;
+    int at = INT_MAX;
+    for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
+        const float x = R.x_at(i);
+        if (x > best) best = x, at = first + i;
+    }
+    R.cluster_best(best, at);
+    const float t = a.temperature ? a.temperature[row] : 1.0f;
+    if (!(best > -INFINITY) || !(t > 0.0f)) {
+        // nothing to choose from, or the largest logit
+        const bool none = !(best > -INFINITY);
+        if (rank == 0 && threadIdx.x == 0) {
+            a.tokens[row] = none ? -1 : at;
+            if (a.logprobs) a.logprobs[row] = none ? -INFINITY : 0.0f;
+        }
+        cl.sync();
+        return;
+    }
+    R.xmax = best;
+    R.t = t;
+    R.z0 = __fdiv_rn(best, t);
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.0f, floor_w = a.min_p ? a.min_p[row] : 0.0f;
+    if (k > 0 && k < a.vocab) R.template cut<false>((uint32_t)k, 0);
+    if (p < 1.0f) {
+        unsigned long long mass = 0;
+        for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
+            const float x = R.x_at(i);
+            if (R.kept(x, order_key(x), i)) mass += R.mass_of(x);
+        }
+        mass = R.cluster_sum(mass);
+        const double want = ceil((double)p * (double)mass);
+        R.template cut<true>(0, want > 1.0 ? (unsigned long long)want : 1ull);
+    }
+    unsigned long long mass = 0;
+    float key = -INFINITY, z_key = 0.0f;
+    int token = INT_MAX;
+    const float *u = a.uniform + row * a.u_stride + first;
+    for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
+        const float x = R.x_at(i);
+        if (!R.kept(x, order_key(x), i)) continue;
+        const float z = R.z_of(x), w = expf(z);
+        if (!(w >= floor_w)) continue;
+        mass += __float2uint_rn(w * 2147483648.0f);
+        float r = z - logf(-logf(__ldcs(u + i)));
+        r = r == r ? r : -INFINITY;                        // a random number outside [0, 1]
+        if (r > key || token == INT_MAX) key = r, token = first + i, z_key = z;
+    }
+    const int mine = token;
+    R.cluster_best(key, token);
+    mass = R.cluster_sum(mass);
+    if (mine == token && token != INT_MAX) {
+        a.tokens[row] = token;
+        if (a.logprobs) a.logprobs[row] = (float)((double)z_key - log((double)mass * 0x1p-31));
+    }
+    cl.sync();
+}
+
+namespace {
+
+template <typename T>
+int launch_sample(SampleArgs a, int32_t rows, cudaStream_t s) {
+    int dev = 0, sms = 148;
+    CK(cudaGetDevice(&dev));
+    CK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    // A cluster of up to 8 CTAs a row: as many as a vocabulary slice of 2,048
+    // tokens each leaves, until the rows alone give every SM two CTAs and the
+    // slice fits.
+    int C = 1;
+    auto bytes = [&](int c) {
+        const int slice = (a.vocab + c - 1) / c;
+        return (size_t)slice * sizeof(T) + 32;
+    };
+    while (C < 8 && (bytes(C) > 72 * 1024 || ((int64_t)rows * C < 2 * sms && a.vocab / C > 2048))) C *= 2;
+    a.slice = (a.vocab + C - 1) / C;
+    const size_t smem = bytes(C);
+    CK(cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * C));
+    cfg.blockDim = dim3(SMP_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    CK(cudaLaunchKernelEx(&cfg, k_sample<T>, a));
+    return INS_OK;
+}
+
+}  // namespace
+}  // namespace ins
+
+using namespace ins;
+
+extern "C" int ins_sample(int32_t rows, int32_t vocab, const void *logits, int32_t dtype, int64_t stride,
+                          const float *uniform, int64_t uniform_stride, const float *temperature,
+                          const int32_t *top_k, const float *top_p, const float *min_p, int64_t *tokens,
+                          float *logprobs, void *stream) {
+    return guarded([&]() -> int {
+        if (rows < 0 || vocab < 1 || vocab > SMP_MAX_VOCAB || rows > INT_MAX / 8)
+            return fail(INS_EINVAL, "sample: rows >= 0, vocab in [1, 262144]");
+        if (dtype != INS_F32 && dtype != INS_F16 && dtype != INS_BF16)
+            return fail(INS_EINVAL, "sample: logits are INS_F32, INS_F16 or INS_BF16");
+        if (rows == 0) return INS_OK;
+        if (!logits || !uniform || !tokens) return fail(INS_EINVAL, "sample: NULL buffer");
+        if (stride < 0 || uniform_stride < 0) return fail(INS_EINVAL, "sample: a negative row stride");
+        if ((uintptr_t)logits % (dtype == INS_F32 ? 4 : 2) || (uintptr_t)uniform % 4)
+            return fail(INS_EINVAL, "sample: a buffer is not aligned to its elements");
+        const SampleArgs a{logits, stride, uniform, uniform_stride, temperature, top_p, min_p,
+                           top_k,  tokens, logprobs, vocab, 0};
+        cudaStream_t s = (cudaStream_t)stream;
+        if (dtype == INS_F32) return launch_sample<float>(a, rows, s);
+        if (dtype == INS_F16) return launch_sample<__half>(a, rows, s);
+        return launch_sample<__nv_bfloat16>(a, rows, s);
+    });
+}

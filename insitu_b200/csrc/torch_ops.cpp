@@ -140,9 +140,135 @@ at::Tensor project(const at::Tensor &w16, const at::Tensor &x, const c10::option
     return y;
 }
 
+int32_t n_ids(at::IntArrayRef ids) {
+    TORCH_CHECK(ids.size() <= INT32_MAX, "insitu: too many sequences");
+    return static_cast<int32_t>(ids.size());
+}
+
+// ins_cache_fork, ins_cache_compact, ins_cache_truncate: the page operations
+// of a decode step. `anchor` is a tensor on the cache's device, which selects
+// the device and its current stream.
+void fork(int64_t h, const at::Tensor &anchor, at::IntArrayRef src, at::IntArrayRef dst,
+          c10::optional<at::IntArrayRef> lengths) {
+    c10::cuda::CUDAGuard guard(anchor.device());
+    TORCH_CHECK_VALUE(src.size() == dst.size() && (!lengths || lengths->size() == src.size()),
+                      "insitu: src, dst and lengths disagree on their number");
+    const std::vector<int32_t> s = ids32(src), d = ids32(dst);
+    check(ins_cache_fork(handle(h), n_ids(src), s.data(), d.data(), lengths ? lengths->data() : nullptr,
+                         at::cuda::getCurrentCUDAStream().stream()));
+}
+
+void compact(int64_t h, const at::Tensor &anchor, at::IntArrayRef seq_ids, at::IntArrayRef base,
+             at::IntArrayRef counts, const at::Tensor &keep) {
+    c10::cuda::CUDAGuard guard(anchor.device());
+    TORCH_CHECK_VALUE(base.size() == seq_ids.size() && counts.size() == seq_ids.size(),
+                      "insitu: seq_ids, base and keep disagree on their number");
+    TORCH_CHECK_VALUE(keep.device().is_cpu() && keep.scalar_type() == at::kLong && keep.is_contiguous(),
+                      "insitu: keep must be a contiguous int64 host tensor");
+    int64_t total = 0;
+    for (const int64_t n : counts) {
+        TORCH_CHECK_VALUE(n >= 0 && n <= keep.numel(), "insitu: a count outside keep");
+        total += n;
+    }
+    TORCH_CHECK_VALUE(total == keep.numel(), "insitu: the counts do not add up to keep's length");
+    const std::vector<int32_t> s = ids32(seq_ids);
+    check(ins_cache_compact(handle(h), n_ids(seq_ids), s.data(), base.data(), counts.data(),
+                            keep.data_ptr<int64_t>(), at::cuda::getCurrentCUDAStream().stream()));
+}
+
+void truncate(int64_t h, const at::Tensor &anchor, at::IntArrayRef seq_ids, at::IntArrayRef lengths) {
+    c10::cuda::CUDAGuard guard(anchor.device());
+    TORCH_CHECK_VALUE(lengths.size() == seq_ids.size(), "insitu: seq_ids and lengths disagree on their number");
+    const std::vector<int32_t> s = ids32(seq_ids);
+    check(ins_cache_truncate(handle(h), n_ids(seq_ids), s.data(), lengths.data(),
+                             at::cuda::getCurrentCUDAStream().stream()));
+}
+
+// ins_cache_rows into a new (sum n, n_kv, row_bytes) uint8 tensor.
+at::Tensor rows(int64_t h, const at::Tensor &anchor, at::IntArrayRef seq_ids, at::IntArrayRef t0, at::IntArrayRef n,
+                int64_t n_kv, int64_t row_bytes) {
+    c10::cuda::CUDAGuard guard(anchor.device());
+    TORCH_CHECK_VALUE(t0.size() == seq_ids.size() && n.size() == seq_ids.size(),
+                      "insitu: seq_ids, t0 and n disagree on their number");
+    int64_t total = 0;
+    for (const int64_t k : n) {
+        TORCH_CHECK_VALUE(k >= 0 && k <= INT32_MAX, "insitu: a row count out of range");
+        total += k;
+    }
+    at::Tensor out = at::empty({total, n_kv, row_bytes}, anchor.options().dtype(at::kByte));
+    const std::vector<int32_t> s = ids32(seq_ids);
+    check(ins_cache_rows(handle(h), n_ids(seq_ids), s.data(), t0.data(), n.data(), out.data_ptr<uint8_t>(),
+                         at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+}
+
+void put_rows(int64_t h, at::IntArrayRef seq_ids, at::IntArrayRef n, const at::Tensor &rows) {
+    TORCH_CHECK_VALUE(rows.is_cuda() && rows.scalar_type() == at::kByte && rows.is_contiguous(),
+                      "insitu: rows must be a contiguous uint8 CUDA tensor");
+    TORCH_CHECK_VALUE(n.size() == seq_ids.size(), "insitu: seq_ids and n disagree on their number");
+    int64_t total = 0;
+    for (const int64_t k : n) {
+        TORCH_CHECK_VALUE(k >= 0 && k <= INT32_MAX, "insitu: a row count out of range");
+        total += k;
+    }
+    TORCH_CHECK_VALUE(rows.dim() == 3 && rows.size(0) == total, "insitu: rows must hold ", total, " rows, got ",
+                      rows.sizes());
+    c10::cuda::CUDAGuard guard(rows.device());
+    const std::vector<int32_t> s = ids32(seq_ids);
+    check(ins_cache_put_rows(handle(h), n_ids(seq_ids), s.data(), n.data(), rows.data_ptr<uint8_t>(),
+                             at::cuda::getCurrentCUDAStream().stream()));
+}
+
+// ins_sample: one token per row of logits (rows, vocab); the settings are
+// device tensors of one value a row, or none.
+std::tuple<at::Tensor, at::Tensor> sample(const at::Tensor &logits, const at::Tensor &uniform,
+                                          const c10::optional<at::Tensor> &temperature,
+                                          const c10::optional<at::Tensor> &top_k,
+                                          const c10::optional<at::Tensor> &top_p,
+                                          const c10::optional<at::Tensor> &min_p) {
+    TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) < 2 || logits.stride(1) == 1),
+                      "insitu: logits must be a (rows, vocab) CUDA tensor with adjacent columns");
+    const auto st = logits.scalar_type();
+    TORCH_CHECK_VALUE(st == at::kFloat || st == at::kHalf || st == at::kBFloat16,
+                      "insitu: logits must be float32, float16 or bfloat16, got ", st);
+    const int64_t n = logits.size(0), vocab = logits.size(1);
+    TORCH_CHECK_VALUE(vocab >= 1 && vocab <= (1 << 18) && n <= (1 << 27), "insitu: vocab must be in [1, 262144], got ",
+                      vocab);
+    TORCH_CHECK_VALUE(uniform.device() == logits.device() && uniform.scalar_type() == at::kFloat &&
+                          uniform.sizes() == logits.sizes() && (vocab < 2 || uniform.stride(1) == 1),
+                      "insitu: uniform must be a float32 tensor of logits' shape and device with adjacent columns");
+    auto setting = [&](const c10::optional<at::Tensor> &t, at::ScalarType type, const char *name) -> const void * {
+        if (!t.has_value()) return nullptr;
+        TORCH_CHECK_VALUE(t->device() == logits.device() && t->scalar_type() == type && t->is_contiguous() &&
+                              t->dim() == 1 && t->size(0) == n,
+                          "insitu: ", name, " must be a contiguous ", type, " tensor of ", n,
+                          " values on logits' device");
+        return t->data_ptr();
+    };
+    const auto *t = static_cast<const float *>(setting(temperature, at::kFloat, "temperature"));
+    const auto *k = static_cast<const int32_t *>(setting(top_k, at::kInt, "top_k"));
+    const auto *p = static_cast<const float *>(setting(top_p, at::kFloat, "top_p"));
+    const auto *m = static_cast<const float *>(setting(min_p, at::kFloat, "min_p"));
+    c10::cuda::CUDAGuard guard(logits.device());
+    at::Tensor tokens = at::empty({n}, logits.options().dtype(at::kLong));
+    at::Tensor logprobs = at::empty({n}, logits.options().dtype(at::kFloat));
+    check(ins_sample((int32_t)n, (int32_t)vocab, logits.data_ptr(),
+                     st == at::kFloat ? INS_F32 : st == at::kHalf ? INS_F16 : INS_BF16, logits.stride(0),
+                     uniform.data_ptr<float>(), uniform.stride(0), t, k, p, m, tokens.data_ptr<int64_t>(),
+                     logprobs.data_ptr<float>(), at::cuda::getCurrentCUDAStream().stream()));
+    return {tokens, logprobs};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(insitu, m) {
+    m.def("fork(int handle, Tensor anchor, int[] src, int[] dst, int[]? lengths) -> ()");
+    m.def("compact(int handle, Tensor anchor, int[] seq_ids, int[] base, int[] counts, Tensor keep) -> ()");
+    m.def("truncate(int handle, Tensor anchor, int[] seq_ids, int[] lengths) -> ()");
+    m.def("rows(int handle, Tensor anchor, int[] seq_ids, int[] t0, int[] n, int n_kv, int row_bytes) -> Tensor");
+    m.def("put_rows(int handle, int[] seq_ids, int[] n, Tensor rows) -> ()");
+    m.def("sample(Tensor logits, Tensor uniform, Tensor? temperature, Tensor? top_k, Tensor? top_p, "
+          "Tensor? min_p) -> (Tensor, Tensor)");
     m.def("ingress(int handle, int[] seq_ids, Tensor k, Tensor v, Tensor? q, int n_kv, int q_heads, "
           "bool prerotated) -> Tensor?");
     m.def("scan(int handle, int[] seq_ids, int[]? lengths, Tensor q_rot, int n_kv, int mode, "
@@ -157,4 +283,10 @@ TORCH_LIBRARY_IMPL(insitu, CUDA, m) {
     m.impl("scan", scan);
     m.impl("step", step);
     m.impl("project", project);
+    m.impl("fork", fork);
+    m.impl("compact", compact);
+    m.impl("truncate", truncate);
+    m.impl("rows", rows);
+    m.impl("put_rows", put_rows);
+    m.impl("sample", sample);
 }

@@ -58,6 +58,11 @@ def _ids(x, n: int) -> list:
     return np.broadcast_to(np.asarray(x, dtype=np.int64), (n,)).tolist()
 
 
+def _list(x) -> list:
+    """Sequence ids (a scalar, a sequence or an array) as a list of Python ints."""
+    return x if isinstance(x, list) else np.atleast_1d(np.asarray(x, dtype=np.int64)).tolist()
+
+
 def _raise_mapped(err: Exception):
     """Re-raise an operator's error as the C ABI's exception class for its
     status (the message starts with "[status N]"), e.g. CapacityError."""
@@ -114,6 +119,7 @@ class PagedCache:
         _lib.check(self._L.ins_cache_create(C.byref(self.cfg), C.byref(tb), self.device.index,
                                             C.byref(h)))
         self._h = h
+        self._anchor = torch.empty(0, dtype=torch.int32, device=self.device)   # names the device to operators
         self.max_seqs = max_seqs
         self.page_tokens = page_tokens
         self.row_bytes = self._L.ins_bytes_per_token(C.byref(self.cfg))
@@ -329,6 +335,80 @@ class PagedCache:
         m = {"online": _lib.INS_SOFTMAX_ONLINE, "two_pass": _lib.INS_SOFTMAX_TWO_PASS}[mode]
         try:
             return self._ops.step(self._h.value, _ids(seq_ids, q.shape[0]), q, k, v, g.n_kv_heads, m, stats)
+        except (RuntimeError, ValueError) as e:
+            _raise_mapped(e)
+
+    # -- page operations ------------------------------------------------------------
+    @property
+    def free_pages(self) -> int:
+        """Pages of the pool that no sequence holds."""
+        return int(self._L.ins_cache_free_pages(self._h))
+
+    def fork(self, src, dst, lengths=None) -> None:
+        """Make each sequence of ``dst`` (empty ones) the first ``lengths`` rows
+        (all by default) of the sequence of ``src`` beside it
+        (ins_cache_fork): full pages are shared, the last one is copied."""
+        src, dst = _list(src), _list(dst)
+        lens = None if lengths is None else _ids(lengths, len(dst))
+        try:
+            self._ops.fork(self._h.value or 0, self._anchor, src, dst, lens)
+        except (RuntimeError, ValueError) as e:
+            _raise_mapped(e)
+
+    def compact(self, seq_ids, keep, base=0) -> None:
+        """Keep, of each sequence's rows from ``base`` on (one number, or one a
+        sequence), those at the offsets ``keep`` and move them together; rows
+        below ``base`` stay (ins_cache_compact). ``keep``: one rising sequence
+        of offsets for each of ``seq_ids``, or a 2-D host tensor. Accepting a
+        drafted tree's path is ``compact(seqs, paths, context_lengths)``."""
+        ids = _list(seq_ids)
+        if len(keep) != len(ids):
+            raise ValueError(f"keep holds {len(keep)} sequences' rows for {len(ids)} sequences")
+        if torch.is_tensor(keep):
+            if keep.dim() != 2 or keep.is_floating_point():
+                raise ValueError("keep must be a 2-D integer tensor, or one sequence of offsets a sequence")
+            counts = [keep.shape[1]] * len(ids)
+            flat = keep.to("cpu", torch.int64).reshape(-1).contiguous()
+        else:
+            parts = [np.asarray(k, dtype=np.int64).reshape(-1) for k in keep]
+            counts = [p.size for p in parts]
+            flat = torch.from_numpy(np.concatenate(parts) if parts else np.zeros(0, np.int64))
+        try:
+            self._ops.compact(self._h.value or 0, self._anchor, ids, _ids(base, len(ids)), counts, flat)
+        except (RuntimeError, ValueError) as e:
+            _raise_mapped(e)
+
+    def truncate(self, seq_ids, lengths) -> None:
+        """Keep the first ``lengths`` rows of each sequence and free the pages
+        after them (ins_cache_truncate); 0 frees a sequence without blocking."""
+        ids = _list(seq_ids)
+        try:
+            self._ops.truncate(self._h.value or 0, self._anchor, ids, _ids(lengths, len(ids)))
+        except (RuntimeError, ValueError) as e:
+            _raise_mapped(e)
+
+    def rows(self, seq_ids, t0=0, n=None) -> torch.Tensor:
+        """Rows [t0, t0 + n) of each sequence (to its end by default), one
+        sequence after another, in the packed format on the device:
+        (sum n, n_kv, row_bytes) uint8 (ins_cache_rows)."""
+        ids = _list(seq_ids)
+        first = _ids(t0, len(ids))
+        count = [self.length(s) - f for s, f in zip(ids, first)] if n is None else _ids(n, len(ids))
+        try:
+            return self._ops.rows(self._h.value or 0, self._anchor, ids, first, count, self.geo.n_kv_heads,
+                                  self.row_bytes)
+        except (RuntimeError, ValueError) as e:
+            _raise_mapped(e)
+
+    def put_rows(self, seq_ids, n, rows: torch.Tensor) -> None:
+        """Append packed rows held on the device, ``n`` for each sequence one
+        after another (ins_cache_put_rows): what ``rows`` returned."""
+        ids = _list(seq_ids)
+        if tuple(rows.shape[1:]) != (self.geo.n_kv_heads, self.row_bytes) or rows.device != self.device:
+            raise ValueError(f"expected (n, {self.geo.n_kv_heads}, {self.row_bytes}) rows on {self.device}, "
+                             f"got {tuple(rows.shape)} on {rows.device}")
+        try:
+            self._ops.put_rows(self._h.value or 0, ids, _ids(n, len(ids)), rows.contiguous())
         except (RuntimeError, ValueError) as e:
             _raise_mapped(e)
 
