@@ -447,6 +447,30 @@ int ins_cache_rows(ins_cache *cache, int32_t B, const int32_t *seq_ids, const in
 int ins_cache_put_rows(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int64_t *n,
                        const uint8_t *rows, void *stream);
 
+/* Attention of drafted tokens, in floating point (the reference scans causal
+ * prefixes only, ops/attention.py:451-513). Sequence seq_ids[i]'s last
+ * nodes[i] cached tokens (0 to 256; already appended by an ingress) are a
+ * tree's nodes, the tokens before them its context. Node j attends the whole
+ * context and the nodes whose bits are set in its mask row -- its ancestors
+ * and itself, though any set is taken; a node that sees nothing gives zeros.
+ * With a cached row's key and value norm * centroid[code] in real units and q
+ * its Q(qk_frac) value, out = sum exp(s - m) v / sum exp(s - m) over what the
+ * node sees, s = <q, k>: fp16 products, fp32 sums, maxima and exponents, one
+ * rounding to bf16. A tree of one node is a decode token's attention, and
+ * agrees with the fixed-point scans within their formats' resolution.
+ *
+ * mask: device uint64 [sum nodes][words], bit j % 64 of word j / 64 is node j
+ * of the same sequence; q_rot: device int32 [sum nodes][n_kv*groups][d], as
+ * ins_ingress rotates it, 16-byte aligned; out: device bf16 of that shape,
+ * 16-byte aligned; workspace: device, ins_tree_workspace bytes for the same
+ * cache, seq_ids and nodes (the lengths at the call), 16-byte aligned, free
+ * again once the call's work is done. Any code widths. Stream-ordered; a
+ * bounded wait that gives up latches INS_ETIMEOUT for ins_cache_status. */
+int64_t ins_tree_workspace(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int32_t *nodes);
+int ins_tree_scan(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int32_t *nodes,
+                  const uint64_t *mask, int32_t words, const int32_t *q_rot, void *out,
+                  void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Element types of ins_sample's logits. */
 enum { INS_F32 = 0, INS_F16 = 1, INS_BF16 = 2 };
 

@@ -22,6 +22,7 @@ UNITS = {
                                 "csrc/project.cuh"),
     "csrc/pages.cu": COMMON + ("csrc/plan.cuh",),
     "csrc/sample.cu": COMMON,
+    "csrc/tree.cu": COMMON + ("csrc/plan.cuh",),
 }
 SOURCES = tuple(dict.fromkeys(s for unit, headers in UNITS.items() for s in (unit, *headers)))
 HEADER = os.path.join(ROOT, "include", "insitu_b200.h")
@@ -109,7 +110,8 @@ SYMBOLS = ("ins_abi_version", "ins_bytes_per_token", "ins_cache_create", "ins_ca
            "ins_cache_launches", "ins_finalize", "ins_exp_lut",
            "ins_scan_recomputed_total", "ins_cache_set_scan_kernel", "ins_cache_set_wait_test",
            "ins_project", "ins_cache_free_pages", "ins_cache_fork", "ins_cache_compact",
-           "ins_cache_truncate", "ins_cache_rows", "ins_cache_put_rows", "ins_sample")
+           "ins_cache_truncate", "ins_cache_rows", "ins_cache_put_rows", "ins_sample",
+           "ins_tree_workspace", "ins_tree_scan")
 
 
 def nvcc() -> str:
@@ -270,6 +272,9 @@ def lib():
     L.ins_cache_rows.argtypes = [vp, i32, vp, vp, vp, vp, vp]
     L.ins_cache_put_rows.argtypes = [vp, i32, vp, vp, vp, vp]
     L.ins_sample.argtypes = [i32, i32, vp, i32, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp]
+    L.ins_tree_workspace.argtypes = [vp, i32, vp, vp]
+    L.ins_tree_workspace.restype = i64
+    L.ins_tree_scan.argtypes = [vp, i32, vp, vp, vp, i32, vp, vp, vp, i64, vp]
     L.ins_last_error.restype = C.c_char_p
     _lib = L
     return L

@@ -219,6 +219,34 @@ void put_rows(int64_t h, at::IntArrayRef seq_ids, at::IntArrayRef n, const at::T
                              at::cuda::getCurrentCUDAStream().stream()));
 }
 
+// ins_tree_scan: attention of each sequence's last nodes[i] cached tokens as
+// a drafted tree; q (sum nodes, q_heads, 64) int32 -> the same shape in bf16.
+at::Tensor tree_scan(int64_t h, at::IntArrayRef seq_ids, at::IntArrayRef nodes, const at::Tensor &mask,
+                     const at::Tensor &q, int64_t q_heads) {
+    check_i32(q, "q", q_heads, 64);
+    TORCH_CHECK_VALUE(nodes.size() == seq_ids.size(), "insitu: seq_ids and the trees disagree on their number");
+    int64_t total = 0;
+    for (const int64_t n : nodes) {
+        TORCH_CHECK_VALUE(n >= 0 && n <= INT32_MAX, "insitu: a node count out of range");
+        total += n;
+    }
+    TORCH_CHECK_VALUE(q.size(0) == total, "insitu: q must hold ", total, " nodes, got ", q.size(0));
+    TORCH_CHECK_VALUE(mask.device() == q.device() && mask.scalar_type() == at::kLong && mask.is_contiguous() &&
+                          mask.dim() == 2 && mask.size(0) == total,
+                      "insitu: mask must be a contiguous int64 (nodes, words) tensor on q's device");
+    c10::cuda::CUDAGuard guard(q.device());
+    const std::vector<int32_t> s = ids32(seq_ids), n = ids32(nodes);
+    const int64_t bytes = ins_tree_workspace(handle(h), n_ids(seq_ids), s.data(), n.data());
+    if (bytes < 0) check(INS_EINVAL);
+    at::Tensor out = at::empty(q.sizes(), q.options().dtype(at::kBFloat16));
+    at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+    check(ins_tree_scan(handle(h), n_ids(seq_ids), s.data(), n.data(),
+                        reinterpret_cast<const uint64_t *>(mask.data_ptr<int64_t>()), (int32_t)mask.size(1),
+                        q.data_ptr<int32_t>(), out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
+                        at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+}
+
 // ins_sample: one token per row of logits (rows, vocab); the settings are
 // device tensors of one value a row, or none.
 std::tuple<at::Tensor, at::Tensor> sample(const at::Tensor &logits, const at::Tensor &uniform,
@@ -267,6 +295,7 @@ TORCH_LIBRARY(insitu, m) {
     m.def("truncate(int handle, Tensor anchor, int[] seq_ids, int[] lengths) -> ()");
     m.def("rows(int handle, Tensor anchor, int[] seq_ids, int[] t0, int[] n, int n_kv, int row_bytes) -> Tensor");
     m.def("put_rows(int handle, int[] seq_ids, int[] n, Tensor rows) -> ()");
+    m.def("tree_scan(int handle, int[] seq_ids, int[] nodes, Tensor mask, Tensor q, int q_heads) -> Tensor");
     m.def("sample(Tensor logits, Tensor uniform, Tensor? temperature, Tensor? top_k, Tensor? top_p, "
           "Tensor? min_p) -> (Tensor, Tensor)");
     m.def("ingress(int handle, int[] seq_ids, Tensor k, Tensor v, Tensor? q, int n_kv, int q_heads, "
@@ -288,5 +317,6 @@ TORCH_LIBRARY_IMPL(insitu, CUDA, m) {
     m.impl("truncate", truncate);
     m.impl("rows", rows);
     m.impl("put_rows", put_rows);
+    m.impl("tree_scan", tree_scan);
     m.impl("sample", sample);
 }

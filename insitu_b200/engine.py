@@ -338,6 +338,20 @@ class PagedCache:
         except (RuntimeError, ValueError) as e:
             _raise_mapped(e)
 
+    def tree_scan(self, seq_ids, q_rot, tree) -> torch.Tensor:
+        """Attention of a drafted tree's nodes (an ``insitu_b200.tree.DraftTree``
+        with one tree for each of ``seq_ids``) over each sequence's context and
+        the nodes' ancestors (ins_tree_scan). The nodes are the sequences' last
+        cached tokens, appended by ``ingress``, whose rotated queries
+        ``q_rot`` (nodes, n_kv*groups, d) are. Returns that shape in bfloat16."""
+        g = self.geo
+        q = self._dev_i32(q_rot, (g.num_heads, g.head_dim))
+        try:
+            return self._ops.tree_scan(self._h.value or 0, _list(seq_ids), tree.counts, tree.mask(self.device), q,
+                                       g.num_heads)
+        except (RuntimeError, ValueError) as e:
+            _raise_mapped(e)
+
     # -- page operations ------------------------------------------------------------
     @property
     def free_pages(self) -> int:
