@@ -518,46 +518,701 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
 }
 
 // ---------------------------------------------------------------------------
+// many rows: tcgen05
+// ---------------------------------------------------------------------------
+//
+// One CTA an SM. Its four decode warps turn 128 cached rows at a time into
+// fp16 key and value tiles in shared memory (a thread a row, norms applied),
+// one thread issues the products S = Q K^T and O += P V on the tensor cores,
+// and two groups of four warps (a stream each) turn S into P, a thread a
+// query row. S, P and O stay in tensor memory: 128 + 64 + 64 columns for each
+// stream, all 512.
+//
+// The two streams keep the exponentials (the bound: 16 a clock and SM) busy
+// while the other's products run. With more than 128 query rows they are two
+// row tiles that share every decoded tile (ROWS); with fewer, one row tile
+// whose KV tiles they take in turn, joined when the CTA is done with it.
+//
+// The work is the list of KV tiles of all (sequence, KV head, row group)
+// items, cut into equal runs, one for each CTA; a CTA walks its run's
+// segments. An item that lies in one run is written at once, the others'
+// parts are joined by k_tree_join: at most two partial slots a CTA.
+
+constexpr int MANY_TILE = 128, MANY_STAGES = 3;
+constexpr int MANY_THREADS = 13 * 32;
+constexpr int MANY_LUT = 65536, MANY_KV = MANY_TILE * 128;
+constexpr int MANY_Q_AT = MANY_LUT, MANY_K_AT = MANY_Q_AT + 2 * MANY_KV, MANY_V_AT = MANY_K_AT + MANY_STAGES * MANY_KV;
+// each decode warp's ring of packed rows: 32 rows of 52 bytes a slot (both widths)
+constexpr int MANY_RING = 4, MANY_SLOT = 32 * 52;
+constexpr int MANY_ML_AT = MANY_V_AT + MANY_STAGES * MANY_KV;
+constexpr int MANY_RING_AT = MANY_ML_AT + 128 * 2 * 4;
+constexpr int MANY_BARS_AT = MANY_RING_AT + 4 * MANY_RING * MANY_SLOT;
+constexpr int MANY_SMEM = MANY_BARS_AT + 320 + 1024;     // + the base's alignment to 1,024
+
+// Tile t of the run list -> its CTA, for `tiles` tiles in `ctas` equal runs.
+__host__ __device__ __forceinline__ int run_of(int64_t t, int64_t tiles, int ctas) {
+    return (int)(((t + 1) * ctas - 1) / tiles);
+}
+__host__ __device__ __forceinline__ int64_t run_start(int c, int64_t tiles, int ctas) { return c * tiles / ctas; }
+
+// One CTA's part of one item.
+struct Segment {
+    int seq, head, row0, lo, hi;             // KV tiles [lo, hi) of the item
+    int slot;                                // partial slot, -1: the whole item
+};
+
+// The segment that starts at tile t (< end) of the run.
+__device__ __forceinline__ Segment segment_at(const TreeSeq *seqs, int n_seqs, const Geo &g, int rows, int64_t t,
+                                              int64_t end, int cta, int64_t *next) {
+    const int b = find_seq<false>(seqs, n_seqs, (int)t);
+    const TreeSeq &sq = seqs[b];
+    const int tiles = (sq.context + sq.nodes + MANY_TILE - 1) / MANY_TILE;
+    const int rts = (sq.nodes * g.H + rows - 1) / rows;
+    const int local = (int)t - sq.unit0, item = local / tiles;
+    Segment s;
+    s.seq = b;
+    s.head = item / rts;
+    s.row0 = (item % rts) * rows;
+    s.lo = local - item * tiles;
+    s.hi = (int)min((int64_t)tiles, s.lo + (end - t));
+    s.slot = s.lo ? 2 * cta : s.hi < tiles ? 2 * cta + 1 : -1;
+    *next = t + (s.hi - s.lo);
+    return s;
+}
+
+// True in one lane of the (whole) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+    return p;
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+#define TC_R32(r)                                                                                                  \
+    "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),     \
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),      \
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),     \
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+#define TC_IN16(r, o)                                                                                              \
+    "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]),            \
+        "r"(r[o + 7]), "r"(r[o + 8]), "r"(r[o + 9]), "r"(r[o + 10]), "r"(r[o + 11]), "r"(r[o + 12]),                \
+        "r"(r[o + 13]), "r"(r[o + 14]), "r"(r[o + 15])
+
+// 32 columns of this warp's 32 lanes (thread: its lane's)
+__device__ __forceinline__ void tc_load32(uint32_t (&r)[32], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,"
+                 "%27,%28,%29,%30,%31}, [%32];"
+                 : TC_R32(r)
+                 : "r"(at)
+                 : "memory");
+}
+#define TC_IO32(r)                                                                                                 \
+    "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),     \
+        "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),      \
+        "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),     \
+        "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+// The loads before it are done; the registers pass through it, so that no use
+// of theirs can be moved ahead of it.
+__device__ __forceinline__ void tc_wait_load(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : TC_IO32(r)::"memory");
+}
+__device__ __forceinline__ void tc_store16(uint32_t at, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+                 TC_IN16(r, 0)
+                 : "memory");
+}
+
+// A shared-memory operand in 8-row groups of 1,024 bytes, 128-byte rows with
+// the 128-byte swizzle: 64 fp16 of the inner dimension a row.
+__device__ __forceinline__ uint64_t tc_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)2 << 61;
+}
+// fp16 x fp16 -> fp32, M = 128; B's rows are N (K-major) or K (MN-major)
+__host__ __device__ constexpr uint32_t tc_idesc(int n, bool b_mn) {
+    return 1u << 4 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n / 8) << 17 | (uint32_t)(128 / 16) << 24;
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
+                 "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+
+// 32 visibility bits of node `mk` from drafted offset d on (d < 0: context).
+__device__ __forceinline__ uint32_t seen32(const uint64_t *mk, int nodes, int d) {
+    auto word = [&](int at) -> uint64_t { return at * 64 < nodes ? mk[at] : 0ull; };
+    uint32_t bits;
+    if (d <= -32) return 0xffffffffu;
+    if (d < 0) bits = (uint32_t)(word(0) << -d) | ((1u << -d) - 1u);
+    else {
+        const int sh = d & 63;
+        bits = (uint32_t)(word(d >> 6) >> sh);
+        if (sh > 32) bits |= (uint32_t)(word((d >> 6) + 1) << (64 - sh));
+    }
+    const int live = nodes - d;                      // bits at and beyond the tree's end are no tokens
+    return live >= 32 ? bits : live <= 0 ? 0u : bits & ((1u << live) - 1u);
+}
+
+// One stream's softmax of a tile, a thread a row of 128 columns.
+template <bool MASKED>
+__device__ __forceinline__ void hide(uint32_t (&x)[32], const uint64_t *mk, int nodes, int d) {
+    if (!MASKED) return;
+    const uint32_t see = seen32(mk, nodes, d);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = (see >> j) & 1 ? x[j] : 0xff800000u;
+}
+__device__ __forceinline__ float largest(const uint32_t (&x)[32], float m) {
+    float m1 = __uint_as_float(x[0]);
+#pragma unroll
+    for (int j = 1; j < 32; j += 2) {
+        m = fmaxf(m, __uint_as_float(x[j]));
+        if (j + 1 < 32) m1 = fmaxf(m1, __uint_as_float(x[j + 1]));
+    }
+    return fmaxf(m, m1);
+}
+__device__ __forceinline__ uint64_t pair64(uint32_t lo, uint32_t hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float2 split64(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+
+// P = exp2(S - ref) in fp16, sum = its row sum in fp32; true if some row of
+// the warp exceeds its ref by more than LAG (P and sum are then not valid).
+template <bool MASKED>
+__device__ __forceinline__ bool weigh(uint32_t S, uint32_t P, float ref, float &sum, const uint64_t *mk, int nodes,
+                                      int d) {
+    const float sub = ref > -INFINITY ? -ref : 0.0f;
+    const uint64_t sub2 = pair64(__float_as_uint(sub), __float_as_uint(sub));
+    uint32_t x[2][32];
+    uint64_t acc[2] = {0, 0};
+    float top = -INFINITY;
+    tc_load32(x[0], S);
+    tc_wait_load(x[0]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        uint32_t(&y)[32] = x[c & 1];
+        if (c < 3) tc_load32(x[(c + 1) & 1], S + 32 * (c + 1));
+        hide<MASKED>(y, mk, nodes, d + 32 * c);
+        top = largest(y, top);
+        uint32_t p[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float2 v = split64(add_pair(pair64(y[2 * j], y[2 * j + 1]), sub2));
+            const float e0 = ex2(v.x), e1 = ex2(v.y);
+            acc[j & 1] = add_pair(acc[j & 1], pair64(__float_as_uint(e0), __float_as_uint(e1)));
+            p[j] = pack_half2(e0, e1);
+        }
+        tc_store16(P + 16 * c, p);
+        if (c < 3) tc_wait_load(x[(c + 1) & 1]);
+    }
+    const float2 v = split64(add_pair(acc[0], acc[1]));
+    sum = v.x + v.y;
+    return __any_sync(FULL, top > ref + LAG);
+}
+
+// Moves ref up to the row's maximum and scales the sums so far to it.
+template <bool MASKED>
+__device__ __noinline__ void raise(uint32_t S, uint32_t O, bool scale, float &ref, float &l, const uint64_t *mk,
+                                   int nodes, int d) {
+    float now = ref;
+    uint32_t x[32];
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        tc_load32(x, S + 32 * c);
+        tc_wait_load(x);
+        hide<MASKED>(x, mk, nodes, d + 32 * c);
+        now = largest(x, now);
+    }
+    const float f = now > -INFINITY ? ex2(ref - now) : 1.0f;
+    ref = now;
+    l *= f;
+    if (scale) {
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+            tc_load32(x, O + 32 * c);
+            tc_wait_load(x);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
+            tc_store16(O + 32 * c, x);
+            tc_store16(O + 32 * c + 16, x + 16);
+        }
+    }
+    tc_wait_st();
+}
+
+// A word of the constant tables (not volatile: loads may be batched).
+__device__ __forceinline__ uint32_t load_shared(uint32_t at) {
+    uint32_t x;
+    asm("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at));
+    return x;
+}
+// half2 x (hi + lo): a 16-bit norm needs two halves to be exact
+__device__ __forceinline__ uint32_t scale_half2(uint32_t x, __half2 hi, __half2 lo) {
+    const __half2 v = *reinterpret_cast<const __half2 *>(&x);
+    const __half2 r = __hfma2(v, hi, __hmul2(v, lo));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+template <int KB, int VB, bool ROWS, class Src>
+__global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a, int64_t all_tiles,
+                                                               const __grid_constant__ Src src) {
+    constexpr int RU = ROWS ? 256 : 128;             // query rows of an item
+    extern __shared__ uint8_t raw[];
+    uint8_t *sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    const uint32_t sm0 = smem_u32(sm);
+    const int tid = threadIdx.x, warp = __shfl_sync(FULL, tid / 32, 0), lane = tid % 32;
+    // barriers: full[3] empty[3] s_ready[2] p_ready[2] q_ready seg_done o_free m_full m_empty fin; then the TMEM address
+    const uint32_t bars = sm0 + MANY_BARS_AT;
+    auto full = [&](int i) { return bars + 8 * i; };
+    auto empty = [&](int i) { return bars + 24 + 8 * i; };
+    auto s_ready = [&](int i) { return bars + 48 + 8 * i; };
+    auto p_ready = [&](int i) { return bars + 64 + 8 * i; };
+    const uint32_t q_ready = bars + 80, seg_done = bars + 88, o_free = bars + 96, m_full = bars + 104,
+                   m_empty = bars + 112, fin = bars + 120;
+    auto row_bar = [&](int w, int slot) { return bars + 128 + 8 * (w * MANY_RING + slot); };
+    volatile uint32_t *tmem_at = reinterpret_cast<uint32_t *>(sm + MANY_BARS_AT + 256);
+
+    // the codes' tables, an entry of 256 bytes: 32 lanes' copies of a key pair, then of a value pair
+    const float cunit = exp2f((float)-g.centroid_frac);
+    for (int i = tid; i < (1 << (2 * KB)) * 32; i += MANY_THREADS) {
+        const int e = i / 32;
+        reinterpret_cast<uint32_t *>(sm)[e * 64 + i % 32] = pack_half2((float)a.tb->k_cent[e & ((1 << KB) - 1)] * cunit,
+                                                                       (float)a.tb->k_cent[e >> KB] * cunit);
+    }
+    for (int i = tid; i < (1 << (2 * VB)) * 32; i += MANY_THREADS) {
+        const int e = i / 32;
+        reinterpret_cast<uint32_t *>(sm)[e * 64 + 32 + i % 32] = pack_half2(
+            (float)a.tb->v_cent[e & ((1 << VB) - 1)] * cunit, (float)a.tb->v_cent[e >> VB] * cunit);
+    }
+    if (tid == 0) {
+        for (int i = 0; i < MANY_STAGES; ++i) bar_init(full(i), 4), bar_init(empty(i), 1);
+        for (int i = 0; i < 2; ++i) bar_init(s_ready(i), 1), bar_init(p_ready(i), 4);
+        bar_init(q_ready, 4), bar_init(seg_done, 1), bar_init(o_free, 8);
+        bar_init(m_full, 4), bar_init(m_empty, 4), bar_init(fin, 1);
+        for (int i = 0; i < 4 * MANY_RING; ++i) bar_init(row_bar(0, i), 1);
+        bar_init_fence();
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32((void *)tmem_at))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    wait_prior_grid();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_at;
+    // of stream i: S at 256 i, P at 256 i + 128, O at 256 i + 192
+
+    const TreeSeq *seqs = reinterpret_cast<const TreeSeq *>(src.data());
+    const int cta = blockIdx.x;
+    int64_t t = run_start(cta, all_tiles, gridDim.x);
+    const int64_t end = run_start(cta + 1, all_tiles, gridDim.x);
+    bool lost = false;                               // a wait gave up: the same for all lanes that wait together
+    auto wait = [&](uint32_t bar, int phase) {
+        if (!lost && !bar_wait(bar, (uint32_t)phase & 1u)) {
+            lost = true;
+            atomicOr(a.status, ST_TIMEOUT);
+        }
+        lost = __any_sync(FULL, lost);
+    };
+
+    if (warp >= 8 && warp < 12) {
+        // ---- decode: thread `row` owns row `row` of each tile, a warp 32 of them
+        const int row = tid - 256;
+        const uint32_t lut = sm0 + lane * 4;
+        const uint32_t ring = sm0 + MANY_RING_AT + (warp - 8) * MANY_RING * MANY_SLOT;
+        const float unit = exp2f((float)-g.norm_frac);
+        int kt = 0, kr = 0;                                      // tiles so far; the ring slot of the segment's first
+        uint32_t uses = 0;                                       // bit i: the parity that ring slot i waits for next
+        for (int seg = 0; t < end && !lost; ++seg) {
+            int64_t next;
+            const Segment s = segment_at(seqs, a.n_seqs, g, RU, t, end, cta, &next);
+            const TreeSeq sq = seqs[s.seq];
+            const int len = sq.context + sq.nodes, rows_all = sq.nodes * g.H;
+            constexpr int KV4 = KB * 2, VV4 = VB * 2;            // 32-bit words of a row's codes
+            // bulk copies of this warp's 32 rows of tile s.lo + k, in the planes' runs that pages leave
+            auto issue = [&](int k) {
+                const int p0 = (s.lo + k) * MANY_TILE + (warp - 8) * 32;
+                if (s.lo + k >= s.hi || p0 >= len) return;
+                const int slot = (kr + k) % MANY_RING, rows16 = (min(32, len - p0) + 15) & ~15;
+                const uint32_t bar = row_bar(warp - 8, slot), dst = ring + slot * MANY_SLOT;
+                if (lane == 0) bar_expect(bar, rows16 * (8 * KB + 8 * VB + 4));
+                __syncwarp();
+                const int first = min(rows16, g.P - p0 % g.P);   // pages hold a multiple of 16 rows: two runs at most
+                const int at = lane ? first : 0, n = lane ? rows16 - first : first;
+                if (lane < 2 && n) {
+                    const int p = p0 + at, in = p % g.P;
+                    const uint8_t *reg =
+                        a.pool + region_off(g, a.table[(int64_t)sq.seq * g.max_pages + p / g.P], s.head);
+                    copy_bulk(dst + at * 8 * KB, reg + (int64_t)in * (8 * KB), n * 8 * KB, bar);
+                    copy_bulk(dst + 32 * 8 * KB + at * 8 * VB, reg + vplane_off(g) + (int64_t)in * (8 * VB), n * 8 * VB,
+                              bar);
+                    copy_bulk(dst + 32 * 8 * (KB + VB) + at * 4, reg + nplane_off(g) + (int64_t)in * 4, n * 4, bar);
+                }
+            };
+            for (int k = 0; k < MANY_RING - 1; ++k) issue(k);
+            // the queries, in log2 units
+            if (seg) wait(seg_done, seg - 1);
+            const float u = LOG2E * exp2f((float)-g.qk_frac);
+            for (int i = row; i < RU * 8; i += 128) {
+                const int r = i / 8, c = i % 8, qr = s.row0 + r;
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (qr < rows_all) {
+                    const int4 *p = reinterpret_cast<const int4 *>(
+                        a.q + (((int64_t)(sq.node0 + qr / g.H) * g.n_kv + s.head) * g.H + qr % g.H) * D + 8 * c);
+                    const int4 x = p[0], y = p[1];
+                    w = make_uint4(pack_half2((float)x.x * u, (float)x.y * u), pack_half2((float)x.z * u, (float)x.w * u),
+                                   pack_half2((float)y.x * u, (float)y.y * u), pack_half2((float)y.z * u, (float)y.w * u));
+                }
+                *reinterpret_cast<uint4 *>(sm + MANY_Q_AT + r * 128 + ((c ^ (r & 7)) * 16)) = w;
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(q_ready);
+
+            for (int k = 0; k < s.hi - s.lo && !lost; ++k, ++kt) {
+                uint32_t ck[KV4], cv[VV4], cn = 0;
+                const bool live = (s.lo + k) * MANY_TILE + row < len;
+                __syncwarp();                                    // the slot's last rows have been read
+                issue(k + MANY_RING - 1);
+                if ((s.lo + k) * MANY_TILE + (warp - 8) * 32 < len) {
+                    const int slot = (kr + k) % MANY_RING;
+                    wait(row_bar(warp - 8, slot), uses >> slot);
+                    uses ^= 1u << slot;
+                    const uint8_t *st = sm + (ring - sm0) + slot * MANY_SLOT;
+                    const uint8_t *pk = st + lane * 8 * KB, *pv = st + 32 * 8 * KB + lane * 8 * VB;
+#pragma unroll
+                    for (int i = 0; i < KV4; i += 2)
+                        *reinterpret_cast<uint2 *>(ck + i) = *reinterpret_cast<const uint2 *>(pk + 4 * i);
+#pragma unroll
+                    for (int i = 0; i < VV4; i += 2)
+                        *reinterpret_cast<uint2 *>(cv + i) = *reinterpret_cast<const uint2 *>(pv + 4 * i);
+                    cn = *reinterpret_cast<const uint32_t *>(st + 32 * 8 * (KB + VB) + lane * 4);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < KV4; ++i) ck[i] = 0;
+#pragma unroll
+                    for (int i = 0; i < VV4; ++i) cv[i] = 0;
+                }
+                cn = live ? cn : 0;                              // past the end: a zero norm makes a zero row
+                const int st = kt % MANY_STAGES;
+                if (kt >= MANY_STAGES) wait(empty(st), kt / MANY_STAGES - 1);
+                const float kn = norm_value(cn & 0xffffu, unit), vn = norm_value(cn >> 16, unit);
+                auto codes = [&](const uint32_t *w, int bits, int j) -> uint32_t {   // pair j of 2-code fields, times 256
+                    if (bits == 4) return __byte_perm(w[j / 4], 0, 0x4404 | ((j % 4) << 4));
+                    const int at = 2 * bits * j, i = at / 32, sh = at % 32;
+                    const uint32_t x = sh + 2 * bits <= 32 ? w[i] >> sh : __funnelshift_r(w[i], w[i + 1], sh);
+                    return (x & ((1u << (2 * bits)) - 1u)) << 8;
+                };
+                auto put = [&](int base, const uint32_t *w, int bits, int off, float nrm) {
+                    const __half2 hi = __float2half2_rn(nrm);
+                    const __half2 lo = __float2half2_rn(nrm - __low2float(hi));
+#pragma unroll
+                    for (int c = 0; c < 8; c += 4) {
+                        uint32_t v[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] = load_shared(lut + off + codes(w, bits, 4 * c + j));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) v[4 * k + j] = scale_half2(v[4 * k + j], hi, lo);
+                            *reinterpret_cast<uint4 *>(sm + base + st * MANY_KV + row * 128 +
+                                                       (((c + k) ^ (row & 7)) * 16)) =
+                                make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                        }
+                    }
+                };
+                put(MANY_K_AT, ck, KB, 0, kn);
+                put(MANY_V_AT, cv, VB, 128, vn);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) bar_arrive(full(st));
+            }
+            kr = (kr + s.hi - s.lo) % MANY_RING;
+            t = next;
+        }
+        // copies that a lost wait left in flight land before the CTA goes
+        if (lost)
+            for (int i = 0; i < MANY_RING; ++i) bar_wait(row_bar(warp - 8, i), uses >> i & 1u);
+    } else if (warp == 12) {
+        // ---- this warp issues every product. All lanes walk the same steps
+        // (so that operands stay in uniform registers: with one lane inside a
+        // branch each product cost some 60 clocks of register moves), and one
+        // elected lane issues.
+        constexpr uint32_t iqk = tc_idesc(128, false), ipv = tc_idesc(64, true);
+        int st_qk = 0, st_pv = 0, np[2] = {0, 0};     // stages of the next score product and the next value product
+        int use = 0;                                  // rounds of the stages so far
+        const uint64_t q_desc = tc_desc(sm0 + MANY_Q_AT), k_desc = tc_desc(sm0 + MANY_K_AT),
+                       v_desc = tc_desc(sm0 + MANY_V_AT);
+        for (int seg = 0; t < end && !lost; ++seg) {
+            int64_t next;
+            const Segment s = segment_at(seqs, a.n_seqs, g, RU, t, end, cta, &next);
+            const int tiles = __shfl_sync(FULL, s.hi - s.lo, 0), steps = ROWS ? 2 * tiles : tiles;
+            auto scores = [&](int step) {
+                const int i = step & 1;
+                if (!ROWS || i == 0) wait(full(st_qk), use);
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t q = q_desc + (ROWS ? i * (MANY_KV >> 4) : 0), k = k_desc + st_qk * (MANY_KV >> 4);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) tc_mma_ss(tmem + 256 * i, q + 2 * x, k + 2 * x, iqk, x > 0);
+                    tc_commit(s_ready(i));
+                }
+                __syncwarp();
+                if (!ROWS || i == 1) {
+                    st_qk = st_qk == MANY_STAGES - 1 ? 0 : st_qk + 1;
+                    use += st_qk == 0;
+                }
+            };
+            wait(q_ready, seg);
+            if (seg) wait(o_free, seg - 1);
+            for (int step = 0; step < min(2, steps) && !lost; ++step) scores(step);
+            for (int step = 0; step < steps && !lost; ++step) {
+                const int i = step & 1;
+                wait(p_ready(i), i ? np[1]++ : np[0]++);
+                if (lost) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t v = v_desc + st_pv * (MANY_KV >> 4);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        tc_mma_ts(tmem + 256 * i + 192, tmem + 256 * i + 128 + 8 * x, v + 128 * x, ipv,
+                                  step >= 2 || x > 0);
+                    if (!ROWS || i == 1) tc_commit(empty(st_pv));
+                    if (step + 2 >= steps) tc_commit(s_ready(i));        // the stream's sums are complete
+                }
+                __syncwarp();
+                if (!ROWS || i == 1) st_pv = st_pv == MANY_STAGES - 1 ? 0 : st_pv + 1;
+                if (step + 2 < steps) scores(step + 2);
+            }
+            if (elect_one()) tc_commit(seg_done);
+            __syncwarp();
+            t = next;
+        }
+        // nothing may be in flight when the tensor memory goes
+        if (elect_one()) tc_commit(fin);
+        __syncwarp();
+        if (!bar_wait(fin, 0)) atomicOr(a.status, ST_TIMEOUT);
+        __syncwarp();
+    } else {
+        // ---- softmax: thread `row` of stream `i` owns one query row
+        const int i = warp / 4, row = tid - 128 * i;
+        const uint32_t lanes = (uint32_t)(warp % 4) << 21;   // lane 32 (warp % 4), in bits 16 up
+        const uint32_t S = tmem + lanes + 256 * i, P = S + 128, O = S + 192;
+        int ns = 0;
+        for (int seg = 0; t < end && !lost; ++seg) {
+            int64_t next;
+            const Segment s = segment_at(seqs, a.n_seqs, g, RU, t, end, cta, &next);
+            const TreeSeq sq = seqs[s.seq];
+            const int rows_all = sq.nodes * g.H, qr = s.row0 + (ROWS ? 128 * i : 0) + row;
+            const bool any_row = qr - lane < rows_all;       // of this warp's 32
+            const int node = min(qr / g.H, sq.nodes - 1);
+            const uint64_t *mk = a.mask + (int64_t)(sq.node0 + node) * a.words;
+            const int tiles = s.hi - s.lo, steps = ROWS ? tiles : (tiles + 1 - i) / 2;
+            float ref = -INFINITY, l = 0.0f;
+            for (int n = 0; n < steps && !lost; ++n) {
+                const int t0 = (s.lo + (ROWS ? n : 2 * n + i)) * MANY_TILE;
+                wait(s_ready(i), ns++);
+                if (lost) break;
+                tc_fence_after();
+                if (any_row) {
+                    float sum;
+                    if (t0 + MANY_TILE <= sq.context) {
+                        // the exponentials are taken under the maximum so far,
+                        // and again in the rare case that it was too low
+                        bool over = true;
+                        if (n > 0) over = weigh<false>(S, P, ref, sum, nullptr, 0, 0);
+                        if (over) {
+                            raise<false>(S, O, n > 0, ref, l, nullptr, 0, 0);
+                            weigh<false>(S, P, ref, sum, nullptr, 0, 0);
+                        }
+                    } else {
+                        bool over = true;
+                        if (n > 0) over = weigh<true>(S, P, ref, sum, mk, sq.nodes, t0 - sq.context);
+                        if (over) {
+                            raise<true>(S, O, n > 0, ref, l, mk, sq.nodes, t0 - sq.context);
+                            weigh<true>(S, P, ref, sum, mk, sq.nodes, t0 - sq.context);
+                        }
+                    }
+                    l += sum;
+                    tc_wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(p_ready(i));
+            }
+            if (steps) wait(s_ready(i), ns++);
+            tc_fence_after();
+            if (lost) break;
+            // this row's sums out
+            float *ml = reinterpret_cast<float *>(sm + MANY_ML_AT);
+            float *hand = reinterpret_cast<float *>(sm + MANY_Q_AT + MANY_KV);   // !ROWS: the second query tile is free
+            float f0 = 1.0f, f1 = 0.0f, m = ref;
+            const bool mine = ROWS || i == 0;
+            if (!ROWS && i == 1) ml[row * 2] = ref, ml[row * 2 + 1] = l;
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+                uint32_t x[32];
+                if (steps) {
+                    tc_load32(x, O + 32 * c);
+                    tc_wait_load(x);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) x[j] = 0;
+                }
+                if (!ROWS) {
+                    const int turn = 2 * seg + c;
+                    if (i == 1) {
+                        if (turn) wait(m_empty, turn - 1);
+                        if (lost) break;
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<uint4 *>(hand + row * 32 + ((j / 4 ^ (row & 7)) * 4)) =
+                                make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(m_full);
+                        continue;
+                    }
+                    wait(m_full, turn);
+                    if (lost) break;
+                    if (c == 0) {
+                        const float m1 = ml[row * 2], l1 = ml[row * 2 + 1];
+                        m = fmaxf(ref, m1);
+                        f0 = m > -INFINITY ? ex2(ref - m) : 0.0f;
+                        f1 = m > -INFINITY ? ex2(m1 - m) : 0.0f;
+                        l = l * f0 + l1 * f1;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 y = *reinterpret_cast<const float4 *>(hand + row * 32 + ((j / 4 ^ (row & 7)) * 4));
+                        const float z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            // a stream without weight may hold anything
+                            const float u0 = f0 > 0.0f ? f0 * __uint_as_float(x[j + k]) : 0.0f;
+                            x[j + k] = __float_as_uint(f1 > 0.0f ? fmaf(f1, z[k], u0) : u0);
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(m_empty);
+                }
+                if (!mine || qr >= rows_all) continue;
+                if (s.slot < 0) {
+                    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                    uint4 *dst = reinterpret_cast<uint4 *>(
+                        a.out + (((int64_t)(sq.node0 + qr / g.H) * g.n_kv + s.head) * g.H + qr % g.H) * D + 32 * c);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(x[8 * j + 2 * k]) * inv,
+                                                                           __uint_as_float(x[8 * j + 2 * k + 1]) * inv);
+                            w[k] = *reinterpret_cast<const uint32_t *>(&v);
+                        }
+                        dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else {
+                    const int64_t at = (int64_t)s.slot * RU + (ROWS ? 128 * i : 0) + row;
+                    uint4 *dst = reinterpret_cast<uint4 *>(a.acc + at * 64 + 32 * c);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) dst[j] = make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+                    if (c == 0) a.ml[at * 2] = m, a.ml[at * 2 + 1] = l;
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(o_free);
+            t = next;
+        }
+    }
+    __syncthreads();
+    if (warp == 12)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// ---------------------------------------------------------------------------
 // joining the splits of a row tile
 // ---------------------------------------------------------------------------
 
-// One CTA per (sequence, row tile, KV head): the splits' partial sums, scaled
-// to the largest of their maxima, added in order and divided by the sum of
-// weights. Rows are `R` a tile.
-template <class Src>
-__global__ void __launch_bounds__(256) k_tree_join(Geo g, TreeArgs a, int32_t R, const __grid_constant__ Src src) {
-    extern __shared__ float wt[];                    // [rows][splits]
+// One CTA per 8 rows of a (sequence, row tile, KV head): the parts' sums,
+// scaled to the largest of their maxima, added in order and divided by the sum
+// of weights. Bound by the parts' bytes, at few items by how many CTAs read
+// them (one CTA an item took 100 us where 8 items had 19 parts of 256 rows).
+// Rows are `R` a tile. MANY: the parts are the runs (of `ctas` over
+// `all_tiles`) that the item's KV tiles lie in, else the item's splits.
+template <bool MANY, class Src>
+__global__ void __launch_bounds__(128) k_tree_join(Geo g, TreeArgs a, int32_t R, int64_t all_tiles, int32_t ctas,
+                                                   const __grid_constant__ Src src) {
+    extern __shared__ float wt[];                    // [8][splits]
     wait_prior_grid();
     const TreeSeq *seqs = reinterpret_cast<const TreeSeq *>(src.data());
-    const TreeSeq sq = seqs[find_seq<true>(seqs, a.n_seqs, blockIdx.x)];
-    if (sq.splits == 1) return;
+    const int per = R / 8, part8 = blockIdx.x % per * 8;
+    const TreeSeq sq = seqs[find_seq<true>(seqs, a.n_seqs, blockIdx.x / per)];
     const int G = g.H, rows_all = sq.nodes * G, tiles = (rows_all + R - 1) / R;
-    const int group = blockIdx.x - sq.group0, head = group % g.n_kv, rt = group / g.n_kv;
-    const int row0 = rt * R, rows = min(R, rows_all - row0);
+    const int group = blockIdx.x / per - sq.group0;
+    const int head = MANY ? group / tiles : group % g.n_kv, rt = MANY ? group % tiles : group / g.n_kv;
+    const int row0 = rt * R + part8, rows = min(8, rows_all - row0);
+    int run0 = 0, splits = sq.splits;
+    if (MANY) {
+        const int kv = (sq.context + sq.nodes + MANY_TILE - 1) / MANY_TILE;
+        const int64_t first = sq.unit0 + (int64_t)group * kv;
+        run0 = run_of(first, all_tiles, ctas);
+        splits = run_of(first + kv - 1, all_tiles, ctas) - run0 + 1;
+    }
+    if (splits == 1 || rows <= 0) return;
     auto slot = [&](int split, int r) {
-        return ((int64_t)sq.unit0 + ((int64_t)split * tiles + rt) * g.n_kv + head) * R + r;
+        if (MANY) return ((int64_t)2 * (run0 + split) + (split == 0)) * R + part8 + r;
+        return ((int64_t)sq.unit0 + ((int64_t)split * tiles + rt) * g.n_kv + head) * R + part8 + r;
     };
-    for (int r = threadIdx.x / 32; r < rows; r += 8) {
+    for (int r = threadIdx.x / 32; r < rows; r += 4) {
         const int lane = threadIdx.x % 32;
         float M = -INFINITY, sum = 0.0f;
-        for (int s = lane; s < sq.splits; s += 32) M = fmaxf(M, a.ml[slot(s, r) * 2]);
+        for (int s = lane; s < splits; s += 32) M = fmaxf(M, a.ml[slot(s, r) * 2]);
         for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, o));
-        for (int s = lane; s < sq.splits; s += 32) {
+        for (int s = lane; s < splits; s += 32) {
             const float f = M > -INFINITY ? ex2(a.ml[slot(s, r) * 2] - M) : 0.0f;
             sum += f * a.ml[slot(s, r) * 2 + 1];
-            wt[r * sq.splits + s] = f;
+            wt[r * splits + s] = f;
         }
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
         const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-        for (int s = lane; s < sq.splits; s += 32) wt[r * sq.splits + s] *= inv;
+        for (int s = lane; s < splits; s += 32) wt[r * splits + s] *= inv;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * 16; i += 256) {
+    for (int i = threadIdx.x; i < rows * 16; i += 128) {
         const int r = i / 16, c4 = i % 16;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int s = 0; s < sq.splits; ++s) {
-            const float f = wt[r * sq.splits + s];
+#pragma unroll 8
+        for (int s = 0; s < splits; ++s) {
+            const float f = wt[r * splits + s];
             const float4 v = reinterpret_cast<const float4 *>(a.acc)[slot(s, r) * 16 + c4];
             o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
         }
@@ -571,14 +1226,20 @@ __global__ void __launch_bounds__(256) k_tree_join(Geo g, TreeArgs a, int32_t R,
 
 namespace {
 
+// Above this many query rows of a KV head the tcgen05 kernel takes over.
+constexpr int MANY_FROM = 32;
+
 // How a call is cut: rows a tile, tokens a split, and what that takes.
 struct TreePlan {
     int rows = 16, warps = 16;
+    bool many = false;                       // k_tree_many's runs, else k_tree_few's units
     int64_t chunk = FEW_TILE, units = 0, groups = 0;
+    int ctas = 0;                            // many: runs
     int max_splits = 1;
     std::vector<TreeSeq> seqs;
+    int64_t slots() const { return many ? 2 * (int64_t)ctas : units; }
     size_t acc_bytes() const {
-        return max_splits > 1 ? (size_t)units * rows * (64 + 2) * sizeof(float) : 0;
+        return max_splits > 1 ? (size_t)slots() * rows * (64 + 2) * sizeof(float) : 0;
     }
 };
 
@@ -603,6 +1264,30 @@ int make_plan(const CacheBase *c, int32_t B, const int32_t *seq, const int32_t *
     }
     if (all > INT32_MAX / (g.n_kv * g.H)) return fail(INS_EBADLEN, "too many nodes in one call");
     if (p.seqs.empty()) return INS_OK;
+    const bool paired = (g.kb == 4 && g.vb == 2) || (g.kb == 3 && g.vb == 3);
+    if (paired && most > MANY_FROM) {
+        p.many = true;
+        p.rows = most > 128 ? 256 : 128;
+        for (TreeSeq &s : p.seqs) {
+            const int64_t rts = ((int64_t)s.nodes * g.H + p.rows - 1) / p.rows;
+            s.unit0 = (int32_t)p.units;
+            s.group0 = (int32_t)p.groups;
+            p.groups += rts * g.n_kv;
+            p.units += rts * g.n_kv * ((s.context + s.nodes + MANY_TILE - 1) / MANY_TILE);
+            if (p.units > INT32_MAX) return fail(INS_EBADLEN, "too much work in one call");
+        }
+        p.ctas = (int)std::min<int64_t>(sms, p.units);
+        for (const TreeSeq &s : p.seqs) {
+            const int64_t kv = (s.context + s.nodes + MANY_TILE - 1) / MANY_TILE;
+            const int64_t items = ((int64_t)s.nodes * g.H + p.rows - 1) / p.rows * g.n_kv;
+            for (int64_t i = 0; i < items; ++i) {
+                const int64_t first = s.unit0 + i * kv;
+                p.max_splits = std::max(p.max_splits, run_of(first + kv - 1, p.units, p.ctas) -
+                                                          run_of(first, p.units, p.ctas) + 1);
+            }
+        }
+        return INS_OK;
+    }
     // rows a tile: two 16-row fragments share each decoded token where there are more than 16 rows
     p.rows = most > 16 ? 32 : 16;
     p.warps = p.rows == 16 ? 16 : 12;
@@ -672,6 +1357,18 @@ int launch_few_rows(CacheBase *c, const TreePlan &p, bool half, const Plan &plan
     return launch_few<KB, VB, 1, false, N1>(c, p, plan, a, s);
 }
 
+template <int KB, int VB, bool ROWS>
+int launch_many(CacheBase *c, const TreePlan &p, const Plan &plan, const TreeArgs &a, cudaStream_t s) {
+    return plan.run(c, s, [&](const auto &src) -> cudaError_t {
+        auto fn = k_tree_many<KB, VB, ROWS, std::decay_t<decltype(src)>>;
+        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, MANY_SMEM);
+        if (e != cudaSuccess) return e;
+        *c->launches += 1;
+        return launch_after(fn, (unsigned)p.ctas, (unsigned)MANY_THREADS, (size_t)MANY_SMEM, s, c->g, a,
+                            (int64_t)p.units, src);
+    });
+}
+
 int tree_body(CacheBase *c, int32_t B, const int32_t *seq, const int32_t *nodes, const uint64_t *mask, int32_t words,
               const int32_t *q, void *out, void *workspace, int64_t workspace_bytes, int64_t *need, cudaStream_t s) {
     int sms = 0;
@@ -699,7 +1396,7 @@ int tree_body(CacheBase *c, int32_t B, const int32_t *seq, const int32_t *nodes,
     a.mask = mask;
     a.out = static_cast<__nv_bfloat16 *>(out);
     a.acc = static_cast<float *>(workspace);
-    a.ml = a.acc + (size_t)p.units * p.rows * 64;
+    a.ml = a.acc + (size_t)p.slots() * p.rows * 64;
     a.status = c->d_status;
     a.n_seqs = (int32_t)p.seqs.size();
     a.words = words;
@@ -710,18 +1407,25 @@ int tree_body(CacheBase *c, int32_t B, const int32_t *seq, const int32_t *nodes,
     bool half = true;
     for (const TreeSeq &t : p.seqs) half &= t.nodes * c->g.H <= 8;
     const int kb = c->g.kb, vb = c->g.vb;
-    const int rc = kb == 4 && vb == 2   ? launch_few_rows<4, 2>(c, p, half, plan, a, s)
+    const bool wide = p.rows == 256;
+    const int rc = p.many && kb == 4    ? (wide ? launch_many<4, 2, true>(c, p, plan, a, s)
+                                                : launch_many<4, 2, false>(c, p, plan, a, s))
+                   : p.many             ? (wide ? launch_many<3, 3, true>(c, p, plan, a, s)
+                                                : launch_many<3, 3, false>(c, p, plan, a, s))
+                   : kb == 4 && vb == 2 ? launch_few_rows<4, 2>(c, p, half, plan, a, s)
                    : kb == 3 && vb == 3 ? launch_few_rows<3, 3>(c, p, half, plan, a, s)
                                         : launch_few_rows<0, 0>(c, p, half, plan, a, s);
     if (rc) return rc;
     if (p.max_splits == 1) return INS_OK;
-    const size_t smem = (size_t)p.rows * p.max_splits * sizeof(float);
+    const size_t smem = (size_t)8 * p.max_splits * sizeof(float);
     return plan.run(c, s, [&](const auto &src) -> cudaError_t {
-        auto fn = k_tree_join<std::decay_t<decltype(src)>>;
+        using S = std::decay_t<decltype(src)>;
+        auto fn = p.many ? k_tree_join<true, S> : k_tree_join<false, S>;
         const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
         *c->launches += 1;
-        return launch_after(fn, (unsigned)p.groups, 256u, smem, s, c->g, a, (int32_t)p.rows, src);
+        return launch_after(fn, (unsigned)(p.groups * (p.rows / 8)), 128u, smem, s, c->g, a, (int32_t)p.rows, (int64_t)p.units,
+                            (int32_t)p.ctas, src);
     });
 }
 
