@@ -17,6 +17,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "plan.cuh"
 
@@ -96,6 +97,13 @@ __device__ __forceinline__ float norm_value(uint32_t x16, float unit) {
     return fmaf(__uint_as_float(0x4b000000u | (x16 ^ 0x8000u)), unit, -8421376.0f * unit);
 }
 
+// Position p's page index and row in the page (a shift where pages hold a power
+// of two rows, as they do by default: a division is some 20 instructions).
+__device__ __forceinline__ int page_of(const Geo &g, int p) { return g.p_log2 >= 0 ? p >> g.p_log2 : p / g.P; }
+__device__ __forceinline__ int row_in_page(const Geo &g, int p) {
+    return g.p_log2 >= 0 ? p & (g.P - 1) : p % g.P;
+}
+
 // The sequence that unit (or, GROUP, row group) `i` belongs to.
 template <bool GROUP>
 __device__ __forceinline__ int find_seq(const TreeSeq *seqs, int n, int i) {
@@ -168,16 +176,15 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
     // tables: constant, so filled before the wait for earlier launches
     const float cunit = exp2f((float)-g.centroid_frac);
     if (L::PAIRS) {
-        for (int i = tid; i < L::K_ENTRIES * 32; i += NW * 32) {
-            const int e = i / 32;
-            reinterpret_cast<uint32_t *>(sm)[i] = pack_half2((float)a.tb->k_cent[e & ((1 << KB) - 1)] * cunit,
-                                                             (float)a.tb->k_cent[e >> KB] * cunit);
-        }
-        for (int i = tid; i < L::V_ENTRIES * 32; i += NW * 32) {
-            const int e = i / 32;
-            reinterpret_cast<uint32_t *>(sm + L::KLUT)[i] = pack_half2(
-                (float)a.tb->v_cent[e & ((1 << VB) - 1)] * cunit, (float)a.tb->v_cent[e >> VB] * cunit);
-        }
+        float *cent = reinterpret_cast<float *>(sm + L::STAGES_AT);
+        if (tid < (1 << KB)) cent[tid] = (float)a.tb->k_cent[tid] * cunit;
+        if (tid >= 32 && tid < 32 + (1 << VB)) cent[tid] = (float)a.tb->v_cent[tid - 32] * cunit;
+        __syncthreads();
+        for (int e = warp; e < L::K_ENTRIES; e += NW)
+            reinterpret_cast<uint32_t *>(sm)[e * 32 + lane] = pack_half2(cent[e & ((1 << KB) - 1)], cent[e >> KB]);
+        for (int e = warp; e < L::V_ENTRIES; e += NW)
+            reinterpret_cast<uint32_t *>(sm + L::KLUT)[e * 32 + lane] =
+                pack_half2(cent[32 + (e & ((1 << VB) - 1))], cent[32 + (e >> VB)]);
     } else {
         __half *tab = reinterpret_cast<__half *>(sm);
         for (int i = tid; i < 512; i += NW * 32)
@@ -238,9 +245,9 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         // one lane per run of rows inside a page; pages hold a multiple of 16 rows
         int at = 0;
         for (int k = 0; at < rows16; ++k) {
-            const int p = p0 + at, in = p % g.P, n_rows = min(rows16 - at, g.P - in);
+            const int p = p0 + at, in = row_in_page(g, p), n_rows = min(rows16 - at, g.P - in);
             if (lane == k) {
-                const uint8_t *reg = a.pool + region_off(g, a.table[(int64_t)sq.seq * g.max_pages + p / g.P], head);
+                const uint8_t *reg = a.pool + region_off(g, a.table[(int64_t)sq.seq * g.max_pages + page_of(g, p)], head);
                 copy_bulk(dst + at * kbytes, reg + (int64_t)in * kbytes, n_rows * kbytes, bar);
                 copy_bulk(dst + FEW_TILE * kbytes + at * vbytes, reg + vplane_off(g) + (int64_t)in * vbytes,
                           n_rows * vbytes, bar);
@@ -522,10 +529,9 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
 // ---------------------------------------------------------------------------
 //
 // One CTA an SM. Its four decode warps turn 128 cached rows at a time into
-// fp16 key and value tiles in shared memory (a thread a row, norms applied),
-// one thread issues the products S = Q K^T and O += P V on the tensor cores,
-// and two groups of four warps (a stream each) turn S into P, a thread a
-// query row. S, P and O stay in tensor memory: 128 + 64 + 64 columns for each
+// fp16 key and value tiles in shared memory (a thread a row, norms applied);
+// one warp issues the products S = Q K^T and O += P V on the tensor cores, and
+// two groups of four warps (a stream each) turn S into P, a thread a query row. S, P and O stay in tensor memory: 128 + 64 + 64 columns for each
 // stream, all 512.
 //
 // The two streams keep the exponentials (the bound: 16 a clock and SM) busy
@@ -547,7 +553,7 @@ constexpr int MANY_RING = 4, MANY_SLOT = 32 * 52;
 constexpr int MANY_ML_AT = MANY_V_AT + MANY_STAGES * MANY_KV;
 constexpr int MANY_RING_AT = MANY_ML_AT + 128 * 2 * 4;
 constexpr int MANY_BARS_AT = MANY_RING_AT + 4 * MANY_RING * MANY_SLOT;
-constexpr int MANY_SMEM = MANY_BARS_AT + 320 + 1024;     // + the base's alignment to 1,024
+constexpr int MANY_SMEM = MANY_BARS_AT + 320;
 
 // Tile t of the run list -> its CTA, for `tiles` tiles in `ctas` equal runs.
 __host__ __device__ __forceinline__ int run_of(int64_t t, int64_t tiles, int ctas) {
@@ -625,6 +631,24 @@ __device__ __forceinline__ void tc_load32(uint32_t (&r)[32], uint32_t at) {
 // of theirs can be moved ahead of it.
 __device__ __forceinline__ void tc_wait_load(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : TC_IO32(r)::"memory");
+}
+__device__ __forceinline__ void tc_load16(uint32_t (&r)[16], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_wait_load(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::
+                     "memory");
+}
+__device__ __forceinline__ void tc_store8(uint32_t at, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tc_store16(uint32_t at, const uint32_t *r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -704,33 +728,43 @@ __device__ __forceinline__ float2 split64(uint64_t v) {
 
 // P = exp2(S - ref) in fp16, sum = its row sum in fp32; true if some row of
 // the warp exceeds its ref by more than LAG (P and sum are then not valid).
-template <bool MASKED>
+// p_free() waits until the product that reads the last P is complete.
+template <bool MASKED, typename F>
 __device__ __forceinline__ bool weigh(uint32_t S, uint32_t P, float ref, float &sum, const uint64_t *mk, int nodes,
-                                      int d) {
-    const float sub = ref > -INFINITY ? -ref : 0.0f;
+                                      int d, F &&p_free) {
+    // P carries a factor of 2^7 (as sum does): with LAG it stays below 2^15, and
+    // fp16 keeps weights down to 2^-31 of the maximum
+    const float sub = (ref > -INFINITY ? -ref : 0.0f) + 7.0f;
     const uint64_t sub2 = pair64(__float_as_uint(sub), __float_as_uint(sub));
-    uint32_t x[2][32];
+    uint32_t x[2][16];
     uint64_t acc[2] = {0, 0};
-    float top = -INFINITY;
-    tc_load32(x[0], S);
+    float top = -INFINITY, top1 = -INFINITY;
+    tc_load16(x[0], S);
     tc_wait_load(x[0]);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        uint32_t(&y)[32] = x[c & 1];
-        if (c < 3) tc_load32(x[(c + 1) & 1], S + 32 * (c + 1));
-        hide<MASKED>(y, mk, nodes, d + 32 * c);
-        top = largest(y, top);
-        uint32_t p[16];
+    for (int c = 0; c < 8; ++c) {
+        uint32_t(&y)[16] = x[c & 1];
+        if (c < 7) tc_load16(x[(c + 1) & 1], S + 16 * (c + 1));
+        if (MASKED) {
+            const uint32_t see = seen32(mk, nodes, d + 16 * c);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < 16; ++j) y[j] = (see >> j) & 1 ? y[j] : 0xff800000u;
+        }
+        uint32_t p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            top = fmaxf(top, __uint_as_float(y[2 * j]));
+            top1 = fmaxf(top1, __uint_as_float(y[2 * j + 1]));
             const float2 v = split64(add_pair(pair64(y[2 * j], y[2 * j + 1]), sub2));
             const float e0 = ex2(v.x), e1 = ex2(v.y);
             acc[j & 1] = add_pair(acc[j & 1], pair64(__float_as_uint(e0), __float_as_uint(e1)));
             p[j] = pack_half2(e0, e1);
         }
-        tc_store16(P + 16 * c, p);
-        if (c < 3) tc_wait_load(x[(c + 1) & 1]);
+        if (c == 0 && !p_free()) return false;
+        tc_store8(P + 8 * c, p);
+        if (c < 7) tc_wait_load(x[(c + 1) & 1]);
     }
+    top = fmaxf(top, top1);
     const float2 v = split64(add_pair(acc[0], acc[1]));
     sum = v.x + v.y;
     return __any_sync(FULL, top > ref + LAG);
@@ -783,11 +817,14 @@ template <int KB, int VB, bool ROWS, class Src>
 __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a, int64_t all_tiles,
                                                                const __grid_constant__ Src src) {
     constexpr int RU = ROWS ? 256 : 128;             // query rows of an item
-    extern __shared__ uint8_t raw[];
-    uint8_t *sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    // the tiles' swizzle needs 1,024-byte alignment; an address that is a
+    // constant keeps the products' operands in uniform registers
+    extern __shared__ __align__(1024) uint8_t many_smem[];
+    uint8_t *const sm = many_smem;
     const uint32_t sm0 = smem_u32(sm);
     const int tid = threadIdx.x, warp = __shfl_sync(FULL, tid / 32, 0), lane = tid % 32;
-    // barriers: full[3] empty[3] s_ready[2] p_ready[2] q_ready seg_done o_free m_full m_empty fin; then the TMEM address
+    // barriers: full[3] empty[3] s_ready[2] p_ready[2] q_ready seg_done o_free m_full m_empty fin, the 16 of the rings
+    // and pv_done[2]; then the TMEM address
     const uint32_t bars = sm0 + MANY_BARS_AT;
     auto full = [&](int i) { return bars + 8 * i; };
     auto empty = [&](int i) { return bars + 24 + 8 * i; };
@@ -796,23 +833,25 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
     const uint32_t q_ready = bars + 80, seg_done = bars + 88, o_free = bars + 96, m_full = bars + 104,
                    m_empty = bars + 112, fin = bars + 120;
     auto row_bar = [&](int w, int slot) { return bars + 128 + 8 * (w * MANY_RING + slot); };
-    volatile uint32_t *tmem_at = reinterpret_cast<uint32_t *>(sm + MANY_BARS_AT + 256);
+    volatile uint32_t *tmem_at = reinterpret_cast<uint32_t *>(sm + MANY_BARS_AT + 272);
+    auto pv_done = [&](int i) { return bars + 256 + 8 * i; };
 
     // the codes' tables, an entry of 256 bytes: 32 lanes' copies of a key pair, then of a value pair
     const float cunit = exp2f((float)-g.centroid_frac);
-    for (int i = tid; i < (1 << (2 * KB)) * 32; i += MANY_THREADS) {
-        const int e = i / 32;
-        reinterpret_cast<uint32_t *>(sm)[e * 64 + i % 32] = pack_half2((float)a.tb->k_cent[e & ((1 << KB) - 1)] * cunit,
-                                                                       (float)a.tb->k_cent[e >> KB] * cunit);
-    }
-    for (int i = tid; i < (1 << (2 * VB)) * 32; i += MANY_THREADS) {
-        const int e = i / 32;
-        reinterpret_cast<uint32_t *>(sm)[e * 64 + 32 + i % 32] = pack_half2(
-            (float)a.tb->v_cent[e & ((1 << VB) - 1)] * cunit, (float)a.tb->v_cent[e >> VB] * cunit);
+    {
+        float *cent = reinterpret_cast<float *>(sm + MANY_K_AT);
+        if (tid < (1 << KB)) cent[tid] = (float)a.tb->k_cent[tid] * cunit;
+        if (tid >= 32 && tid < 32 + (1 << VB)) cent[tid] = (float)a.tb->v_cent[tid - 32] * cunit;
+        __syncthreads();
+        for (int e = warp; e < (1 << (2 * KB)); e += MANY_THREADS / 32)
+            reinterpret_cast<uint32_t *>(sm)[e * 64 + lane] = pack_half2(cent[e & ((1 << KB) - 1)], cent[e >> KB]);
+        for (int e = warp; e < (1 << (2 * VB)); e += MANY_THREADS / 32)
+            reinterpret_cast<uint32_t *>(sm)[e * 64 + 32 + lane] =
+                pack_half2(cent[32 + (e & ((1 << VB) - 1))], cent[32 + (e >> VB)]);
     }
     if (tid == 0) {
         for (int i = 0; i < MANY_STAGES; ++i) bar_init(full(i), 4), bar_init(empty(i), 1);
-        for (int i = 0; i < 2; ++i) bar_init(s_ready(i), 1), bar_init(p_ready(i), 4);
+        for (int i = 0; i < 2; ++i) bar_init(s_ready(i), 1), bar_init(p_ready(i), 4), bar_init(pv_done(i), 1);
         bar_init(q_ready, 4), bar_init(seg_done, 1), bar_init(o_free, 8);
         bar_init(m_full, 4), bar_init(m_empty, 4), bar_init(fin, 1);
         for (int i = 0; i < 4 * MANY_RING; ++i) bar_init(row_bar(0, i), 1);
@@ -827,7 +866,16 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
     wait_prior_grid();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_at;
+    // All 512 columns are this CTA's, so they start at address 0 (a constant, for
+    // the same reason).
+    constexpr uint32_t tmem = 0;
+    if (*tmem_at != tmem || (sm0 & 1023)) {                  // never: reported, not worked around
+        if (tid == 0) atomicOr(a.status, ST_INTERNAL);
+        __syncthreads();
+        if (warp == 12)
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(*tmem_at) : "memory");
+        return;
+    }
     // of stream i: S at 256 i, P at 256 i + 128, O at 256 i + 192
 
     const TreeSeq *seqs = reinterpret_cast<const TreeSeq *>(src.data());
@@ -857,7 +905,17 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
             const TreeSeq sq = seqs[s.seq];
             const int len = sq.context + sq.nodes, rows_all = sq.nodes * g.H;
             constexpr int KV4 = KB * 2, VV4 = VB * 2;            // 32-bit words of a row's codes
-            // bulk copies of this warp's 32 rows of tile s.lo + k, in the planes' runs that pages leave
+            const int32_t *pages = a.table + (int64_t)sq.seq * g.max_pages;
+            // Bulk copies of this warp's 32 rows of tile s.lo + k, in the runs
+            // that pages leave: two at most, as pages hold a multiple of 16
+            // rows; lane 0 copies the first, lane 1 the second. A run's page is
+            // looked up one tile ahead.
+            int page = 0;
+            auto look_up = [&](int k) {
+                const int p0 = (s.lo + k) * MANY_TILE + (warp - 8) * 32;
+                const int p = p0 + (lane ? g.P - row_in_page(g, p0) : 0);
+                if (lane < 2 && s.lo + k < s.hi && p < min(len, p0 + 32)) page = pages[page_of(g, p)];
+            };
             auto issue = [&](int k) {
                 const int p0 = (s.lo + k) * MANY_TILE + (warp - 8) * 32;
                 if (s.lo + k >= s.hi || p0 >= len) return;
@@ -865,24 +923,25 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                 const uint32_t bar = row_bar(warp - 8, slot), dst = ring + slot * MANY_SLOT;
                 if (lane == 0) bar_expect(bar, rows16 * (8 * KB + 8 * VB + 4));
                 __syncwarp();
-                const int first = min(rows16, g.P - p0 % g.P);   // pages hold a multiple of 16 rows: two runs at most
-                const int at = lane ? first : 0, n = lane ? rows16 - first : first;
+                const int in0 = row_in_page(g, p0), first = min(rows16, g.P - in0);
+                const int at = lane ? first : 0, n = lane ? rows16 - first : first, in = lane ? 0 : in0;
                 if (lane < 2 && n) {
-                    const int p = p0 + at, in = p % g.P;
-                    const uint8_t *reg =
-                        a.pool + region_off(g, a.table[(int64_t)sq.seq * g.max_pages + p / g.P], s.head);
+                    const uint8_t *reg = a.pool + region_off(g, page, s.head);
                     copy_bulk(dst + at * 8 * KB, reg + (int64_t)in * (8 * KB), n * 8 * KB, bar);
                     copy_bulk(dst + 32 * 8 * KB + at * 8 * VB, reg + vplane_off(g) + (int64_t)in * (8 * VB), n * 8 * VB,
                               bar);
                     copy_bulk(dst + 32 * 8 * (KB + VB) + at * 4, reg + nplane_off(g) + (int64_t)in * 4, n * 4, bar);
                 }
+                look_up(k + 1);
             };
+            look_up(0);
             for (int k = 0; k < MANY_RING - 1; ++k) issue(k);
             // the queries, in log2 units
             if (seg) wait(seg_done, seg - 1);
             const float u = LOG2E * exp2f((float)-g.qk_frac);
-            for (int i = row; i < RU * 8; i += 128) {
-                const int r = i / 8, c = i % 8, qr = s.row0 + r;
+#pragma unroll 4
+            for (int x = 0; x < RU / 16; ++x) {
+                const int i = row + 128 * x, r = i / 8, c = i % 8, qr = s.row0 + r;
                 uint4 w = make_uint4(0, 0, 0, 0);
                 if (qr < rows_all) {
                     const int4 *p = reinterpret_cast<const int4 *>(
@@ -927,6 +986,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                 const float kn = norm_value(cn & 0xffffu, unit), vn = norm_value(cn >> 16, unit);
                 auto codes = [&](const uint32_t *w, int bits, int j) -> uint32_t {   // pair j of 2-code fields, times 256
                     if (bits == 4) return __byte_perm(w[j / 4], 0, 0x4404 | ((j % 4) << 4));
+                    if (bits == 2)
+                        return __byte_perm((j & 1 ? w[j / 8] >> 4 : w[j / 8]) & 0x0f0f0f0fu, 0,
+                                           0x4404 | ((j % 8 / 2) << 4));
                     const int at = 2 * bits * j, i = at / 32, sh = at % 32;
                     const uint32_t x = sh + 2 * bits <= 32 ? w[i] >> sh : __funnelshift_r(w[i], w[i + 1], sh);
                     return (x & ((1u << (2 * bits)) - 1u)) << 8;
@@ -998,6 +1060,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                 const int i = step & 1;
                 wait(p_ready(i), i ? np[1]++ : np[0]++);
                 if (lost) break;
+                // the stream's next scores first: S is read, P waits for pv_done
+                if (step + 2 < steps) scores(step + 2);
                 tc_fence_after();
                 if (elect_one()) {
                     const uint64_t v = v_desc + st_pv * (MANY_KV >> 4);
@@ -1006,11 +1070,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                         tc_mma_ts(tmem + 256 * i + 192, tmem + 256 * i + 128 + 8 * x, v + 128 * x, ipv,
                                   step >= 2 || x > 0);
                     if (!ROWS || i == 1) tc_commit(empty(st_pv));
-                    if (step + 2 >= steps) tc_commit(s_ready(i));        // the stream's sums are complete
+                    tc_commit(pv_done(i));
                 }
                 __syncwarp();
                 if (!ROWS || i == 1) st_pv = st_pv == MANY_STAGES - 1 ? 0 : st_pv + 1;
-                if (step + 2 < steps) scores(step + 2);
             }
             if (elect_one()) tc_commit(seg_done);
             __syncwarp();
@@ -1026,7 +1089,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
         const int i = warp / 4, row = tid - 128 * i;
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;   // lane 32 (warp % 4), in bits 16 up
         const uint32_t S = tmem + lanes + 256 * i, P = S + 128, O = S + 192;
-        int ns = 0;
+        int ns = 0, nv = 0;                                  // score and value products waited for
         for (int seg = 0; t < end && !lost; ++seg) {
             int64_t next;
             const Segment s = segment_at(seqs, a.n_seqs, g, RU, t, end, cta, &next);
@@ -1042,33 +1105,38 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                 wait(s_ready(i), ns++);
                 if (lost) break;
                 tc_fence_after();
+                // P and O are this stream's again once its last value product is done
+                bool have = n == 0;
+                auto p_free = [&] {
+                    if (!have) wait(pv_done(i), nv++);
+                    have = true;
+                    return !lost;
+                };
                 if (any_row) {
-                    float sum;
-                    if (t0 + MANY_TILE <= sq.context) {
-                        // the exponentials are taken under the maximum so far,
-                        // and again in the rare case that it was too low
+                    float sum = 0.0f;
+                    auto step = [&](auto masked) {
+                        constexpr bool M = decltype(masked)::value;
+                        // the exponentials are taken under the maximum so far, and
+                        // again in the rare case that it was too low
                         bool over = true;
-                        if (n > 0) over = weigh<false>(S, P, ref, sum, nullptr, 0, 0);
-                        if (over) {
-                            raise<false>(S, O, n > 0, ref, l, nullptr, 0, 0);
-                            weigh<false>(S, P, ref, sum, nullptr, 0, 0);
+                        if (n > 0) over = weigh<M>(S, P, ref, sum, mk, sq.nodes, t0 - sq.context, p_free);
+                        if (over && !lost) {
+                            raise<M>(S, O, n > 0, ref, l, mk, sq.nodes, t0 - sq.context);
+                            weigh<M>(S, P, ref, sum, mk, sq.nodes, t0 - sq.context, p_free);
                         }
-                    } else {
-                        bool over = true;
-                        if (n > 0) over = weigh<true>(S, P, ref, sum, mk, sq.nodes, t0 - sq.context);
-                        if (over) {
-                            raise<true>(S, O, n > 0, ref, l, mk, sq.nodes, t0 - sq.context);
-                            weigh<true>(S, P, ref, sum, mk, sq.nodes, t0 - sq.context);
-                        }
-                    }
+                    };
+                    if (t0 + MANY_TILE <= sq.context) step(std::false_type());
+                    else step(std::true_type());
                     l += sum;
                     tc_wait_st();
+                } else {
+                    p_free();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(p_ready(i));
             }
-            if (steps) wait(s_ready(i), ns++);
+            if (steps) wait(pv_done(i), nv++);
             tc_fence_after();
             if (lost) break;
             // this row's sums out
