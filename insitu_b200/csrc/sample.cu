@@ -10,10 +10,12 @@
 // No sort: both cuts are order statistics (by count, by mass), found by
 // histograms that narrow a range of values. The row's logits are read from
 // memory once, into the shared memory of a thread-block cluster (each CTA a
-// contiguous slice of the vocabulary); the later passes read them there, and
-// the CTAs exchange histograms through distributed shared memory. A cut needs
-// the exact order of the values, so the histograms' last levels work on the
-// values' bits, and on the indexes where equal values are split.
+// contiguous slice of the vocabulary), and the CTAs exchange histograms through
+// distributed shared memory. The cuts run over the few tokens within 10 nats
+// of the maximum, which one pass lists, where those decide them (they hold the
+// k-th largest, the mass), else over the whole slice. The histograms' last
+// levels work on the values' bits, and on the indexes where equal values are
+// split, so the order is exact.
 //
 // Masses are summed as integers, w_i rounded to 2^-31 (64-bit totals): the
 // result then does not depend on the order of the atomics, and the rounding
@@ -21,7 +23,9 @@
 // 128,000 tokens by some 1e-8 of it.
 //
 // Bound: one read of the logits (and of the random numbers, where a row is
-// not filtered); at a few rows the passes' latency.
+// not filtered); at a few rows the passes' latency. Histograms over the whole
+// slice alone, with exact divisions, took 322 us for 256 rows of 128,000
+// (186 instructions a logit).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,6 +40,8 @@ namespace cg = cooperative_groups;
 constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32, SMP_BINS = 256;
 constexpr int SMP_MAX_VOCAB = 1 << 18;
 constexpr int SMP_WINDOWS = 4;               // first-level windows of 8 nats each, the last one open
+constexpr int SMP_LIST = 2048;               // tokens a CTA can list
+constexpr float SMP_NEAR = 10.0f;            // nats below the maximum that are listed
 
 struct SampleArgs {
     const void *logits;
@@ -53,9 +59,6 @@ __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// Logits as the order sees them: NaN counts as masked (-inf), -0 as 0.
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.0f; }
-
 // Unsigned integers in the order of the floats.
 __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x);
@@ -69,11 +72,11 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // cluster barrier a step is enough.
 struct SampleShared {
     uint32_t cnt[2][SMP_BINS], lo[2][SMP_BINS], hi[2][SMP_BINS];
-    unsigned long long sum[2];
+    unsigned long long sum[2], sum2[2];
     float val[2];
     int32_t idx[2];
     // this CTA only
-    unsigned long long wsum[SMP_WARPS];
+    unsigned long long wsum[SMP_WARPS], wsum2[SMP_WARPS];
     float wval[SMP_WARPS];
     int32_t widx[SMP_WARPS];
     uint32_t scan_c[SMP_BINS / 32];
@@ -82,53 +85,155 @@ struct SampleShared {
     uint32_t hit_cnt, hit_before_c;
     unsigned long long hit_mass, hit_before_m;
     uint32_t key_lo, key_hi;
+    int32_t listed;
+    float list_x[SMP_LIST];
+    int32_t list_i[SMP_LIST];
 };
 
+// The largest of a 16-byte vector's elements (NaN ignored).
+__device__ __forceinline__ float vec_max(const uint4 &v, const float *) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
+__device__ __forceinline__ float vec_max(const uint4 &v, const __half *) {
+    const __half2 *h = reinterpret_cast<const __half2 *>(&v);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float vec_max(const uint4 &v, const __nv_bfloat16 *) {
+    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+
+// A slice in shared memory: `head` single elements, `body` 16-byte vectors,
+// single elements again, at the alignment within 16 bytes that the row has in
+// global memory.
+template <typename T>
+struct Slice {
+    static constexpr int V = 16 / sizeof(T);
+    T *at;
+    const uint4 *vec;                        // the body, 16-byte aligned also where it is empty
+    int n, head, body;
+
+    // Copies n elements from global memory; returns this thread's largest.
+    __device__ __forceinline__ float stage(uint8_t *smem, const T *src, int count) {
+        const int shift = (int)(((uintptr_t)src & 15u) / sizeof(T));
+        at = reinterpret_cast<T *>(smem) + shift;
+        n = count;
+        head = min(n, (V - shift) % V);
+        body = (n - head) / V;
+        float top = -INFINITY;
+        const uint4 *vs = reinterpret_cast<const uint4 *>(((uintptr_t)src + 15u) & ~(uintptr_t)15u);
+        uint4 *vd = reinterpret_cast<uint4 *>(smem + (shift ? 16 : 0));
+        vec = vd;
+        int i = threadIdx.x;
+        for (; i + 7 * SMP_THREADS < body; i += 8 * SMP_THREADS) {
+            uint4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = __ldcs(vs + i + k * SMP_THREADS);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                vd[i + k * SMP_THREADS] = v[k];
+                top = fmaxf(top, vec_max(v[k], at));
+            }
+        }
+#pragma unroll 4
+        for (; i < body; i += SMP_THREADS) {
+            const uint4 v = __ldcs(vs + i);
+            vd[i] = v;
+            top = fmaxf(top, vec_max(v, at));
+        }
+        for (int k = threadIdx.x; k < n - body * V; k += SMP_THREADS) {
+            const int e = k < head ? k : k + body * V;
+            at[e] = src[e];
+            top = fmaxf(top, to_f32(at[e]));
+        }
+        __syncthreads();
+        return top;
+    }
+    // f(x, i) for each element whose value is at least `from` (never a NaN, and
+    // -0 as 0).
+    template <typename F>
+    __device__ __forceinline__ void above(float from, F &&f) const {
+        for (int i = threadIdx.x; i < body; i += SMP_THREADS) {
+            const uint4 v = vec[i];
+            if (!(vec_max(v, at) >= from)) continue;
+            const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float x = to_f32(e[k]);
+                if (x >= from) f(x + 0.0f, head + i * V + k);
+            }
+        }
+        for (int k = threadIdx.x; k < n - body * V; k += SMP_THREADS) {
+            const int e = k < head ? k : k + body * V;
+            const float x = to_f32(at[e]);
+            if (x >= from) f(x + 0.0f, e);
+        }
+    }
+};
+
+// A row's tokens as the cuts see them: the CTA's slice, or its list.
 template <typename T>
 struct Row {
     SampleShared &sm;
     cg::cluster_group cl;
-    const T *slice;                          // this CTA's logits, in shared memory
-    int n, first, parity, C;
-    float xmax, z0, t;
+    Slice<T> slice;                          // this CTA's logits, in shared memory
+    int n, first, parity, C;                 // n: tokens listed
+    float xmax, inv_t, bins;                 // 1 / t; first-level bins a unit of x
     // kept so far: value key above thr_key, or equal to it at an index up to thr_idx
     uint32_t thr_key;
     int32_t thr_idx;
+    bool list;
 
-    __device__ __forceinline__ float x_at(int i) const { return clean(to_f32(slice[i])); }
-    __device__ __forceinline__ float z_of(float x) const {
-        const float z = __fsub_rn(__fdiv_rn(x, t), z0);
-        return x == xmax ? 0.0f : z == z ? z : -INFINITY;   // both quotients beyond the float range: NaN
+    // f(x, key, index) for each kept token that is not below `from`
+    template <typename F>
+    __device__ __forceinline__ void each(float from, F &&f) const {
+        auto token = [&](float x, int i) {
+            const uint32_t key = order_key(x);
+            if (key > thr_key || (key == thr_key && i <= thr_idx)) f(x, key, i);
+        };
+        if (list) {
+            for (int i = threadIdx.x; i < n; i += SMP_THREADS)
+                if (sm.list_x[i] >= from) token(sm.list_x[i], sm.list_i[i]);
+        } else {
+            slice.above(fmaxf(from, -3.4028235e38f), [&](float x, int i) { token(x, first + i); });
+        }
     }
-    __device__ __forceinline__ bool kept(float x, uint32_t key, int i) const {
-        return x > -INFINITY && (key > thr_key || (key == thr_key && first + i <= thr_idx));
+    // z and w: 2^-23 of z from the two roundings, 2^-22 of w from the exponential
+    __device__ __forceinline__ float z_of(float x) const { return x == xmax ? 0.0f : (x - xmax) * inv_t; }
+    __device__ __forceinline__ float w_of(float z) const {
+        float w;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(z * 1.4426950408889634f));
+        return w;
     }
     // w in units of 2^-31
     __device__ __forceinline__ uint32_t mass_of(float x) const {
-        return __float2uint_rn(expf(z_of(x)) * 2147483648.0f);
+        return __float2uint_rn(w_of(z_of(x)) * 2147483648.0f);
     }
     // First-level bin: the distance below the maximum in 1/32 of t. Rounding
     // is monotone, so the bins are ranges of values.
     __device__ __forceinline__ int bin_of(float x) const {
         const float d = x == xmax ? 0.0f : xmax - x;
-        return min(__float2int_rz(d * __fdiv_rn(32.0f, t)), SMP_WINDOWS * SMP_BINS - 1);
+        return min(__float2int_rz(d * bins), SMP_WINDOWS * SMP_BINS - 1);
     }
 
-    // Sums of the cluster, for every thread.
-    __device__ unsigned long long cluster_sum(unsigned long long v) {
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
-        if (threadIdx.x % 32 == 0) sm.wsum[threadIdx.x / 32] = v;
+    // Two sums of the cluster, for every thread.
+    __device__ void cluster_sum(unsigned long long &v, unsigned long long &u) {
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o), u += __shfl_xor_sync(FULL, u, o);
+        if (threadIdx.x % 32 == 0) sm.wsum[threadIdx.x / 32] = v, sm.wsum2[threadIdx.x / 32] = u;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            unsigned long long s = 0;
-            for (int w = 0; w < SMP_WARPS; ++w) s += sm.wsum[w];
-            sm.sum[parity] = s;
+        if (threadIdx.x < 32) {
+            v = threadIdx.x < SMP_WARPS ? sm.wsum[threadIdx.x] : 0;
+            u = threadIdx.x < SMP_WARPS ? sm.wsum2[threadIdx.x] : 0;
+            for (int o = SMP_WARPS / 2; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o), u += __shfl_xor_sync(FULL, u, o);
+            if (threadIdx.x == 0) sm.sum[parity] = v, sm.sum2[parity] = u;
         }
         cl.sync();
-        unsigned long long s = 0;
-        for (int r = 0; r < C; ++r) s += *cl.map_shared_rank(&sm.sum[parity], r);
+        v = u = 0;
+        for (int r = 0; r < C; ++r)
+            v += *cl.map_shared_rank(&sm.sum[parity], r), u += *cl.map_shared_rank(&sm.sum2[parity], r);
         parity ^= 1;
-        return s;
     }
     // The largest value of the cluster and the lowest index that has it.
     __device__ void cluster_best(float &v, int &i) {
@@ -140,11 +245,15 @@ struct Row {
         }
         if (threadIdx.x % 32 == 0) sm.wval[threadIdx.x / 32] = v, sm.widx[threadIdx.x / 32] = i;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < SMP_WARPS; ++w)
-                if (better(sm.wval[w], sm.widx[w], v, i)) v = sm.wval[w], i = sm.widx[w];
-            sm.val[parity] = v;
-            sm.idx[parity] = i;
+        if (threadIdx.x < 32) {
+            v = threadIdx.x < SMP_WARPS ? sm.wval[threadIdx.x] : -INFINITY;
+            i = threadIdx.x < SMP_WARPS ? sm.widx[threadIdx.x] : INT_MAX;
+            for (int o = SMP_WARPS / 2; o; o >>= 1) {
+                const float ov = __shfl_xor_sync(FULL, v, o);
+                const int oi = __shfl_xor_sync(FULL, i, o);
+                if (better(ov, oi, v, i)) v = ov, i = oi;
+            }
+            if (threadIdx.x == 0) sm.val[parity] = v, sm.idx[parity] = i;
         }
         cl.sync();
         v = -INFINITY, i = INT_MAX;
@@ -252,12 +361,14 @@ struct Row {
         int bin = SMP_BINS, win = 0;
         for (; win < SMP_WINDOWS; ++win) {
             clear();
-            for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
-                const float x = x_at(i);
-                if (!kept(x, order_key(x), i)) continue;
+            // (the margin covers the bins' roundings)
+            const float from = win + 1 < SMP_WINDOWS
+                                   ? xmax - (win + 1) * SMP_BINS * 1.0001f / bins - 1e-6f * fabsf(xmax)
+                                   : -INFINITY;
+            each(from, [&](float x, uint32_t, int) {
                 const int b = bin_of(x) - win * SMP_BINS;
                 if (b >= 0 && b < SMP_BINS) count(b, BY_MASS ? mass_of(x) : 0u);
-            }
+            });
             bin = crossing<BY_MASS>(need_c, need_m, before_c, before_m, in_c);
             need_c -= before_c;
             need_m -= before_m;
@@ -278,12 +389,9 @@ struct Row {
         while (a < b && !whole()) {
             const int sh = max(0, 32 - __clz(b - a) - 8);
             clear();
-            for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
-                const float x = x_at(i);
-                const uint32_t key = order_key(x);
-                if (key < a || key > b || !kept(x, key, i)) continue;
-                count((int)((b - key) >> sh), BY_MASS ? mass_of(x) : 0u);
-            }
+            each(key_value(a), [&](float x, uint32_t key, int) {
+                if (key >= a && key <= b) count((int)((b - key) >> sh), BY_MASS ? mass_of(x) : 0u);
+            });
             const int c = crossing<BY_MASS>(need_c, need_m, before_c, before_m, in_c);
             need_c -= before_c;
             need_m -= before_m;
@@ -302,11 +410,9 @@ struct Row {
             while (need != in_c && ia < ib) {
                 const int sh = max(0, 32 - __clz(ib - ia) - 8);
                 clear();
-                for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
-                    const float x = x_at(i);
-                    if (order_key(x) != a || first + i < ia || first + i > ib || !kept(x, a, i)) continue;
-                    count((first + i - ia) >> sh, 0u);
-                }
+                each(key_value(a), [&](float, uint32_t key, int i) {
+                    if (key == a && i >= ia && i <= ib) count((i - ia) >> sh, 0u);
+                });
                 const int c = crossing<false>(need, 0, before_c, before_m, in_c);
                 need -= before_c;
                 ia += c << sh;
@@ -320,24 +426,6 @@ struct Row {
     }
 };
 
-// Copies n elements from global memory into shared memory at the same
-// alignment within 16 bytes; returns where they start.
-template <typename T>
-__device__ __forceinline__ const T *stage_slice(uint8_t *smem, const T *src, int n) {
-    constexpr int V = 16 / sizeof(T);
-    const int shift = (int)(((uintptr_t)src & 15u) / sizeof(T));
-    T *dst = reinterpret_cast<T *>(smem) + shift;
-    const int head = min(n, (V - shift) % V), body = (n - head) / V;
-    for (int i = threadIdx.x; i < head; i += SMP_THREADS) dst[i] = src[i];
-    const uint4 *vs = reinterpret_cast<const uint4 *>(src + head);
-    uint4 *vd = reinterpret_cast<uint4 *>(dst + head);
-#pragma unroll 8
-    for (int i = threadIdx.x; i < body; i += SMP_THREADS) vd[i] = __ldcs(vs + i);
-    for (int i = head + body * V + threadIdx.x; i < n; i += SMP_THREADS) dst[i] = src[i];
-    __syncthreads();
-    return dst;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(SMP_THREADS) k_sample(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t dyn[];
@@ -347,20 +435,22 @@ __global__ void __launch_bounds__(SMP_THREADS) k_sample(const SampleArgs a) {
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int64_t row = blockIdx.x / C;
     const int first = min(rank * a.slice, a.vocab), n = min(a.slice, a.vocab - first);
-    const T *src = reinterpret_cast<const T *>(a.logits) + row * a.stride + first;
-    Row<T> R{sm, cl, stage_slice<T>(dyn, src, n), n, first, 0, C, 0.0f, 0.0f, 1.0f, 0u, INT_MAX};
-
-    float best = -INFINITY;
-    int at = INT_MAX;
-    for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
-        const float x = R.x_at(i);
-        if (x > best) best = x, at = first + i;
-    }
-    R.cluster_best(best, at);
     const float t = a.temperature ? a.temperature[row] : 1.0f;
-    if (!(best > -INFINITY) || !(t > 0.0f)) {
-        // nothing to choose from, or the largest logit
-        const bool none = !(best > -INFINITY);
+    const int k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.0f, floor_w = a.min_p ? a.min_p[row] : 0.0f;
+    if (threadIdx.x == 0) sm.listed = 0;
+    Slice<T> slice;
+    float best = slice.stage(dyn, reinterpret_cast<const T *>(a.logits) + row * a.stride + first, n);
+    Row<T> R{sm, cl, slice, 0, first, 0, C, 0.0f, 1.0f, 32.0f, 0u, INT_MAX, false};
+    int at = INT_MAX;
+    R.cluster_best(best, at);
+    best += 0.0f;
+    const bool none = !(best > -INFINITY);
+    if (none || !(t > 0.0f)) {
+        // nothing to choose from, or the largest logit at its lowest index
+        float v = -INFINITY;
+        if (!none) slice.above(best, [&](float x, int i) { v = x, at = min(at, first + i); });
+        R.cluster_best(v, at);
         if (rank == 0 && threadIdx.x == 0) {
             a.tokens[row] = none ? -1 : at;
             if (a.logprobs) a.logprobs[row] = none ? -INFINITY : 0.0f;
@@ -369,38 +459,93 @@ __global__ void __launch_bounds__(SMP_THREADS) k_sample(const SampleArgs a) {
         return;
     }
     R.xmax = best;
-    R.t = t;
-    R.z0 = __fdiv_rn(best, t);
-    const int k = a.top_k ? a.top_k[row] : 0;
-    const float p = a.top_p ? a.top_p[row] : 1.0f, floor_w = a.min_p ? a.min_p[row] : 0.0f;
-    if (k > 0 && k < a.vocab) R.template cut<false>((uint32_t)k, 0);
-    if (p < 1.0f) {
-        unsigned long long mass = 0;
-        for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
-            const float x = R.x_at(i);
-            if (R.kept(x, order_key(x), i)) mass += R.mass_of(x);
+    R.inv_t = __fdiv_rn(1.0f, t);
+    R.bins = __fdiv_rn(32.0f, t);
+    const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1.0f;
+    unsigned long long total = 0;            // mass of all tokens, where top_p cuts them
+    if (by_count || by_mass || floor_w > 0.0f) {
+        // List the tokens near the maximum. What top_p takes its share of (all
+        // tokens: w below 2^-32, 22.2 nats away, counts as 0) is summed in the
+        // same pass.
+        const bool sum_all = by_mass && !by_count;
+        float near = SMP_NEAR;
+        if (!by_count && !by_mass) near = -logf(floor_w) + 0.01f;        // min_p alone cuts there
+        const float list_from = best - near * t;
+        const float from = sum_all ? fminf(list_from, best - 22.2f * t) : list_from;
+        unsigned long long mass = 0, listed = 0;
+        slice.above(fmaxf(from, -3.4028235e38f), [&](float x, int i) {
+            const uint32_t m = by_mass ? R.mass_of(x) : 0u;
+            mass += m;
+            if (x < list_from) return;
+            const int to = atomicAdd(&sm.listed, 1);
+            if (to < SMP_LIST) sm.list_x[to] = x, sm.list_i[to] = first + i;
+        });
+        __syncthreads();
+        // tokens listed in the low half, CTAs whose list ran over in the high one
+        const int mine = sm.listed;
+        if (threadIdx.x == 0) listed = (unsigned long long)mine + ((unsigned long long)(mine > SMP_LIST) << 32);
+        total = mass;
+        R.cluster_sum(total, listed);
+        bool enough = listed >> 32 == 0;
+        if (by_count) enough &= listed >= (unsigned long long)k;
+        if (enough && sum_all) {
+            unsigned long long in = 0, unused = 0;
+            for (int i = threadIdx.x; i < mine; i += SMP_THREADS) in += R.mass_of(sm.list_x[i]);
+            R.cluster_sum(in, unused);
+            enough = (double)in >= ceil((double)p * (double)total);
         }
-        mass = R.cluster_sum(mass);
-        const double want = ceil((double)p * (double)mass);
+        if (enough) R.list = true, R.n = mine;
+    }
+    if (by_count) R.template cut<false>((uint32_t)k, 0);
+    if (by_mass) {
+        if (by_count) {
+            unsigned long long unused = 0;
+            total = 0;
+            R.each(-INFINITY, [&](float x, uint32_t, int) { total += R.mass_of(x); });
+            R.cluster_sum(total, unused);
+        }
+        const double want = ceil((double)p * (double)total);
         R.template cut<true>(0, want > 1.0 ? (unsigned long long)want : 1ull);
     }
-    unsigned long long mass = 0;
-    float key = -INFINITY, z_key = 0.0f;
+    unsigned long long mass = 0, unused = 0;
+    float key = -INFINITY, z_key = 0.0f, reach = INFINITY;
     int token = INT_MAX;
-    const float *u = a.uniform + row * a.u_stride + first;
-    for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
-        const float x = R.x_at(i);
-        if (!R.kept(x, order_key(x), i)) continue;
-        const float z = R.z_of(x), w = expf(z);
-        if (!(w >= floor_w)) continue;
+    const float *u = a.uniform + row * a.u_stride;
+    auto draw = [&](float x, float un, int i) {
+        const float z = R.z_of(x), w = R.w_of(z);
+        if (!(w >= floor_w)) return;
         mass += __float2uint_rn(w * 2147483648.0f);
-        float r = z - logf(-logf(__ldcs(u + i)));
+        // z - log(-log u) beats `key` only where -log u < w exp(-key), and
+        // 1 - u <= -log u: most tokens need no logarithm (the margin covers
+        // the roundings)
+        if (1.0f - un > w * reach) return;
+        float r = z - logf(-logf(un));
         r = r == r ? r : -INFINITY;                        // a random number outside [0, 1]
-        if (r > key || token == INT_MAX) key = r, token = first + i, z_key = z;
+        if (r > key || token == INT_MAX || (r == key && i < token)) {
+            key = r, token = i, z_key = z;
+            reach = 1.001f * expf(-key);                   // infinite for -inf: no bound
+        }
+    };
+    if (R.list || R.thr_key) {
+        R.each(R.thr_key ? key_value(R.thr_key) : -INFINITY,
+               [&](float x, uint32_t, int i) { draw(x, __ldcs(u + i), i); });
+    } else {
+        u += first;
+        for (int i = threadIdx.x; i < n; i += 8 * SMP_THREADS) {
+            float un[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) un[k] = i + k * SMP_THREADS < n ? __ldcs(u + i + k * SMP_THREADS) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int e = i + k * SMP_THREADS;
+                const float x = e < n ? to_f32(slice.at[e]) : -INFINITY;
+                if (x > -INFINITY) draw(x + 0.0f, un[k], first + e);
+            }
+        }
     }
     const int mine = token;
     R.cluster_best(key, token);
-    mass = R.cluster_sum(mass);
+    R.cluster_sum(mass, unused);
     if (mine == token && token != INT_MAX) {
         a.tokens[row] = token;
         if (a.logprobs) a.logprobs[row] = (float)((double)z_key - log((double)mass * 0x1p-31));
