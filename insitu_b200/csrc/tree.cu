@@ -85,9 +85,15 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// A word of the constant tables (not volatile: loads may be batched).
+__device__ __forceinline__ uint32_t load_shared(uint32_t at) {
+    uint32_t x;
+    asm("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at));
+    return x;
+}
 // c += a b, one 16x8 tile of 16-wide products
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -129,7 +135,7 @@ __device__ __forceinline__ int find_seq(const TreeSeq *seqs, int n, int i) {
 // adjacent channels (one run of its bits), of its value 8 adjacent channels,
 // and the query fragments are laid out to match. A pair of key codes is one
 // index into a table of half2 with a copy for each lane (32 banks: no
-// conflicts); 2-bit values are picked from two registers by byte permutes.
+// conflicts), and so is a pair of value codes of two tokens.
 // Norms stay factored out: the key's scales the score, the value's the
 // probability.
 //
@@ -146,16 +152,21 @@ struct FewLayout {
     static constexpr bool PAIRS = KB != 0;                       // else one code at a time, any width
     static constexpr int K_ENTRIES = PAIRS ? 1 << (2 * KB) : 0;
     static constexpr int V_ENTRIES = PAIRS && VB > 2 ? 1 << (2 * VB) : 0;
-    static constexpr int KLUT = K_ENTRIES * 128, VLUT = V_ENTRIES * 128, SINGLE = PAIRS ? 0 : 1024;
-    static constexpr int STAGES_AT = KLUT + VLUT + SINGLE;
+    // 4b/2b: a key entry's 32 lanes' copies fill 128 of its 256 bytes, so that
+    // one byte permute makes an entry's address of a code byte; the other 128
+    // hold value pairs (entries a + 16 b < 64) and, from entry 64 on, the norms
+    static constexpr bool WIDE = KB == 4 && VB == 2;
+    static constexpr int KLUT = K_ENTRIES * (WIDE ? 256 : 128), VLUT = V_ENTRIES * 128, SINGLE = PAIRS ? 0 : 1024;
+    static constexpr int NORMS_AT = KLUT + VLUT + SINGLE;        // [warps][64] (key, value) norms, where not WIDE
+    __host__ __device__ static constexpr int stages_at(int warps) { return NORMS_AT + (WIDE ? 0 : warps * 512); }
     __host__ __device__ static int stage_bytes(const Geo &g) { return FEW_TILE * (g.kbytes + g.vbytes + 4); }
     __host__ __device__ static int bars_at(const Geo &g, int warps) {
-        return STAGES_AT + warps * FEW_STAGES * stage_bytes(g);
+        return stages_at(warps) + warps * FEW_STAGES * stage_bytes(g);
     }
     // the end-of-loop join reuses the stages: [warps][rows][64] floats, [warps][rows][2]
     __host__ static size_t bytes(const Geo &g, int warps, int rows) {
         const size_t loop = (size_t)bars_at(g, warps) + warps * FEW_STAGES * 8;
-        const size_t join = (size_t)STAGES_AT + (size_t)warps * rows * (64 + 2) * 4;
+        const size_t join = (size_t)stages_at(warps) + (size_t)warps * rows * (64 + 2) * 4;
         return std::max(loop, join);
     }
 };
@@ -170,18 +181,22 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
     const uint32_t sm0 = smem_u32(sm);
     const int kbytes = KB ? KB * 8 : g.kbytes, vbytes = VB ? VB * 8 : g.vbytes;
     const int stage = FEW_TILE * (kbytes + vbytes + 4);
-    const uint32_t ring = sm0 + L::STAGES_AT + warp * FEW_STAGES * stage;
+    const uint32_t ring = sm0 + L::stages_at(NW) + warp * FEW_STAGES * stage;
     const uint32_t bars = sm0 + L::bars_at(g, NW) + warp * FEW_STAGES * 8;
 
     // tables: constant, so filled before the wait for earlier launches
     const float cunit = exp2f((float)-g.centroid_frac);
     if (L::PAIRS) {
-        float *cent = reinterpret_cast<float *>(sm + L::STAGES_AT);
+        float *cent = reinterpret_cast<float *>(sm + L::stages_at(NW));
         if (tid < (1 << KB)) cent[tid] = (float)a.tb->k_cent[tid] * cunit;
         if (tid >= 32 && tid < 32 + (1 << VB)) cent[tid] = (float)a.tb->v_cent[tid - 32] * cunit;
         __syncthreads();
         for (int e = warp; e < L::K_ENTRIES; e += NW)
-            reinterpret_cast<uint32_t *>(sm)[e * 32 + lane] = pack_half2(cent[e & ((1 << KB) - 1)], cent[e >> KB]);
+            reinterpret_cast<uint32_t *>(sm)[e * (L::WIDE ? 64 : 32) + lane] =
+                pack_half2(cent[e & ((1 << KB) - 1)], cent[e >> KB]);
+        if (L::WIDE)
+            for (int e = warp; e < 64; e += NW)
+                reinterpret_cast<uint32_t *>(sm)[e * 64 + 32 + lane] = pack_half2(cent[32 + (e & 3)], cent[32 + (e >> 4)]);
         for (int e = warp; e < L::V_ENTRIES; e += NW)
             reinterpret_cast<uint32_t *>(sm + L::KLUT)[e * 32 + lane] =
                 pack_half2(cent[32 + (e & ((1 << VB) - 1))], cent[32 + (e >> VB)]);
@@ -190,13 +205,6 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         for (int i = tid; i < 512; i += NW * 32)
             tab[i] = __float2half_rn((float)(i < 256 ? a.tb->k_cent[i] : a.tb->v_cent[i - 256]) * cunit);
     }
-    uint32_t v_lo = 0, v_hi = 0;                     // the four 2-bit value centroids' low and high bytes
-    if (VB == 2)
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t h = __half_as_ushort(__float2half_rn((float)a.tb->v_cent[i] * cunit));
-            v_lo |= (h & 255u) << (8 * i);
-            v_hi |= (h >> 8) << (8 * i);
-        }
     if (lane == 0)
         for (int i = 0; i < FEW_STAGES; ++i) bar_init(bars + i * 8, 1);
     bar_init_fence();
@@ -269,6 +277,9 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         l[m][0] = l[m][1] = 0.0f;
     }
     const float nunit = exp2f((float)-g.norm_frac);
+    // this warp's norms of a tile: 16 tokens' (key, value) in each 128 bytes
+    uint8_t *norms = sm + (L::WIDE ? (64 + warp * 4) * 256 + 128 : L::NORMS_AT + warp * 512);
+    constexpr int nstride = L::WIDE ? 256 : 128;
     bool lost = false;
     int issued = 0;
     for (; issued < FEW_STAGES - 1; ++issued) issue(issued);
@@ -282,6 +293,15 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         }
         const uint8_t *st = sm + (ring - sm0) + (n % FEW_STAGES) * stage;
         const uint8_t *sv = st + FEW_TILE * kbytes, *sn = sv + FEW_TILE * vbytes;
+        // the tile's norms as floats, once
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int tok = lane + 32 * i;
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(sn + tok * 4);
+            *reinterpret_cast<float2 *>(norms + (tok / 16) * nstride + (tok % 16) * 8) =
+                make_float2(norm_value(w & 0xffffu, nunit), norm_value(w >> 16, nunit));
+        }
+        __syncwarp();
         const int p0 = lo + j * FEW_TILE, live = min(FEW_TILE, hi - p0);
         const bool masked = p0 + FEW_TILE > sq.context;
 #pragma unroll 1
@@ -295,21 +315,16 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                     const uint2 w = *reinterpret_cast<const uint2 *>(st + tok * 32 + t4 * 8);
                     const uint32_t lut = sm0 + lane * 4;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t word = i < 4 ? w.x : w.y;
-                        const int s = 8 * (i & 3);
-                        const uint32_t off = (s < 7 ? word << (7 - s) : word >> (s - 7)) & 0x7f80u;
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(kf[nt][i / 2][i % 2]) : "r"(lut + off));
-                    }
+                    for (int i = 0; i < 8; ++i)
+                        kf[nt][i / 2][i % 2] =
+                            load_shared(lut + __byte_perm(i < 4 ? w.x : w.y, 0, 0x4404 | ((i & 3) << 4)));
                 } else if constexpr (KB == 3) {
                     const uint16_t *p = reinterpret_cast<const uint16_t *>(st + tok * 24 + t4 * 6);
                     const uint64_t w = (uint64_t)p[0] | (uint64_t)p[1] << 16 | (uint64_t)p[2] << 32;
                     const uint32_t lut = sm0 + lane * 4;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        asm volatile("ld.shared.u32 %0, [%1];"
-                                     : "=r"(kf[nt][i / 2][i % 2])
-                                     : "r"(lut + ((uint32_t)(w >> (6 * i)) & 63u) * 128u));
+                        kf[nt][i / 2][i % 2] = load_shared(lut + ((uint32_t)(w >> (6 * i)) & 63u) * 128u);
                 } else {
                     const uint8_t *row = st + tok * kbytes;
                     const uint16_t *tab = reinterpret_cast<const uint16_t *>(sm);
@@ -324,11 +339,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
             float kn[4], vn[4];
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(sn + (s16 + nt * 8 + 2 * t4) * 4);
-                kn[2 * nt] = norm_value(w.x & 0xffffu, nunit);
-                vn[2 * nt] = norm_value(w.x >> 16, nunit);
-                kn[2 * nt + 1] = norm_value(w.y & 0xffffu, nunit);
-                vn[2 * nt + 1] = norm_value(w.y >> 16, nunit);
+                const float4 w = *reinterpret_cast<const float4 *>(norms + (s16 / 16) * nstride + (nt * 8 + 2 * t4) * 8);
+                kn[2 * nt] = w.x, vn[2 * nt] = w.y, kn[2 * nt + 1] = w.z, vn[2 * nt + 1] = w.w;
             }
             float s[MT][2][4];
             float top = -INFINITY;                    // largest excess over the running maximum
@@ -407,25 +419,30 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
             }
             // values: fragment rows (tokens) 2 t4, +1, +8, +9; column g8 of channel group c is channel 8 g8 + c
             if constexpr (VB == 2) {
-                uint32_t e[4], o[4];
+                // a byte of z: the codes of two channels of a token (low half)
+                // and of the next one (high half); even and odd channels apart,
+                // each byte is a value pair's entry
+                uint32_t e[2], o[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int tok = s16 + 2 * t4 + (i & 1) + (i >> 1) * 8;
-                    uint32_t x = *reinterpret_cast<const uint16_t *>(sv + tok * 16 + g8 * 2);
-                    x = (x | x << 8) & 0x00ff00ffu;
-                    x = (x | x << 4) & 0x0f0f0f0fu;       // a byte: the codes of channels 2i, 2i + 1
-                    e[i] = x & 0x03030303u;
-                    o[i] = (x >> 2) & 0x03030303u;
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t x[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int tok = s16 + 2 * t4 + k + i * 8;
+                        x[k] = __byte_perm(*reinterpret_cast<const uint16_t *>(sv + tok * 16 + g8 * 2), 0, 0x4140);
+                        x[k] = (x[k] | x[k] << 4) & 0x0f0f0f0fu;
+                    }
+                    const uint32_t z = x[1] * 16 + x[0];
+                    e[i] = z & 0x33333333u;
+                    o[i] = (z >> 2) & 0x33333333u;
                 }
+                const uint32_t lut = sm0 + lane * 4 + 128;
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     uint32_t b[2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t pair = __byte_perm(c & 1 ? o[2 * i] : e[2 * i], c & 1 ? o[2 * i + 1] : e[2 * i + 1],
-                                                          (c >> 1) | ((4 + (c >> 1)) << 4));
-                        b[i] = __byte_perm(v_lo, v_hi, pair * 0x11u + 0x4040u);
-                    }
+                    for (int i = 0; i < 2; ++i)
+                        b[i] = load_shared(lut + __byte_perm(c & 1 ? o[i] : e[i], 0, 0x4404 | ((c >> 1) << 4)));
 #pragma unroll
                     for (int m = 0; m < MT; ++m) mma16816(acc[m][c], pf[m], b[0], b[1]);
                 }
@@ -444,7 +461,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t idx = ((x[2 * i] >> (3 * c)) & 7u) | (((x[2 * i + 1] >> (3 * c)) & 7u) << 3);
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(b[i]) : "r"(lut + idx * 128u));
+                        b[i] = load_shared(lut + idx * 128u);
                     }
 #pragma unroll
                     for (int m = 0; m < MT; ++m) mma16816(acc[m][c], pf[m], b[0], b[1]);
@@ -475,7 +492,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
 
     // join the warps: each row's maximum, then the scaled sums
     __syncthreads();
-    float *jacc = reinterpret_cast<float *>(sm + L::STAGES_AT), *jml = jacc + NW * R * 64;
+    float *jacc = reinterpret_cast<float *>(sm + L::stages_at(NW)), *jml = jacc + NW * R * 64;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -800,12 +817,6 @@ __device__ __noinline__ void raise(uint32_t S, uint32_t O, bool scale, float &re
     tc_wait_st();
 }
 
-// A word of the constant tables (not volatile: loads may be batched).
-__device__ __forceinline__ uint32_t load_shared(uint32_t at) {
-    uint32_t x;
-    asm("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at));
-    return x;
-}
 // half2 x (hi + lo): a 16-bit norm needs two halves to be exact
 __device__ __forceinline__ uint32_t scale_half2(uint32_t x, __half2 hi, __half2 lo) {
     const __half2 v = *reinterpret_cast<const __half2 *>(&x);
