@@ -85,6 +85,11 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// Byte `i` of w times 256 plus `lane4` (below 256): the address of a code
+// byte's entry in a table of 256-byte entries, at this lane's copy.
+__device__ __forceinline__ uint32_t entry_at(uint32_t w, int i, uint32_t lane4) {
+    return __byte_perm(w, lane4, 0x5504 | (i << 4));
+}
 // A word of the constant tables (not volatile: loads may be batched).
 __device__ __forceinline__ uint32_t load_shared(uint32_t at) {
     uint32_t x;
@@ -280,6 +285,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
     // this warp's norms of a tile: 16 tokens' (key, value) in each 128 bytes
     uint8_t *norms = sm + (L::WIDE ? (64 + warp * 4) * 256 + 128 : L::NORMS_AT + warp * 512);
     constexpr int nstride = L::WIDE ? 256 : 128;
+    const uint32_t lane4 = lane * 4;
     bool lost = false;
     int issued = 0;
     for (; issued < FEW_STAGES - 1; ++issued) issue(issued);
@@ -313,11 +319,10 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                 const int tok = s16 + nt * 8 + g8;
                 if constexpr (KB == 4) {
                     const uint2 w = *reinterpret_cast<const uint2 *>(st + tok * 32 + t4 * 8);
-                    const uint32_t lut = sm0 + lane * 4;
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         kf[nt][i / 2][i % 2] =
-                            load_shared(lut + __byte_perm(i < 4 ? w.x : w.y, 0, 0x4404 | ((i & 3) << 4)));
+                            *reinterpret_cast<const uint32_t *>(sm + entry_at(i < 4 ? w.x : w.y, i & 3, lane4));
                 } else if constexpr (KB == 3) {
                     const uint16_t *p = reinterpret_cast<const uint16_t *>(st + tok * 24 + t4 * 6);
                     const uint64_t w = (uint64_t)p[0] | (uint64_t)p[1] << 16 | (uint64_t)p[2] << 32;
@@ -436,13 +441,13 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                     e[i] = z & 0x33333333u;
                     o[i] = (z >> 2) & 0x33333333u;
                 }
-                const uint32_t lut = sm0 + lane * 4 + 128;
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     uint32_t b[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
-                        b[i] = load_shared(lut + __byte_perm(c & 1 ? o[i] : e[i], 0, 0x4404 | ((c >> 1) << 4)));
+                        b[i] = *reinterpret_cast<const uint32_t *>(sm + 128 +
+                                                                   entry_at(c & 1 ? o[i] : e[i], c >> 1, lane4));
 #pragma unroll
                     for (int m = 0; m < MT; ++m) mma16816(acc[m][c], pf[m], b[0], b[1]);
                 }
@@ -905,7 +910,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
     if (warp >= 8 && warp < 12) {
         // ---- decode: thread `row` owns row `row` of each tile, a warp 32 of them
         const int row = tid - 256;
-        const uint32_t lut = sm0 + lane * 4;
+        const uint32_t lane4 = lane * 4;
         const uint32_t ring = sm0 + MANY_RING_AT + (warp - 8) * MANY_RING * MANY_SLOT;
         const float unit = exp2f((float)-g.norm_frac);
         int kt = 0, kr = 0;                                      // tiles so far; the ring slot of the segment's first
@@ -995,14 +1000,12 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                 const int st = kt % MANY_STAGES;
                 if (kt >= MANY_STAGES) wait(empty(st), kt / MANY_STAGES - 1);
                 const float kn = norm_value(cn & 0xffffu, unit), vn = norm_value(cn >> 16, unit);
-                auto codes = [&](const uint32_t *w, int bits, int j) -> uint32_t {   // pair j of 2-code fields, times 256
-                    if (bits == 4) return __byte_perm(w[j / 4], 0, 0x4404 | ((j % 4) << 4));
-                    if (bits == 2)
-                        return __byte_perm((j & 1 ? w[j / 8] >> 4 : w[j / 8]) & 0x0f0f0f0fu, 0,
-                                           0x4404 | ((j % 8 / 2) << 4));
+                auto codes = [&](const uint32_t *w, int bits, int j) -> uint32_t {   // pair j's entry, this lane's copy
+                    if (bits == 4) return entry_at(w[j / 4], j % 4, lane4);
+                    if (bits == 2) return entry_at((j & 1 ? w[j / 8] >> 4 : w[j / 8]) & 0x0f0f0f0fu, j % 8 / 2, lane4);
                     const int at = 2 * bits * j, i = at / 32, sh = at % 32;
                     const uint32_t x = sh + 2 * bits <= 32 ? w[i] >> sh : __funnelshift_r(w[i], w[i + 1], sh);
-                    return (x & ((1u << (2 * bits)) - 1u)) << 8;
+                    return (x & ((1u << (2 * bits)) - 1u)) << 8 | lane4;
                 };
                 auto put = [&](int base, const uint32_t *w, int bits, int off, float nrm) {
                     const __half2 hi = __float2half2_rn(nrm);
@@ -1011,7 +1014,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                     for (int c = 0; c < 8; c += 4) {
                         uint32_t v[16];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) v[j] = load_shared(lut + off + codes(w, bits, 4 * c + j));
+                        for (int j = 0; j < 16; ++j)
+                            v[j] = *reinterpret_cast<const uint32_t *>(sm + off + codes(w, bits, 4 * c + j));
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
 #pragma unroll
