@@ -12,13 +12,19 @@ reference's operator interfaces above it:
     CompressedAttention ops/attention.py
     DecodeAttention     the batched decode step below the seam (kernel.py:253-355)
     PagedCache          the C-ABI handle itself
+
+and adds what a serving loop needs next to them:
+
+    DraftTree           trees of drafted tokens, attended by PagedCache.tree_scan
+    Sampler             tokens from logits: temperature, top-k, top-p, min-p
+    (PagedCache)        fork, compact, truncate, rows, put_rows: page operations
 """
 
 from .config import FixedFormat, Geometry, QuantConfig
 
 __all__ = ["FixedFormat", "Geometry", "QuantConfig", "Rotation", "KVQuantizer", "CompressedKV",
            "KVCache", "CompressedCache", "CompressedAttention", "AttentionStats",
-           "DecodeAttention", "PagedCache", "AttentionLayer"]
+           "DecodeAttention", "PagedCache", "AttentionLayer", "DraftTree", "Sampler"]
 
 
 def __getattr__(name):
@@ -42,6 +48,12 @@ def __getattr__(name):
     if name == "DecodeAttention":
         from .decode import DecodeAttention
         return DecodeAttention
+    if name == "DraftTree":
+        from .tree import DraftTree
+        return DraftTree
+    if name == "Sampler":
+        from .sampling import Sampler
+        return Sampler
     if name == "PagedCache":
         from .engine import PagedCache
         return PagedCache

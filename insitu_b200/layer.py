@@ -92,6 +92,7 @@ class AttentionLayer:
         self._conv_n = torch.zeros(2, dtype=torch.int64, device=dev)
         self._conv_max = torch.zeros(1, dtype=torch.float64, device=dev)
         self._last_conv = None
+        self._drafted = None           # (context, nodes) of a verify that waits for its accept
 
     def forward(self, x, positions=None):
         """Rows of x are decode tokens, in order (a prefill when there are
@@ -123,6 +124,50 @@ class AttentionLayer:
         acc = merged.to(torch.float64) / float(1 << self.fmt.qk_frac)      # Q.to_float
         y = project(self.w_o, acc, self.b_o, rounded=True)
         return y, merged
+
+    # -- drafted trees -----------------------------------------------------------
+    def _qkv_wire(self, x, positions):
+        """Projections and the seam of x's rows: the wire q, k, v on the device."""
+        n = x.shape[0]
+        q, k, v = project(self.w_qkv, x, self.b_qkv, rounded=True).split(self._split, dim=1)
+        return self.seam(q.reshape(n, self.hq, self.d), k.reshape(n, self.hk, self.d), v.reshape(n, self.hk, self.d),
+                         positions, host_stats=False)
+
+    def verify(self, x, tree):
+        """The nodes of a drafted tree (an ``insitu_b200.tree.DraftTree`` of one
+        tree) in one pass: x (nodes, hidden) holds each node's input, its
+        position is its depth after the context, and it attends the context
+        and its ancestors (``tree_scan``, the floating-point form of the
+        cache's attention). The nodes' rows stay cached until ``accept`` says
+        which of them to keep. Returns y (nodes, hidden) fp32 and the
+        attention output (nodes, num_heads, head_dim) bf16."""
+        pc = self.dec.pc
+        if len(tree.counts) != 1 or tree.depths is None:
+            raise ValueError("verify takes one tree with parents")
+        x = torch.as_tensor(x).to(pc.device, torch.float32)
+        n = x.shape[0]
+        if n != tree.counts[0]:
+            raise ValueError(f"{n} inputs for a tree of {tree.counts[0]} nodes")
+        T = pc.length(self.seq)
+        wq, wk, wv, conv = self._qkv_wire(x, T + tree.depths - 1)
+        self.last_wire, self._last_conv = (wq, wk, wv), conv
+        self._conv_n += conv[:2]
+        torch.maximum(self._conv_max, conv[2:].view(torch.float64), out=self._conv_max)
+        out = pc.tree_scan([self.seq], pc.ingress([self.seq] * n, wk, wv, wq), tree)
+        self._drafted = (T, n)
+        return project(self.w_o, out.reshape(n, self.hq * self.d).to(torch.float32), self.b_o, rounded=True), out
+
+    def accept(self, path) -> None:
+        """Keep, of the nodes that the last ``verify`` appended, those of
+        ``path`` (rising node numbers, e.g. ``DraftTree.accept``'s) as the
+        context's next tokens, and drop the others."""
+        if self._drafted is None:
+            raise RuntimeError("accept needs verify first")
+        T, n = self._drafted
+        if self.dec.pc.length(self.seq) != T + n:
+            raise RuntimeError("the cache changed between verify and accept")
+        self.dec.pc.compact([self.seq], [path], [T])
+        self._drafted = None
 
     @property
     def conversion(self) -> dict:
