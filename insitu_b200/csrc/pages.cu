@@ -305,6 +305,7 @@ int compact_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *bas
                  const int64_t *keep, cudaStream_t s) {
     const int P = c->cfg.page_tokens;
     if (int rc = check_distinct(B, seq)) return rc;
+    Moves m;
     int64_t total = 0;
     for (int32_t b = 0; b < B; ++b) {
         if (int rc = check_seq(c, seq[b])) return rc;
@@ -313,13 +314,14 @@ int compact_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *bas
             return fail(INS_EBADLEN, "compact: rows outside sequence " + std::to_string(seq[b]) + "'s " +
                                          std::to_string(len) + " cached tokens");
         if (n && !keep) return fail(INS_EINVAL, "compact: keep is NULL");
-        int64_t last = -1;
-        for (int64_t i = 0; i < n; ++i) {
-            const int64_t k = keep[total + i];
-            if (k <= last)
-                return fail(INS_EINVAL, "compact: kept rows must be distinct, in rising order, from 0");
-            last = k;
-        }
+        // checked and narrowed in one pass (a long keep list is most of the host's work)
+        m.kept.resize((size_t)(total + n));
+        const int64_t *k = keep + total, last = n ? k[n - 1] : -1;
+        int32_t *to = m.kept.data() + total;
+        int rising = n == 0 || k[0] >= 0;
+        for (int64_t i = 0; i < n; ++i) to[i] = (int32_t)k[i];
+        for (int64_t i = 1; i < n; ++i) rising &= k[i] > k[i - 1];
+        if (!rising) return fail(INS_EINVAL, "compact: kept rows must be distinct, in rising order, from 0");
         if (last >= len - base[b])
             return fail(INS_EBADLEN, "compact: row " + std::to_string(base[b] + last) + " outside sequence " +
                                          std::to_string(seq[b]) + "'s " + std::to_string(len) + " cached tokens");
@@ -371,7 +373,6 @@ int compact_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *bas
         room -= more;
         j.fresh = true;
     }
-    Moves m;
     const size_t row = (size_t)c->cfg.max_pages_per_seq;
     // every allocation the plan needs happens before the cache changes
     size_t n_pages = 0, n_units = 0;
@@ -379,8 +380,6 @@ int compact_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *bas
         n_pages += (size_t)(j.p1 - j.p0);
         n_units += (size_t)((j.end - j.p0 * P) / MOVE_ROWS + 2);
     }
-    m.kept.reserve((size_t)total);
-    for (int64_t i = 0; i < total; ++i) m.kept.push_back((int32_t)keep[i]);
     std::vector<int32_t> dropped;
     size_t old_pages = 0;
     for (int32_t b = 0; b < B; ++b) old_pages += (size_t)pages_for(c, c->h_seq_lens[seq[b]]);

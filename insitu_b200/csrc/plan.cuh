@@ -24,14 +24,15 @@ struct PlanPtr {
 };
 
 // The plan under construction: typed arrays one after another, each aligned
-// to its element (the first to 16 bytes).
+// to its element (the first to 16 bytes). It refers to the arrays, which must
+// outlive run(): a long one is copied once, into the pinned upload buffer.
 class Plan {
   public:
     template <typename T>
     size_t add(const T *v, size_t n) {
-        const size_t at = (bytes_.size() + alignof(T) - 1) / alignof(T) * alignof(T);
-        bytes_.resize(at + n * sizeof(T));
-        if (n) std::memcpy(bytes_.data() + at, v, n * sizeof(T));
+        const size_t at = (size_ + alignof(T) - 1) / alignof(T) * alignof(T);
+        parts_.push_back(Part{at, v, n * sizeof(T)});
+        size_ = at + n * sizeof(T);
         return at;
     }
     template <typename T>
@@ -41,25 +42,34 @@ class Plan {
     // or PlanPtr; launch returns a cudaError_t.
     template <typename F>
     int run(CacheBase *c, cudaStream_t s, F &&launch) const {
-        const size_t n = bytes_.size();
-        if (n <= 512) return inlined<512>(launch);
-        if (n <= (size_t)PARAM_UPLOAD_MAX) return inlined<PARAM_UPLOAD_MAX>(launch);
-        if (int rc = c->stage_p.reserve(n)) return rc;
-        std::memcpy(c->stage_p.h, bytes_.data(), n);
-        if (int rc = c->stage_p.upload(n, s)) return rc;
+        if (size_ <= 512) return inlined<512>(launch);
+        if (size_ <= (size_t)PARAM_UPLOAD_MAX) return inlined<PARAM_UPLOAD_MAX>(launch);
+        if (int rc = c->stage_p.reserve(size_)) return rc;
+        write(static_cast<uint8_t *>(c->stage_p.h));
+        if (int rc = c->stage_p.upload(size_, s)) return rc;
         CK(launch(PlanPtr{(const uint8_t *)c->stage_p.d}));
         return INS_OK;
     }
 
   private:
+    struct Part {
+        size_t at;
+        const void *from;
+        size_t bytes;
+    };
+    void write(uint8_t *to) const {
+        for (const Part &p : parts_)
+            if (p.bytes) std::memcpy(to + p.at, p.from, p.bytes);
+    }
     template <int N, typename F>
     int inlined(F &&launch) const {
         PlanInline<N> p;
-        if (!bytes_.empty()) std::memcpy(p.b, bytes_.data(), bytes_.size());
+        write(p.b);
         CK(launch(p));
         return INS_OK;
     }
-    std::vector<uint8_t> bytes_;
+    std::vector<Part> parts_;
+    size_t size_ = 0;
 };
 
 }  // namespace ins
