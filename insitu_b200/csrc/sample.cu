@@ -11,7 +11,7 @@
 // histograms that narrow a range of values. The row's logits are read from
 // memory once, into the shared memory of a thread-block cluster (each CTA a
 // contiguous slice of the vocabulary), and the CTAs exchange histograms through
-// distributed shared memory. The cuts run over the few tokens within 10 nats
+// distributed shared memory. The cuts run over the few tokens within 6 nats
 // of the maximum, which one pass lists, where those decide them (they hold the
 // k-th largest, the mass), else over the whole slice. The histograms' last
 // levels work on the values' bits, and on the indexes where equal values are
@@ -41,7 +41,7 @@ constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32, SMP_BINS = 256;
 constexpr int SMP_MAX_VOCAB = 1 << 18;
 constexpr int SMP_WINDOWS = 4;               // first-level windows of 8 nats each, the last one open
 constexpr int SMP_LIST = 2048;               // tokens a CTA can list
-constexpr float SMP_NEAR = 10.0f;            // nats below the maximum that are listed
+constexpr float SMP_NEAR = 6.0f;             // nats below the maximum that are listed
 
 struct SampleArgs {
     const void *logits;
