@@ -868,7 +868,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
     if (tid == 0) {
         for (int i = 0; i < MANY_STAGES; ++i) bar_init(full(i), 4), bar_init(empty(i), 1);
         for (int i = 0; i < 2; ++i) bar_init(s_ready(i), 1), bar_init(p_ready(i), 4), bar_init(pv_done(i), 1);
-        bar_init(q_ready, 4), bar_init(seg_done, 1), bar_init(o_free, 8);
+        bar_init(q_ready, 8), bar_init(seg_done, 1), bar_init(o_free, 8);
         bar_init(m_full, 4), bar_init(m_empty, 4), bar_init(fin, 1);
         for (int i = 0; i < 4 * MANY_RING; ++i) bar_init(row_bar(0, i), 1);
         bar_init_fence();
@@ -919,7 +919,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
             int64_t next;
             const Segment s = segment_at(seqs, a.n_seqs, g, RU, t, end, cta, &next);
             const TreeSeq sq = seqs[s.seq];
-            const int len = sq.context + sq.nodes, rows_all = sq.nodes * g.H;
+            const int len = sq.context + sq.nodes;
             constexpr int KV4 = KB * 2, VV4 = VB * 2;            // 32-bit words of a row's codes
             const int32_t *pages = a.table + (int64_t)sq.seq * g.max_pages;
             // Bulk copies of this warp's 32 rows of tile s.lo + k, in the runs
@@ -952,26 +952,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
             };
             look_up(0);
             for (int k = 0; k < MANY_RING - 1; ++k) issue(k);
-            // the queries, in log2 units
-            if (seg) wait(seg_done, seg - 1);
-            const float u = LOG2E * exp2f((float)-g.qk_frac);
-#pragma unroll 4
-            for (int x = 0; x < RU / 16; ++x) {
-                const int i = row + 128 * x, r = i / 8, c = i % 8, qr = s.row0 + r;
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (qr < rows_all) {
-                    const int4 *p = reinterpret_cast<const int4 *>(
-                        a.q + (((int64_t)(sq.node0 + qr / g.H) * g.n_kv + s.head) * g.H + qr % g.H) * D + 8 * c);
-                    const int4 x = p[0], y = p[1];
-                    w = make_uint4(pack_half2((float)x.x * u, (float)x.y * u), pack_half2((float)x.z * u, (float)x.w * u),
-                                   pack_half2((float)y.x * u, (float)y.y * u), pack_half2((float)y.z * u, (float)y.w * u));
-                }
-                *reinterpret_cast<uint4 *>(sm + MANY_Q_AT + r * 128 + ((c ^ (r & 7)) * 16)) = w;
-            }
-            fence_async();
-            __syncwarp();
-            if (lane == 0) bar_arrive(q_ready);
-
             for (int k = 0; k < s.hi - s.lo && !lost; ++k, ++kt) {
                 uint32_t ck[KV4], cv[VV4], cn = 0;
                 const bool live = (s.lo + k) * MANY_TILE + row < len;
@@ -1114,6 +1094,29 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
             const int node = min(qr / g.H, sq.nodes - 1);
             const uint64_t *mk = a.mask + (int64_t)(sq.node0 + node) * a.words;
             const int tiles = s.hi - s.lo, steps = ROWS ? tiles : (tiles + 1 - i) / 2;
+            // The queries, in log2 units: this stream's row tile, whose products
+            // are done, or (!ROWS) half of the one tile, once both streams' are.
+            if (!ROWS && seg) wait(seg_done, seg - 1);
+            {
+                const float u = LOG2E * exp2f((float)-g.qk_frac);
+#pragma unroll
+                for (int x = 0; x < (ROWS ? 8 : 4); ++x) {
+                    const int at = (ROWS ? 1024 * i + row + 128 * x : tid + 256 * x), r = at / 8, c = at % 8;
+                    const int q = s.row0 + r;
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (q < rows_all) {
+                        const int4 *p = reinterpret_cast<const int4 *>(
+                            a.q + (((int64_t)(sq.node0 + q / g.H) * g.n_kv + s.head) * g.H + q % g.H) * D + 8 * c);
+                        const int4 y = p[0], z = p[1];
+                        w = make_uint4(pack_half2((float)y.x * u, (float)y.y * u), pack_half2((float)y.z * u, (float)y.w * u),
+                                       pack_half2((float)z.x * u, (float)z.y * u), pack_half2((float)z.z * u, (float)z.w * u));
+                    }
+                    *reinterpret_cast<uint4 *>(sm + MANY_Q_AT + r * 128 + ((c ^ (r & 7)) * 16)) = w;
+                }
+                fence_async();
+                __syncwarp();
+                if (lane == 0) bar_arrive(q_ready);
+            }
             float ref = -INFINITY, l = 0.0f;
             for (int n = 0; n < steps && !lost; ++n) {
                 const int t0 = (s.lo + (ROWS ? n : 2 * n + i)) * MANY_TILE;
