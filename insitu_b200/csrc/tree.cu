@@ -1312,8 +1312,17 @@ __global__ void __launch_bounds__(128) k_tree_join(Geo g, TreeArgs a, int32_t R,
 
 namespace {
 
-// Above this many query rows of a KV head the tcgen05 kernel takes over.
-constexpr int MANY_FROM = 32;
+// Above MANY_FROM query rows of a KV head the tcgen05 kernel takes over; up to
+// MANY_SURE rows only where each SM has more than MANY_TILES of its KV tiles
+// to do, as its start costs more (fewer units of work, tensor memory, the
+// join of 128-row slots) and its tiles less. Measured, 8 KV heads of 4 query
+// heads, 4b/2b, k_tree_few against k_tree_many: 9 nodes (36 rows) of one
+// sequence, 2,304 tokens (1 tile an SM) 21.8 : 22.8 us, 18,800 (8) 27.3 : 31.5,
+// 65,536 (28) 55.1 : 55.0, 131,072 (55) 92.5 : 88.2, 16 sequences of 32,768
+// (222) 375 : 295; 16 nodes (64 rows) 27.4 : 32.3, 55.0 : 56.4, 92.5 : 89.3,
+// 384 : 298; 3b/3b, 6 sequences to 9,001 tokens (about 20) 45.5 : 41.7. Above
+// 64 rows k_tree_few decodes each row three times and more.
+constexpr int MANY_FROM = 32, MANY_SURE = 64, MANY_TILES = 12;
 
 // How a call is cut: rows a tile, tokens a split, and what that takes.
 struct TreePlan {
@@ -1351,8 +1360,13 @@ int make_plan(const CacheBase *c, int32_t B, const int32_t *seq, const int32_t *
     if (all > INT32_MAX / (g.n_kv * g.H)) return fail(INS_EBADLEN, "too many nodes in one call");
     if (p.seqs.empty()) return INS_OK;
     const bool paired = (g.kb == 4 && g.vb == 2) || (g.kb == 3 && g.vb == 3);
-    if (paired && most > MANY_FROM) {
+    int64_t kv_tiles = 0;
+    for (const TreeSeq &s : p.seqs) kv_tiles += g.n_kv * ((s.context + s.nodes + MANY_TILE - 1) / MANY_TILE);
+    if (paired && (most > MANY_SURE || (most > MANY_FROM && kv_tiles > (int64_t)MANY_TILES * sms))) {
         p.many = true;
+        // 256-row tiles share each decoded row between both streams: above 128
+        // rows 128 : 166 us with 128-row tiles (64 nodes, 131,072 tokens); with
+        // 128 rows or fewer one stream would idle, 93 : 110 us (32 nodes)
         p.rows = most > 128 ? 256 : 128;
         for (TreeSeq &s : p.seqs) {
             const int64_t rts = ((int64_t)s.nodes * g.H + p.rows - 1) / p.rows;
@@ -1374,7 +1388,9 @@ int make_plan(const CacheBase *c, int32_t B, const int32_t *seq, const int32_t *
         }
         return INS_OK;
     }
-    // rows a tile: two 16-row fragments share each decoded token where there are more than 16 rows
+    // Rows a tile: two 16-row fragments share each decoded token where there
+    // are more than 16 rows. At 16 rows (4 nodes, 131,072 tokens) one fragment
+    // takes 41.9 us, two 55.8; at 17 to 32 one fragment would decode twice.
     p.rows = most > 16 ? 32 : 16;
     p.warps = p.rows == 16 ? 16 : 12;
     auto units_at = [&](int64_t chunk) {
@@ -1490,6 +1506,8 @@ int tree_body(CacheBase *c, int32_t B, const int32_t *seq, const int32_t *nodes,
     a.row_tiles_rows = p.rows;
     Plan plan;
     plan.add(p.seqs);
+    // up to 8 rows the fragment's second half holds none and its work is left
+    // out: one node, 131,072 tokens 38.1 us, with it 40.3
     bool half = true;
     for (const TreeSeq &t : p.seqs) half &= t.nodes * c->g.H <= 8;
     const int kb = c->g.kb, vb = c->g.vb;
