@@ -102,6 +102,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The transpose of an 8 x 8 matrix of 16-bit elements, two of row lane / 4 a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 // A 16-bit norm's value (int16 / 2^norm_frac): 2^23 + x is a float's bits, so
 // no integer conversion (which runs at an eighth of the rate) is needed.
 __device__ __forceinline__ float norm_value(uint32_t x16, float unit) {
@@ -149,7 +155,7 @@ __device__ __forceinline__ int find_seq(const TreeSeq *seqs, int n, int i) {
 // norm below 2^14, inside fp16's range, so a rescale of the accumulators is
 // rare and the maximum needs no exchange of lanes at every step.
 
-constexpr int FEW_TILE = 64, FEW_STAGES = 3;
+constexpr int FEW_TILE = 64;
 constexpr float LAG = 8.0f;
 
 template <int KB, int VB>
@@ -163,14 +169,16 @@ struct FewLayout {
     static constexpr bool WIDE = KB == 4 && VB == 2;
     static constexpr int KLUT = K_ENTRIES * (WIDE ? 256 : 128), VLUT = V_ENTRIES * 128, SINGLE = PAIRS ? 0 : 1024;
     static constexpr int NORMS_AT = KLUT + VLUT + SINGLE;        // [warps][64] (key, value) norms, where not WIDE
+    // ring slots a warp
+    __host__ __device__ static constexpr int stages(int warps) { return warps > 16 ? 2 : 3; }
     __host__ __device__ static constexpr int stages_at(int warps) { return NORMS_AT + (WIDE ? 0 : warps * 512); }
     __host__ __device__ static int stage_bytes(const Geo &g) { return FEW_TILE * (g.kbytes + g.vbytes + 4); }
     __host__ __device__ static int bars_at(const Geo &g, int warps) {
-        return stages_at(warps) + warps * FEW_STAGES * stage_bytes(g);
+        return stages_at(warps) + warps * stages(warps) * stage_bytes(g);
     }
     // the end-of-loop join reuses the stages: [warps][rows][64] floats, [warps][rows][2]
     __host__ static size_t bytes(const Geo &g, int warps, int rows) {
-        const size_t loop = (size_t)bars_at(g, warps) + warps * FEW_STAGES * 8;
+        const size_t loop = (size_t)bars_at(g, warps) + warps * stages(warps) * 8;
         const size_t join = (size_t)stages_at(warps) + (size_t)warps * rows * (64 + 2) * 4;
         return std::max(loop, join);
     }
@@ -180,14 +188,15 @@ template <int KB, int VB, int MT, bool HALF, int NW, class Src>
 __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, const __grid_constant__ Src src) {
     using L = FewLayout<KB, VB>;
     constexpr int R = 16 * MT;                       // rows of this CTA's tile
-    constexpr int HR = HALF ? 1 : 2;                 // of a fragment's two row halves, those that hold queries
+    constexpr int HR = HALF ? 1 : 2;                 // of a query fragment's two row halves, those that hold queries
+    constexpr int STAGES = L::stages(NW);
     extern __shared__ __align__(128) uint8_t sm[];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, t4 = lane % 4, g8 = lane / 4;
     const uint32_t sm0 = smem_u32(sm);
     const int kbytes = KB ? KB * 8 : g.kbytes, vbytes = VB ? VB * 8 : g.vbytes;
     const int stage = FEW_TILE * (kbytes + vbytes + 4);
-    const uint32_t ring = sm0 + L::stages_at(NW) + warp * FEW_STAGES * stage;
-    const uint32_t bars = sm0 + L::bars_at(g, NW) + warp * FEW_STAGES * 8;
+    const uint32_t ring = sm0 + L::stages_at(NW) + warp * STAGES * stage;
+    const uint32_t bars = sm0 + L::bars_at(g, NW) + warp * STAGES * 8;
 
     // tables: constant, so filled before the wait for earlier launches
     const float cunit = exp2f((float)-g.centroid_frac);
@@ -211,7 +220,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
             tab[i] = __float2half_rn((float)(i < 256 ? a.tb->k_cent[i] : a.tb->v_cent[i - 256]) * cunit);
     }
     if (lane == 0)
-        for (int i = 0; i < FEW_STAGES; ++i) bar_init(bars + i * 8, 1);
+        for (int i = 0; i < STAGES; ++i) bar_init(bars + i * 8, 1);
     bar_init_fence();
     wait_prior_grid();
     __syncthreads();
@@ -252,7 +261,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         const int j = warp + n * NW;
         if (j >= n_tiles) return;
         const int p0 = lo + j * FEW_TILE, rows16 = (min(FEW_TILE, hi - p0) + 15) & ~15;
-        const uint32_t bar = bars + (n % FEW_STAGES) * 8, dst = ring + (n % FEW_STAGES) * stage;
+        const uint32_t bar = bars + (n % STAGES) * 8, dst = ring + (n % STAGES) * stage;
         if (lane == 0) bar_expect(bar, rows16 * (kbytes + vbytes + 4));
         __syncwarp();
         // one lane per run of rows inside a page; pages hold a multiple of 16 rows
@@ -271,11 +280,11 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         }
     };
 
-    float acc[MT][8][4], m_ref[MT][2], l[MT][2];
+    float acc[MT][HALF ? 4 : 8][4], m_ref[MT][2], l[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
+        for (int c = 0; c < (HALF ? 4 : 8); ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[m][c][i] = 0.0f;
         m_ref[m][0] = m_ref[m][1] = -INFINITY;
@@ -288,16 +297,16 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
     const uint32_t lane4 = lane * 4;
     bool lost = false;
     int issued = 0;
-    for (; issued < FEW_STAGES - 1; ++issued) issue(issued);
+    for (; issued < STAGES - 1; ++issued) issue(issued);
     int n = 0;
     for (int j = warp; j < n_tiles; j += NW, ++n) {
         __syncwarp();                                 // every lane has read the slot's previous tile
         issue(issued++);
-        if (!bar_wait(bars + (n % FEW_STAGES) * 8, (n / FEW_STAGES) & 1)) {
+        if (!bar_wait(bars + (n % STAGES) * 8, (n / STAGES) & 1)) {
             lost = true;
             break;
         }
-        const uint8_t *st = sm + (ring - sm0) + (n % FEW_STAGES) * stage;
+        const uint8_t *st = sm + (ring - sm0) + (n % STAGES) * stage;
         const uint8_t *sv = st + FEW_TILE * kbytes, *sn = sv + FEW_TILE * vbytes;
         // the tile's norms as floats, once
 #pragma unroll
@@ -308,10 +317,9 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                 make_float2(norm_value(w & 0xffffu, nunit), norm_value(w >> 16, nunit));
         }
         __syncwarp();
-        const int p0 = lo + j * FEW_TILE, live = min(FEW_TILE, hi - p0);
-        const bool masked = p0 + FEW_TILE > sq.context;
-#pragma unroll 1
-        for (int s16 = 0; s16 < live; s16 += 16) {
+        const int p0 = lo + j * FEW_TILE;
+        auto step = [&](int s16, auto masked) {
+            constexpr bool M = decltype(masked)::value;
             // keys: fragment column g8 of token group nt is token s16 + 8 nt + g8
             uint32_t kf[2][4][2];
 #pragma unroll
@@ -340,88 +348,154 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                             (uint32_t)tab[code_at_bytes(row, 16 * t4 + 2 * i + 1, g.kb, kbytes)] << 16;
                 }
             }
-            // norms of the fragment's tokens: columns 2 t4, 2 t4 + 1 of both groups
-            float kn[4], vn[4];
+            [[maybe_unused]] uint32_t pf[MT][4], pt[2];
+            if constexpr (HALF) {
+                // tokens are the rows (g8, g8 + 8), queries the columns (2 t4, 2 t4 + 1)
+                const float *nr = reinterpret_cast<const float *>(norms + (s16 / 16) * nstride + g8 * 8);
+                const float2 n0 = *reinterpret_cast<const float2 *>(nr), n1 = *reinterpret_cast<const float2 *>(nr + 16);
+                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                const float4 w = *reinterpret_cast<const float4 *>(norms + (s16 / 16) * nstride + (nt * 8 + 2 * t4) * 8);
-                kn[2 * nt] = w.x, vn[2 * nt] = w.y, kn[2 * nt + 1] = w.z, vn[2 * nt + 1] = w.w;
-            }
-            float s[MT][2][4];
-            float top = -INFINITY;                    // largest excess over the running maximum
+                for (int ks = 0; ks < 4; ++ks) {
+                    const uint32_t k[4] = {kf[0][ks][0], kf[1][ks][0], kf[0][ks][1], kf[1][ks][1]};
+                    mma16816(s, k, qf[0][ks][0], qf[0][ks][2]);
+                }
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
+                for (int i = 0; i < 4; ++i) s[i] *= i < 2 ? n0.x : n1.x;
+                if (M) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int node = min((row0 + 2 * t4 + (i & 1)) / G, sq.nodes - 1);
+                        const uint64_t *mk = a.mask + (int64_t)(sq.node0 + node) * a.words;
+                        const int p = p0 + s16 + (i / 2) * 8 + g8, d = p - sq.context;
+                        if (!(p < hi && (d < 0 || ((mk[d >> 6] >> (d & 63)) & 1)))) s[i] = -INFINITY;
+                    }
+                }
+                const float mx[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+                bool over = false;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) over |= mx[q] > m_ref[0][q] + LAG;      // never for -inf
+                if (__any_sync(FULL, over)) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        float now = fmaxf(m_ref[0][q], mx[q]);
+#pragma unroll
+                        for (int o = 4; o < 32; o *= 2) now = fmaxf(now, __shfl_xor_sync(FULL, now, o));
+                        const float f = now > -INFINITY ? ex2(m_ref[0][q] - now) : 1.0f;
+                        m_ref[0][q] = now;
+                        l[0][q] *= f;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) acc[0][c][q] *= f, acc[0][c][2 + q] *= f;
+                    }
+                }
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // a row that has seen nothing yet keeps -inf - 0, not -inf - (-inf)
+                    const float ref = m_ref[0][i & 1];
+                    e[i] = ex2(s[i] - (ref > -INFINITY ? ref : 0.0f));
+                    l[0][i & 1] += e[i];
+                }
+                pt[0] = transpose8(pack_half2(e[0] * n0.y, e[1] * n0.y));
+                pt[1] = transpose8(pack_half2(e[2] * n1.y, e[3] * n1.y));
+            } else {
+                // norms of the fragment's tokens: columns 2 t4, 2 t4 + 1 of both groups
+                float kn[4], vn[4];
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[m][nt][i] = 0.0f;
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) mma16816(s[m][nt], qf[m][ks], kf[nt][ks][0], kf[nt][ks][1]);
-#pragma unroll
-                    for (int i = 0; i < 2 * HR; ++i) s[m][nt][i] *= kn[2 * nt + (i & 1)];
+                    const float4 w = *reinterpret_cast<const float4 *>(norms + (s16 / 16) * nstride + (nt * 8 + 2 * t4) * 8);
+                    kn[2 * nt] = w.x, vn[2 * nt] = w.y, kn[2 * nt + 1] = w.z, vn[2 * nt + 1] = w.w;
                 }
-            }
-            if (masked) {
+                float s[MT][2][4];
+                float top = -INFINITY;                    // largest excess over the running maximum
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int half = 0; half < HR; ++half) {
-                        const int node = min((row0 + m * 16 + half * 8 + g8) / G, sq.nodes - 1);
-                        const uint64_t *mk = a.mask + (int64_t)(sq.node0 + node) * a.words;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int p = p0 + s16 + (i / 2) * 8 + 2 * t4 + (i & 1), d = p - sq.context;
-                            const bool see = p < hi && (d < 0 || ((mk[d >> 6] >> (d & 63)) & 1));
-                            if (!see) s[m][i / 2][half * 2 + (i & 1)] = -INFINITY;
-                        }
-                    }
-            }
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int half = 0; half < HR; ++half) {
-                    const float mx = fmaxf(fmaxf(s[m][0][half * 2], s[m][0][half * 2 + 1]),
-                                           fmaxf(s[m][1][half * 2], s[m][1][half * 2 + 1]));
-                    top = fmaxf(top, mx > -INFINITY ? mx - m_ref[m][half] : -INFINITY);
-                }
-            if (__any_sync(FULL, top > LAG)) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int half = 0; half < HR; ++half) {
-                        float mx = fmaxf(fmaxf(s[m][0][half * 2], s[m][0][half * 2 + 1]),
-                                         fmaxf(s[m][1][half * 2], s[m][1][half * 2 + 1]));
-                        mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
-                        const float now = fmaxf(m_ref[m][half], mx);
-                        const float f = now > -INFINITY ? ex2(m_ref[m][half] - now) : 1.0f;
-                        m_ref[m][half] = now;
-                        l[m][half] *= f;
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            acc[m][c][half * 2] *= f;
-                            acc[m][c][half * 2 + 1] *= f;
-                        }
-                    }
-            }
-            uint32_t pf[MT][4];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
+                for (int m = 0; m < MT; ++m) {
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt) {
-                        if (half >= HR) {
-                            pf[m][nt * 2 + half] = 0;
-                            continue;
-                        }
-                        // a row that has seen nothing yet keeps -inf - 0, not -inf - (-inf)
-                        const float ref = m_ref[m][half] > -INFINITY ? m_ref[m][half] : 0.0f;
-                        const float e0 = ex2(s[m][nt][half * 2] - ref), e1 = ex2(s[m][nt][half * 2 + 1] - ref);
-                        l[m][half] += e0 + e1;
-                        pf[m][nt * 2 + half] = pack_half2(e0 * vn[2 * nt], e1 * vn[2 * nt + 1]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[m][nt][i] = 0.0f;
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) mma16816(s[m][nt], qf[m][ks], kf[nt][ks][0], kf[nt][ks][1]);
+#pragma unroll
+                        for (int i = 0; i < 2 * HR; ++i) s[m][nt][i] *= kn[2 * nt + (i & 1)];
                     }
+                }
+                if (M) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int half = 0; half < HR; ++half) {
+                            const int node = min((row0 + m * 16 + half * 8 + g8) / G, sq.nodes - 1);
+                            const uint64_t *mk = a.mask + (int64_t)(sq.node0 + node) * a.words;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int p = p0 + s16 + (i / 2) * 8 + 2 * t4 + (i & 1), d = p - sq.context;
+                                const bool see = p < hi && (d < 0 || ((mk[d >> 6] >> (d & 63)) & 1));
+                                if (!see) s[m][i / 2][half * 2 + (i & 1)] = -INFINITY;
+                            }
+                        }
+                }
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int half = 0; half < HR; ++half) {
+                        const float mx = fmaxf(fmaxf(s[m][0][half * 2], s[m][0][half * 2 + 1]),
+                                               fmaxf(s[m][1][half * 2], s[m][1][half * 2 + 1]));
+                        top = fmaxf(top, mx > -INFINITY ? mx - m_ref[m][half] : -INFINITY);
+                    }
+                if (__any_sync(FULL, top > LAG)) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int half = 0; half < HR; ++half) {
+                            float mx = fmaxf(fmaxf(s[m][0][half * 2], s[m][0][half * 2 + 1]),
+                                             fmaxf(s[m][1][half * 2], s[m][1][half * 2 + 1]));
+                            mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
+                            mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
+                            const float now = fmaxf(m_ref[m][half], mx);
+                            const float f = now > -INFINITY ? ex2(m_ref[m][half] - now) : 1.0f;
+                            m_ref[m][half] = now;
+                            l[m][half] *= f;
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                acc[m][c][half * 2] *= f;
+                                acc[m][c][half * 2 + 1] *= f;
+                            }
+                        }
+                }
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
+#pragma unroll
+                        for (int nt = 0; nt < 2; ++nt) {
+                            if (half >= HR) {
+                                pf[m][nt * 2 + half] = 0;
+                                continue;
+                            }
+                            // a row that has seen nothing yet keeps -inf - 0, not -inf - (-inf)
+                            const float ref = m_ref[m][half] > -INFINITY ? m_ref[m][half] : 0.0f;
+                            const float e0 = ex2(s[m][nt][half * 2] - ref), e1 = ex2(s[m][nt][half * 2 + 1] - ref);
+                            l[m][half] += e0 + e1;
+                            pf[m][nt * 2 + half] = pack_half2(e0 * vn[2 * nt], e1 * vn[2 * nt + 1]);
+                        }
+                }
             }
+            // channel group c's two value registers: an operand's columns, or (HALF) every
+            // second time half its rows
+            [[maybe_unused]] uint32_t even[2] = {0u, 0u};
+            auto add_values = [&](int c, const uint32_t (&b)[2]) {
+                if constexpr (HALF) {
+                    if (c & 1) {
+                        const uint32_t v[4] = {even[0], b[0], even[1], b[1]};
+                        mma16816(acc[0][c / 2], v, pt[0], pt[1]);
+                    } else {
+                        even[0] = b[0], even[1] = b[1];
+                    }
+                } else {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) mma16816(acc[m][c], pf[m], b[0], b[1]);
+                }
+            };
             // values: fragment rows (tokens) 2 t4, +1, +8, +9; column g8 of channel group c is channel 8 g8 + c
             if constexpr (VB == 2) {
                 // a byte of z: the codes of two channels of a token (low half)
@@ -448,8 +522,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                     for (int i = 0; i < 2; ++i)
                         b[i] = *reinterpret_cast<const uint32_t *>(sm + 128 +
                                                                    entry_at(c & 1 ? o[i] : e[i], c >> 1, lane4));
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) mma16816(acc[m][c], pf[m], b[0], b[1]);
+                    add_values(c, b);
                 }
             } else if constexpr (VB == 3) {
                 uint32_t x[4];
@@ -468,8 +541,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                         const uint32_t idx = ((x[2 * i] >> (3 * c)) & 7u) | (((x[2 * i + 1] >> (3 * c)) & 7u) << 3);
                         b[i] = load_shared(lut + idx * 128u);
                     }
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) mma16816(acc[m][c], pf[m], b[0], b[1]);
+                    add_values(c, b);
                 }
             } else {
                 const uint16_t *tab = reinterpret_cast<const uint16_t *>(sm) + 256;
@@ -482,38 +554,60 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                         b[i] = (uint32_t)tab[code_at_bytes(row, 8 * g8 + c, g.vb, vbytes)] |
                                (uint32_t)tab[code_at_bytes(row + vbytes, 8 * g8 + c, g.vb, vbytes)] << 16;
                     }
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) mma16816(acc[m][c], pf[m], b[0], b[1]);
+                    add_values(c, b);
                 }
             }
+        };
+        // a tile inside the context is whole (hi - lo is a multiple of it) and needs no mask
+        if (p0 + FEW_TILE <= sq.context) {
+#pragma unroll 1
+            for (int s16 = 0; s16 < FEW_TILE; s16 += 16) step(s16, std::false_type());
+        } else {
+#pragma unroll 1
+            for (int s16 = 0; s16 < min(FEW_TILE, hi - p0); s16 += 16) step(s16, std::true_type());
         }
     }
     if (lost) {
         // report it, and let the copies in flight land before the CTA goes
         if (lane == 0) atomicOr(a.status, ST_TIMEOUT);
         for (int k = n; k < issued; ++k)
-            if (warp + k * NW < n_tiles) bar_wait(bars + (k % FEW_STAGES) * 8, (k / FEW_STAGES) & 1);
+            if (warp + k * NW < n_tiles) bar_wait(bars + (k % STAGES) * 8, (k / STAGES) & 1);
     }
 
     // join the warps: each row's maximum, then the scaled sums
     __syncthreads();
     float *jacc = reinterpret_cast<float *>(sm + L::stages_at(NW)), *jml = jacc + NW * R * 64;
+    if constexpr (HALF) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+        for (int q = 0; q < 2; ++q) {
+            float sum = l[0][q];
 #pragma unroll
-        for (int half = 0; half < HR; ++half) {
-            float sum = l[m][half];
-            sum += __shfl_xor_sync(FULL, sum, 1);
-            sum += __shfl_xor_sync(FULL, sum, 2);
-            const int r = m * 16 + half * 8 + g8;
-            if (t4 == 0) jml[(warp * R + r) * 2] = m_ref[m][half], jml[(warp * R + r) * 2 + 1] = sum;
+            for (int o = 4; o < 32; o *= 2) sum += __shfl_xor_sync(FULL, sum, o);
+            const int r = 2 * t4 + q;
+            if (g8 == 0) jml[(warp * R + r) * 2] = m_ref[0][q], jml[(warp * R + r) * 2 + 1] = sum;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                // columns 2 t4, 2 t4 + 1 are channels 16 t4 + c and 16 t4 + 8 + c
-                jacc[(warp * R + r) * 64 + 16 * t4 + c] = acc[m][c][half * 2];
-                jacc[(warp * R + r) * 64 + 16 * t4 + 8 + c] = acc[m][c][half * 2 + 1];
-            }
+            for (int c = 0; c < 4; ++c)              // rows g8, g8 + 8 are channels 8 g8 + 2 c, + 1
+                *reinterpret_cast<float2 *>(jacc + (warp * R + r) * 64 + 8 * g8 + 2 * c) =
+                    make_float2(acc[0][c][q], acc[0][c][2 + q]);
         }
+    } else {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int half = 0; half < HR; ++half) {
+                float sum = l[m][half];
+                sum += __shfl_xor_sync(FULL, sum, 1);
+                sum += __shfl_xor_sync(FULL, sum, 2);
+                const int r = m * 16 + half * 8 + g8;
+                if (t4 == 0) jml[(warp * R + r) * 2] = m_ref[m][half], jml[(warp * R + r) * 2 + 1] = sum;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    // columns 2 t4, 2 t4 + 1 are channels 16 t4 + c and 16 t4 + 8 + c
+                    jacc[(warp * R + r) * 64 + 16 * t4 + c] = acc[m][c][half * 2];
+                    jacc[(warp * R + r) * 64 + 16 * t4 + 8 + c] = acc[m][c][half * 2 + 1];
+                }
+            }
+    }
     __syncthreads();
     constexpr int ROWS = HALF ? 8 : R;
     const int used = min(NW, n_tiles);
@@ -1326,7 +1420,7 @@ constexpr int MANY_FROM = 32, MANY_SURE = 64, MANY_TILES = 12;
 
 // How a call is cut: rows a tile, tokens a split, and what that takes.
 struct TreePlan {
-    int rows = 16, warps = 16;
+    int rows = 16;
     bool many = false;                       // k_tree_many's runs, else k_tree_few's units
     int64_t chunk = FEW_TILE, units = 0, groups = 0;
     int ctas = 0;                            // many: runs
@@ -1392,7 +1486,6 @@ int make_plan(const CacheBase *c, int32_t B, const int32_t *seq, const int32_t *
     // are more than 16 rows. At 16 rows (4 nodes, 131,072 tokens) one fragment
     // takes 41.9 us, two 55.8; at 17 to 32 one fragment would decode twice.
     p.rows = most > 16 ? 32 : 16;
-    p.warps = p.rows == 16 ? 16 : 12;
     auto units_at = [&](int64_t chunk) {
         int64_t u = 0;
         for (const TreeSeq &s : p.seqs) {
@@ -1453,9 +1546,9 @@ int launch_few(CacheBase *c, const TreePlan &p, const Plan &plan, const TreeArgs
 template <int KB, int VB>
 int launch_few_rows(CacheBase *c, const TreePlan &p, bool half, const Plan &plan, const TreeArgs &a, cudaStream_t s) {
     // 8-bit rows make a stage 8.4 KB: 8 warps of them fit
-    constexpr int N1 = KB ? 16 : 8, N2 = KB ? 12 : 8;
+    constexpr int NH = KB ? 24 : 8, N1 = KB ? 16 : 8, N2 = KB ? 12 : 8;
     if (p.rows == 32) return launch_few<KB, VB, 2, false, N2>(c, p, plan, a, s);
-    if (half) return launch_few<KB, VB, 1, true, N1>(c, p, plan, a, s);
+    if (half) return launch_few<KB, VB, 1, true, NH>(c, p, plan, a, s);
     return launch_few<KB, VB, 1, false, N1>(c, p, plan, a, s);
 }
 
