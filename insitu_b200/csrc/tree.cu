@@ -1546,7 +1546,7 @@ int launch_few(CacheBase *c, const TreePlan &p, const Plan &plan, const TreeArgs
 template <int KB, int VB>
 int launch_few_rows(CacheBase *c, const TreePlan &p, bool half, const Plan &plan, const TreeArgs &a, cudaStream_t s) {
     // 8-bit rows make a stage 8.4 KB: 8 warps of them fit
-    constexpr int NH = KB ? 24 : 8, N1 = KB ? 16 : 8, N2 = KB ? 12 : 8;
+    constexpr int NH = KB ? 24 : 8, N1 = KB ? 20 : 8, N2 = KB ? 12 : 8;
     if (p.rows == 32) return launch_few<KB, VB, 2, false, N2>(c, p, plan, a, s);
     if (half) return launch_few<KB, VB, 1, true, NH>(c, p, plan, a, s);
     return launch_few<KB, VB, 1, false, N1>(c, p, plan, a, s);
