@@ -157,6 +157,9 @@ __device__ __forceinline__ int find_seq(const TreeSeq *seqs, int n, int i) {
 
 constexpr int FEW_TILE = 64;
 constexpr float LAG = 8.0f;
+// The running maximum of a row that has seen nothing: finite, so that a masked
+// score's exponential is exp2(-inf) = 0 under it too, and below every score.
+constexpr float NONE = -1e30f;
 
 template <int KB, int VB>
 struct FewLayout {
@@ -165,13 +168,14 @@ struct FewLayout {
     static constexpr int V_ENTRIES = PAIRS && VB > 2 ? 1 << (2 * VB) : 0;
     // 4b/2b: a key entry's 32 lanes' copies fill 128 of its 256 bytes, so that
     // one byte permute makes an entry's address of a code byte; the other 128
-    // hold value pairs (entries a + 16 b < 64) and, from entry 64 on, the norms
+    // hold, for a byte of two tokens' codes of two channels, both channels'
+    // pairs: 8 bytes, 16 copies (a 64-bit load takes half a warp at a time)
     static constexpr bool WIDE = KB == 4 && VB == 2;
     static constexpr int KLUT = K_ENTRIES * (WIDE ? 256 : 128), VLUT = V_ENTRIES * 128, SINGLE = PAIRS ? 0 : 1024;
-    static constexpr int NORMS_AT = KLUT + VLUT + SINGLE;        // [warps][64] (key, value) norms, where not WIDE
+    static constexpr int NORMS_AT = KLUT + VLUT + SINGLE;        // [warps][64] (key, value) norms
     // ring slots a warp
     __host__ __device__ static constexpr int stages(int warps) { return warps > 16 ? 2 : 3; }
-    __host__ __device__ static constexpr int stages_at(int warps) { return NORMS_AT + (WIDE ? 0 : warps * 512); }
+    __host__ __device__ static constexpr int stages_at(int warps) { return NORMS_AT + warps * 512; }
     __host__ __device__ static int stage_bytes(const Geo &g) { return FEW_TILE * (g.kbytes + g.vbytes + 4); }
     __host__ __device__ static int bars_at(const Geo &g, int warps) {
         return stages_at(warps) + warps * stages(warps) * stage_bytes(g);
@@ -209,8 +213,11 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
             reinterpret_cast<uint32_t *>(sm)[e * (L::WIDE ? 64 : 32) + lane] =
                 pack_half2(cent[e & ((1 << KB) - 1)], cent[e >> KB]);
         if (L::WIDE)
-            for (int e = warp; e < 64; e += NW)
-                reinterpret_cast<uint32_t *>(sm)[e * 64 + 32 + lane] = pack_half2(cent[32 + (e & 3)], cent[32 + (e >> 4)]);
+            for (int e = warp; e < 256; e += NW) {
+                const int c = 2 * (lane / 16);                   // this half warp's channel of the two
+                reinterpret_cast<uint32_t *>(sm)[e * 64 + 32 + lane % 16 * 2 + lane / 16] =
+                    pack_half2(cent[32 + (e >> c & 3)], cent[32 + (e >> (4 + c) & 3)]);
+            }
         for (int e = warp; e < L::V_ENTRIES; e += NW)
             reinterpret_cast<uint32_t *>(sm + L::KLUT)[e * 32 + lane] =
                 pack_half2(cent[32 + (e & ((1 << VB) - 1))], cent[32 + (e >> VB)]);
@@ -287,14 +294,13 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         for (int c = 0; c < (HALF ? 4 : 8); ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[m][c][i] = 0.0f;
-        m_ref[m][0] = m_ref[m][1] = -INFINITY;
+        m_ref[m][0] = m_ref[m][1] = NONE;
         l[m][0] = l[m][1] = 0.0f;
     }
     const float nunit = exp2f((float)-g.norm_frac);
     // this warp's norms of a tile: 16 tokens' (key, value) in each 128 bytes
-    uint8_t *norms = sm + (L::WIDE ? (64 + warp * 4) * 256 + 128 : L::NORMS_AT + warp * 512);
-    constexpr int nstride = L::WIDE ? 256 : 128;
-    const uint32_t lane4 = lane * 4;
+    uint8_t *norms = sm + L::NORMS_AT + warp * 512;
+    const uint32_t lane4 = lane * 4, value8 = 128 + lane % 16 * 8;
     bool lost = false;
     int issued = 0;
     for (; issued < STAGES - 1; ++issued) issue(issued);
@@ -313,7 +319,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         for (int i = 0; i < 2; ++i) {
             const int tok = lane + 32 * i;
             const uint32_t w = *reinterpret_cast<const uint32_t *>(sn + tok * 4);
-            *reinterpret_cast<float2 *>(norms + (tok / 16) * nstride + (tok % 16) * 8) =
+            *reinterpret_cast<float2 *>(norms + tok * 8) =
                 make_float2(norm_value(w & 0xffffu, nunit), norm_value(w >> 16, nunit));
         }
         __syncwarp();
@@ -351,7 +357,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
             [[maybe_unused]] uint32_t pf[MT][4], pt[2];
             if constexpr (HALF) {
                 // tokens are the rows (g8, g8 + 8), queries the columns (2 t4, 2 t4 + 1)
-                const float *nr = reinterpret_cast<const float *>(norms + (s16 / 16) * nstride + g8 * 8);
+                const float *nr = reinterpret_cast<const float *>(norms + s16 * 8 + g8 * 8);
                 const float2 n0 = *reinterpret_cast<const float2 *>(nr), n1 = *reinterpret_cast<const float2 *>(nr + 16);
                 float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -380,7 +386,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                         float now = fmaxf(m_ref[0][q], mx[q]);
 #pragma unroll
                         for (int o = 4; o < 32; o *= 2) now = fmaxf(now, __shfl_xor_sync(FULL, now, o));
-                        const float f = now > -INFINITY ? ex2(m_ref[0][q] - now) : 1.0f;
+                        const float f = ex2(m_ref[0][q] - now);
                         m_ref[0][q] = now;
                         l[0][q] *= f;
 #pragma unroll
@@ -390,9 +396,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                 float e[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    // a row that has seen nothing yet keeps -inf - 0, not -inf - (-inf)
-                    const float ref = m_ref[0][i & 1];
-                    e[i] = ex2(s[i] - (ref > -INFINITY ? ref : 0.0f));
+                    e[i] = ex2(s[i] - m_ref[0][i & 1]);
                     l[0][i & 1] += e[i];
                 }
                 pt[0] = transpose8(pack_half2(e[0] * n0.y, e[1] * n0.y));
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                 float kn[4], vn[4];
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
-                    const float4 w = *reinterpret_cast<const float4 *>(norms + (s16 / 16) * nstride + (nt * 8 + 2 * t4) * 8);
+                    const float4 w = *reinterpret_cast<const float4 *>(norms + s16 * 8 + (nt * 8 + 2 * t4) * 8);
                     kn[2 * nt] = w.x, vn[2 * nt] = w.y, kn[2 * nt + 1] = w.z, vn[2 * nt + 1] = w.w;
                 }
                 float s[MT][2][4];
@@ -440,7 +444,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                     for (int half = 0; half < HR; ++half) {
                         const float mx = fmaxf(fmaxf(s[m][0][half * 2], s[m][0][half * 2 + 1]),
                                                fmaxf(s[m][1][half * 2], s[m][1][half * 2 + 1]));
-                        top = fmaxf(top, mx > -INFINITY ? mx - m_ref[m][half] : -INFINITY);
+                        top = fmaxf(top, mx - m_ref[m][half]);
                     }
                 if (__any_sync(FULL, top > LAG)) {
 #pragma unroll
@@ -452,7 +456,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                             mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
                             mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
                             const float now = fmaxf(m_ref[m][half], mx);
-                            const float f = now > -INFINITY ? ex2(m_ref[m][half] - now) : 1.0f;
+                            const float f = ex2(m_ref[m][half] - now);
                             m_ref[m][half] = now;
                             l[m][half] *= f;
 #pragma unroll
@@ -472,9 +476,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                                 pf[m][nt * 2 + half] = 0;
                                 continue;
                             }
-                            // a row that has seen nothing yet keeps -inf - 0, not -inf - (-inf)
-                            const float ref = m_ref[m][half] > -INFINITY ? m_ref[m][half] : 0.0f;
-                            const float e0 = ex2(s[m][nt][half * 2] - ref), e1 = ex2(s[m][nt][half * 2 + 1] - ref);
+                            const float e0 = ex2(s[m][nt][half * 2] - m_ref[m][half]), e1 = ex2(s[m][nt][half * 2 + 1] - m_ref[m][half]);
                             l[m][half] += e0 + e1;
                             pf[m][nt * 2 + half] = pack_half2(e0 * vn[2 * nt], e1 * vn[2 * nt + 1]);
                         }
@@ -499,9 +501,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
             // values: fragment rows (tokens) 2 t4, +1, +8, +9; column g8 of channel group c is channel 8 g8 + c
             if constexpr (VB == 2) {
                 // a byte of z: the codes of two channels of a token (low half)
-                // and of the next one (high half); even and odd channels apart,
-                // each byte is a value pair's entry
-                uint32_t e[2], o[2];
+                // and of the next one (high half), an entry of both channels' pairs
+                uint32_t z[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     uint32_t x[2];
@@ -511,18 +512,14 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                         x[k] = __byte_perm(*reinterpret_cast<const uint16_t *>(sv + tok * 16 + g8 * 2), 0, 0x4140);
                         x[k] = (x[k] | x[k] << 4) & 0x0f0f0f0fu;
                     }
-                    const uint32_t z = x[1] * 16 + x[0];
-                    e[i] = z & 0x33333333u;
-                    o[i] = (z >> 2) & 0x33333333u;
+                    z[i] = x[1] * 16 + x[0];
                 }
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    uint32_t b[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        b[i] = *reinterpret_cast<const uint32_t *>(sm + 128 +
-                                                                   entry_at(c & 1 ? o[i] : e[i], c >> 1, lane4));
-                    add_values(c, b);
+                for (int k = 0; k < 4; ++k) {
+                    const uint2 v0 = *reinterpret_cast<const uint2 *>(sm + entry_at(z[0], k, value8));
+                    const uint2 v1 = *reinterpret_cast<const uint2 *>(sm + entry_at(z[1], k, value8));
+                    add_values(2 * k, {v0.x, v1.x});
+                    add_values(2 * k + 1, {v0.y, v1.y});
                 }
             } else if constexpr (VB == 3) {
                 uint32_t x[4];
@@ -584,7 +581,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
 #pragma unroll
             for (int o = 4; o < 32; o *= 2) sum += __shfl_xor_sync(FULL, sum, o);
             const int r = 2 * t4 + q;
-            if (g8 == 0) jml[(warp * R + r) * 2] = m_ref[0][q], jml[(warp * R + r) * 2 + 1] = sum;
+            if (g8 == 0) jml[(warp * R + r) * 2] = m_ref[0][q] > NONE ? m_ref[0][q] : -INFINITY, jml[(warp * R + r) * 2 + 1] = sum;
 #pragma unroll
             for (int c = 0; c < 4; ++c)              // rows g8, g8 + 8 are channels 8 g8 + 2 c, + 1
                 *reinterpret_cast<float2 *>(jacc + (warp * R + r) * 64 + 8 * g8 + 2 * c) =
@@ -599,7 +596,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                 sum += __shfl_xor_sync(FULL, sum, 1);
                 sum += __shfl_xor_sync(FULL, sum, 2);
                 const int r = m * 16 + half * 8 + g8;
-                if (t4 == 0) jml[(warp * R + r) * 2] = m_ref[m][half], jml[(warp * R + r) * 2 + 1] = sum;
+                if (t4 == 0) jml[(warp * R + r) * 2] = m_ref[m][half] > NONE ? m_ref[m][half] : -INFINITY, jml[(warp * R + r) * 2 + 1] = sum;
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     // columns 2 t4, 2 t4 + 1 are channels 16 t4 + c and 16 t4 + 8 + c
@@ -1545,10 +1542,13 @@ int launch_few(CacheBase *c, const TreePlan &p, const Plan &plan, const TreeArgs
 
 template <int KB, int VB>
 int launch_few_rows(CacheBase *c, const TreePlan &p, bool half, const Plan &plan, const TreeArgs &a, cudaStream_t s) {
-    // 8-bit rows make a stage 8.4 KB: 8 warps of them fit
-    constexpr int NH = KB ? 24 : 8, N1 = KB ? 20 : 8, N2 = KB ? 12 : 8;
+    // Warps: five a scheduler where 96 registers hold their state (1 token of
+    // 1M rows: 20 warps 151 us, 23 warps of 80 registers 153; 3b/3b 195, 209),
+    // three where 32 rows take 168 (8 nodes of 1M: 12 warps 317 us, 14 spill:
+    // 540). 8-bit rows make a stage 8.4 KB: 8 warps of them fit.
+    constexpr int N1 = KB ? 20 : 8, N2 = KB ? 12 : 8;
     if (p.rows == 32) return launch_few<KB, VB, 2, false, N2>(c, p, plan, a, s);
-    if (half) return launch_few<KB, VB, 1, true, NH>(c, p, plan, a, s);
+    if (half) return launch_few<KB, VB, 1, true, N1>(c, p, plan, a, s);
     return launch_few<KB, VB, 1, false, N1>(c, p, plan, a, s);
 }
 
