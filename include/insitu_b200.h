@@ -417,7 +417,8 @@ int ins_merge_parts(ins_cache *cache, int32_t B, int32_t n_parts, const void *pa
  *
  * fork: sequence dst[i], which must be empty, becomes the first lengths[i]
  * rows of src[i] (all of them when lengths is NULL). Full pages are shared, a
- * page that is not full is copied.
+ * page that is not full is copied. No sequence may be both a source and a
+ * target of one call.
  *
  * compact: of sequence seq_ids[i], rows below base[i] stay, and of those from
  * base[i] on the counts[i] rows base[i] + keep[..] stay, moved together after

@@ -258,9 +258,15 @@ int fork_body(CacheBase *c, int32_t B, const int32_t *src, const int32_t *dst, c
     const int P = c->cfg.page_tokens;
     int64_t need = 0;
     if (int rc = check_distinct(B, dst)) return rc;
+    // no source may be a target too: the lengths checked here are those that
+    // are taken below, and no copy reads a page that another one writes
+    std::vector<int32_t> targets(dst, dst + B);
+    std::sort(targets.begin(), targets.end());
     for (int32_t b = 0; b < B; ++b) {
         if (int rc = check_seq(c, src[b])) return rc;
         if (int rc = check_seq(c, dst[b])) return rc;
+        if (std::binary_search(targets.begin(), targets.end(), src[b]))
+            return fail(INS_EINVAL, "fork: sequence " + std::to_string(src[b]) + " is a source and a target of one call");
         if (c->h_seq_lens[dst[b]])
             return fail(INS_EINVAL, "fork: sequence " + std::to_string(dst[b]) + " is not empty");
         const int64_t len = c->h_seq_lens[src[b]], n = lengths ? lengths[b] : len;

@@ -359,9 +359,10 @@ class PagedCache:
         return int(self._L.ins_cache_free_pages(self._h))
 
     def fork(self, src, dst, lengths=None) -> None:
-        """Make each sequence of ``dst`` (empty ones) the first ``lengths`` rows
-        (all by default) of the sequence of ``src`` beside it
-        (ins_cache_fork): full pages are shared, the last one is copied."""
+        """Make each sequence of ``dst`` (empty ones, none of them in ``src``)
+        the first ``lengths`` rows (all by default) of the sequence of ``src``
+        beside it (ins_cache_fork): full pages are shared, the last one is
+        copied."""
         src, dst = _list(src), _list(dst)
         lens = None if lengths is None else _ids(lengths, len(dst))
         try:
