@@ -361,10 +361,11 @@ struct Row {
         int bin = SMP_BINS, win = 0;
         for (; win < SMP_WINDOWS; ++win) {
             clear();
-            // (the margin covers the bins' roundings)
-            const float from = win + 1 < SMP_WINDOWS
-                                   ? xmax - (win + 1) * SMP_BINS * 1.0001f / bins - 1e-6f * fabsf(xmax)
-                                   : -INFINITY;
+            // (the margin covers the bins' roundings; below an infinite maximum
+            // every distance is infinite, so only the last window holds more)
+            const float edge = xmax < INFINITY ? xmax - (win + 1) * SMP_BINS * 1.0001f / bins - 1e-6f * fabsf(xmax)
+                                               : xmax;
+            const float from = win + 1 < SMP_WINDOWS ? edge : -INFINITY;
             each(from, [&](float x, uint32_t, int) {
                 const int b = bin_of(x) - win * SMP_BINS;
                 if (b >= 0 && b < SMP_BINS) count(b, BY_MASS ? mass_of(x) : 0u);
