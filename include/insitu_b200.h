@@ -488,9 +488,9 @@ enum { INS_F32 = 0, INS_F16 = 1, INS_BF16 = 2 };
  * uniform: device float, likewise. vocab in [1, 262144]. temperature, top_k, top_p, min_p: device,
  * one value a row, each may be NULL (1, no cut, no cut, no cut). A temperature
  * that is not above 0 takes the largest logit; top_k <= 0 or >= vocab, top_p
- * >= 1 and min_p <= 0 cut nothing. A NaN logit counts as -inf, and a logit of
- * -inf is never chosen; a row with nothing else gives token -1 and
- * log-probability -inf. tokens: device int64 [rows]; logprobs: device float
+ * >= 1 and min_p <= 0 cut nothing; a min_p above 1, or a NaN, keeps nothing.
+ * A NaN logit counts as -inf, and a logit of -inf is never chosen; a row with
+ * nothing left gives token -1 and log-probability -inf. tokens: device int64 [rows]; logprobs: device float
  * [rows] or NULL, the token's log-probability among the kept ones (0 for a
  * row taken by its largest logit). Runs on the device of the current context,
  * stream-ordered. */

@@ -547,9 +547,10 @@ __global__ void __launch_bounds__(SMP_THREADS) k_sample(const SampleArgs a) {
     const int mine = token;
     R.cluster_best(key, token);
     R.cluster_sum(mass, unused);
-    if (mine == token && token != INT_MAX) {
-        a.tokens[row] = token;
-        if (a.logprobs) a.logprobs[row] = (float)((double)z_key - log((double)mass * 0x1p-31));
+    const bool empty = token == INT_MAX;     // a min_p above 1, or a NaN, keeps no token
+    if (empty ? rank == 0 && threadIdx.x == 0 : mine == token) {
+        a.tokens[row] = empty ? -1 : token;
+        if (a.logprobs) a.logprobs[row] = empty ? -INFINITY : (float)((double)z_key - log((double)mass * 0x1p-31));
     }
     cl.sync();
 }

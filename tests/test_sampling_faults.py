@@ -46,3 +46,27 @@ def test_several_infinite_logits_are_cut_by_their_index(settings, vocab, dtype):
     u[:, :10] = 0.25                            # a lower index does not win by its number
     u[:, -1] = 0.99
     compare(x, u, **settings)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [1, 40, 5001, 40000])
+@pytest.mark.parametrize("k,p", [(0, 1.0), (7, 1.0), (0, 0.8), (7, 0.8)])
+def test_a_min_p_that_keeps_nothing_writes_its_outputs(vocab, k, p):
+    """The C entry takes any min_p: rows above 1, infinite or NaN have no token
+    left, the rows beside them are drawn as always."""
+    from insitu_b200 import _lib
+    x, u = inputs(5, vocab, seed=vocab)
+    x[4] = -float("inf")
+    column = lambda v, dtype: torch.tensor(v, dtype=dtype, device="cuda")
+    m = column([1.5, float("nan"), 0.02, float("inf"), 0.0], torch.float32)
+    top_k, top_p = column([k] * 5, torch.int32), column([p] * 5, torch.float32)
+    tokens = torch.full((5,), 777, dtype=torch.int64, device="cuda")
+    logp = torch.full((5,), 777.0, device="cuda")
+    at = lambda t: t.data_ptr()
+    _lib.check(_lib.lib().ins_sample(5, vocab, at(x), 0, x.stride(0), at(u), u.stride(0), None, at(top_k), at(top_p),
+                                     at(m), at(tokens), at(logp), torch.cuda.current_stream().cuda_stream))
+    token, lp = reference(x[2].cpu().numpy(), u[2].cpu().numpy(), 1.0, k, float(np.float32(p)), float(np.float32(0.02)))
+    assert tokens.tolist() == [-1, -1, token, -1, -1]
+    assert torch.isinf(logp[[0, 1, 3, 4]]).all() and abs(float(logp[2]) - lp) <= 2.0 ** -22 * 20 + 1e-6
+    op = _lib.ops().sample(x, u, None, top_k, top_p, m)
+    assert torch.equal(op[0], tokens) and torch.equal(op[1], logp)
