@@ -17,10 +17,13 @@
 // levels work on the values' bits, and on the indexes where equal values are
 // split, so the order is exact.
 //
-// Masses are summed as integers, w_i rounded to 2^-31 (64-bit totals): the
-// result then does not depend on the order of the atomics, and the rounding
-// (2^-32 a token at most, against a largest w of 1) moves the total of
-// 128,000 tokens by some 1e-8 of it.
+// Masses are summed as integers (64-bit totals), so that a result does not
+// depend on the order of the atomics. Those that decide a cut are w_i rounded
+// to 2^-31, 2^-32 a token at most against a largest w of 1: a cut by top_p is
+// that of the definition with masses moved by up to vocab * 2^-32 of the total
+// (6e-5 at 262,144 tokens, where all but one lie just below 2^-32, 22.2 nats
+// under the maximum, and count as nothing). The log-probability's mass is
+// summed to 2^-40.
 //
 // Bound: one read of the logits (and of the random numbers, where a row is
 // not filtered); at a few rows the passes' latency. Histograms over the whole
@@ -512,10 +515,11 @@ __global__ void __launch_bounds__(SMP_THREADS) k_sample(const SampleArgs a) {
     float key = -INFINITY, z_key = 0.0f, reach = INFINITY;
     int token = INT_MAX;
     const float *u = a.uniform + row * a.u_stride;
-    auto draw = [&](float x, float un, int i) {
+    // adds the token's mass by add(w), unless min_p drops it
+    auto draw = [&](float x, float un, int i, auto &&add) {
         const float z = R.z_of(x), w = R.w_of(z);
         if (!(w >= floor_w)) return;
-        mass += __float2uint_rn(w * 2147483648.0f);
+        add(w);
         // z - log(-log u) beats `key` only where -log u < w exp(-key), and
         // 1 - u <= -log u: most tokens need no logarithm (the margin covers
         // the roundings)
@@ -527,22 +531,31 @@ __global__ void __launch_bounds__(SMP_THREADS) k_sample(const SampleArgs a) {
             reach = 1.001f * expf(-key);                   // infinite for -inf: no bound
         }
     };
+    // in units of 2^-40 (2^18 tokens of mass 1 make 2^58); integers where the order is the list's
+    auto units = [](float w) { return __float2ull_rn(w * 0x1p40f); };
     if (R.list || R.thr_key) {
         R.each(R.thr_key ? key_value(R.thr_key) : -INFINITY,
-               [&](float x, uint32_t, int i) { draw(x, __ldcs(u + i), i); });
+               [&](float x, uint32_t, int i) { draw(x, __ldcs(u + i), i, [&](float w) { mass += units(w); }); });
     } else {
         u += first;
+        float sum = 0.0f, lost = 0.0f;
         for (int i = threadIdx.x; i < n; i += 8 * SMP_THREADS) {
             float un[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) un[k] = i + k * SMP_THREADS < n ? __ldcs(u + i + k * SMP_THREADS) : 0.0f;
+            float eight = 0.0f;              // the tokens' sum, within 2^-21 of itself
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const int e = i + k * SMP_THREADS;
                 const float x = e < n ? to_f32(slice.at[e]) : -INFINITY;
-                if (x > -INFINITY) draw(x + 0.0f, un[k], first + e);
+                if (x > -INFINITY) draw(x + 0.0f, un[k], first + e, [&](float w) { eight += w; });
             }
+            // compensated: the thread's sum (in a fixed order) is rounded as one addition is
+            const float y = eight - lost, next = sum + y;
+            lost = next - sum - y;
+            sum = next;
         }
+        mass = units(sum);
     }
     const int mine = token;
     R.cluster_best(key, token);
@@ -550,7 +563,7 @@ __global__ void __launch_bounds__(SMP_THREADS) k_sample(const SampleArgs a) {
     const bool empty = token == INT_MAX;     // a min_p above 1, or a NaN, keeps no token
     if (empty ? rank == 0 && threadIdx.x == 0 : mine == token) {
         a.tokens[row] = empty ? -1 : token;
-        if (a.logprobs) a.logprobs[row] = empty ? -INFINITY : (float)((double)z_key - log((double)mass * 0x1p-31));
+        if (a.logprobs) a.logprobs[row] = empty ? -INFINITY : (float)((double)z_key - log((double)mass * 0x1p-40));
     }
     cl.sync();
 }

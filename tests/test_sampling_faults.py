@@ -70,3 +70,18 @@ def test_a_min_p_that_keeps_nothing_writes_its_outputs(vocab, k, p):
     assert torch.isinf(logp[[0, 1, 3, 4]]).all() and abs(float(logp[2]) - lp) <= 2.0 ** -22 * 20 + 1e-6
     op = _lib.ops().sample(x, u, None, top_k, top_p, m)
     assert torch.equal(op[0], tokens) and torch.equal(op[1], logp)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [128000, 262144])
+@pytest.mark.parametrize("settings", [dict(), dict(k=120000), dict(m=1e-10), dict(k=120000, t=2.0)])
+def test_a_flat_tail_far_below_the_peak_counts_in_the_log_probability(vocab, settings):
+    """Tokens 22.2 to 23 nats under the maximum weigh less than 2^-32 each, and
+    together 3e-5: summed to 2^-31 they were nothing."""
+    x, u = inputs(3, vocab, seed=vocab)
+    t = settings.get("t", 1.0)
+    x = (-22.6 + 0.15 * x) * t                  # 2.5 * 0.15 nats wide
+    x[:, 777] = 0.0
+    x[1] = x[1].clamp(min=-22.9 * t)
+    x[2, ::3] = -22.3 * t
+    compare(x, u, **settings)
