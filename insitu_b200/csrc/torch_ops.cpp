@@ -10,6 +10,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
@@ -138,6 +139,12 @@ at::Tensor project(const at::Tensor &w16, const at::Tensor &x, const c10::option
                       reinterpret_cast<const uint16_t *>(w16.data_ptr<at::Half>()), x.data_ptr<float>(), b,
                       y.data_ptr<float>(), at::cuda::getCurrentCUDAStream().stream()));
     return y;
+}
+
+// Tells the allocator that the current stream reads `t`, a tensor that an
+// object keeps between calls: once dropped, its memory is not reused before.
+void used_here(const at::Tensor &t) {
+    c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), at::cuda::getCurrentCUDAStream());
 }
 
 int32_t n_ids(at::IntArrayRef ids) {
@@ -271,13 +278,14 @@ std::tuple<at::Tensor, at::Tensor> sample(const at::Tensor &logits, const at::Te
                               t->dim() == 1 && t->size(0) == n,
                           "insitu: ", name, " must be a contiguous ", type, " tensor of ", n,
                           " values on logits' device");
+        used_here(*t);
         return t->data_ptr();
     };
+    c10::cuda::CUDAGuard guard(logits.device());
     const auto *t = static_cast<const float *>(setting(temperature, at::kFloat, "temperature"));
     const auto *k = static_cast<const int32_t *>(setting(top_k, at::kInt, "top_k"));
     const auto *p = static_cast<const float *>(setting(top_p, at::kFloat, "top_p"));
     const auto *m = static_cast<const float *>(setting(min_p, at::kFloat, "min_p"));
-    c10::cuda::CUDAGuard guard(logits.device());
     at::Tensor tokens = at::empty({n}, logits.options().dtype(at::kLong));
     at::Tensor logprobs = at::empty({n}, logits.options().dtype(at::kFloat));
     check(ins_sample((int32_t)n, (int32_t)vocab, logits.data_ptr(),

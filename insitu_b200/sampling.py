@@ -33,11 +33,12 @@ class Sampler:
 
     ``temperature`` (0 takes the largest logit), ``top_k`` (0: off), ``top_p``
     and ``min_p`` are numbers, or 1-D tensors or sequences of one value a row.
-    They are checked here, so a call reads nothing back from the device."""
+    They are checked here, so a call reads nothing back from the device. One
+    ``Sampler`` may be used on several streams."""
 
     def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         self._rows = None
-        self._per_row, self._scalar = {}, {}
+        self._per_row, self._scalar, self._filled = {}, {}, {}
         for name, value in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
             dtype, neutral, valid, words = _SETTINGS[name]
             t = torch.as_tensor(value)
@@ -45,18 +46,24 @@ class Sampler:
                 raise ValueError(f"{name} must be a number or one value a row")
             if dtype == torch.int32 and (t.is_floating_point() or t.dtype == torch.bool):
                 raise TypeError(f"{name} must be an integer")
-            if not bool(valid(t if dtype == torch.int32 else t.to(dtype)).all()):
+            held = (t.clamp(max=MAX_VOCAB) if dtype == torch.int32 else t).to(dtype).contiguous()
+            # (reading the check's answer also waits for `held`, where t is on the device)
+            if not bool(valid(t if dtype == torch.int32 else held).all()):
                 raise ValueError(f"{name} must be {words}")
             if t.dim() == 0:
-                if t.item() != neutral:
-                    self._scalar[name] = t.clamp(max=MAX_VOCAB).to(dtype) if dtype == torch.int32 else t.to(dtype)
+                if held.item() != neutral:
+                    self._scalar[name] = held.item()
                 continue
             if self._rows not in (None, t.numel()):
                 raise ValueError(f"{name} holds {t.numel()} values; other settings hold {self._rows}")
             self._rows = t.numel()
-            self._per_row[name] = (t.clamp(max=MAX_VOCAB) if dtype == torch.int32 else t).to(dtype).contiguous()
+            self._per_row[name] = held
 
     def _values(self, n: int, device) -> list:
+        """The settings' device tensors for n rows. Calls on any stream share
+        them, so they come by copies from the host that the host waits for
+        (the first call, and one with more rows than any before), and the
+        operator tells the allocator which streams read them."""
         if self._rows not in (None, n):
             raise ValueError(f"the settings are for {self._rows} rows; logits hold {n}")
         out = []
@@ -64,11 +71,13 @@ class Sampler:
             t = self._per_row.get(name)
             if t is not None:
                 if t.device != device:
-                    t = self._per_row[name] = t.to(device)
+                    t = self._per_row[name] = t.cpu().to(device)
             elif name in self._scalar:
-                t = self._scalar[name]
-                if t.device != device or t.dim() == 0 or t.numel() < n:
-                    t = self._scalar[name] = t.reshape(-1)[:1].to(device).repeat(n)
+                t = self._filled.get(name)
+                if t is None or t.device != device or t.numel() < n:
+                    rows = max(256, 1 << (n - 1).bit_length())
+                    t = torch.full((rows,), self._scalar[name], dtype=_SETTINGS[name][0]).to(device)
+                    self._filled[name] = t
                 t = t[:n]
             out.append(t)
         return out

@@ -85,3 +85,73 @@ def test_a_flat_tail_far_below_the_peak_counts_in_the_log_probability(vocab, set
     x[1] = x[1].clamp(min=-22.9 * t)
     x[2, ::3] = -22.3 * t
     compare(x, u, **settings)
+
+
+def _sleep():
+    torch.cuda._sleep(200_000_000)              # about a tenth of a second of this stream
+
+
+def _drawn(settings, x, u):
+    from insitu_b200.sampling import Sampler
+    out = Sampler(**settings)(x, u)
+    torch.cuda.synchronize()
+    return out
+
+
+SETTINGS = dict(temperature=1.7, top_k=40, top_p=0.9, min_p=0.01)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [9, 700])
+def test_a_sampler_fills_its_settings_before_another_stream_reads_them(rows):
+    """A second stream's call, not ordered after the first stream's: the first
+    stream has still a tenth of a second of other work to do."""
+    from insitu_b200.sampling import Sampler
+    x, u = inputs(rows, 500, seed=1)
+    want = _drawn(SETTINGS, x, u)
+    sampler, other = Sampler(**SETTINGS), torch.cuda.Stream()
+    sampler(x[:3], u[:3])
+    zeros = [torch.zeros(n, device="cuda") for n in (9, 256, 700, 1024) for _ in range(20)]
+    torch.cuda.synchronize()
+    del zeros                                   # memory that a fill would find holds zeros
+    _sleep()
+    sampler(x, u)
+    with torch.cuda.stream(other):
+        got = sampler(x, u)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_settings_that_a_sampler_replaces_stay_while_another_stream_reads_them():
+    from insitu_b200.sampling import Sampler
+    x, u = inputs(700, 500, seed=2)
+    want = _drawn(SETTINGS, x[:9], u[:9])
+    sampler, other = Sampler(**SETTINGS), torch.cuda.Stream()
+    sampler(x[:9], u[:9])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        _sleep()
+        got = sampler(x[:9], u[:9])
+    sampler(x, u)                               # more rows than any call before: new tensors
+    for n in (9, 256):
+        zeros = [torch.zeros(n, device="cuda") for _ in range(200)]
+        zeros += [torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(200)]
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+def test_settings_given_on_the_device_are_ready_on_every_stream():
+    from insitu_b200.sampling import Sampler
+    x, u = inputs(700, 500, seed=3)
+    want = _drawn(SETTINGS, x, u)
+    columns = {k: torch.full((700,), v, dtype=torch.float64 if isinstance(v, float) else torch.int64, device="cuda")
+               for k, v in SETTINGS.items()}
+    torch.cuda.synchronize()
+    _sleep()
+    sampler, other = Sampler(**columns), torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        got = sampler(x, u)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
