@@ -242,6 +242,7 @@ at::Tensor tree_scan(int64_t h, at::IntArrayRef seq_ids, at::IntArrayRef nodes, 
                           mask.dim() == 2 && mask.size(0) == total,
                       "insitu: mask must be a contiguous int64 (nodes, words) tensor on q's device");
     c10::cuda::CUDAGuard guard(q.device());
+    used_here(mask);
     const std::vector<int32_t> s = ids32(seq_ids), n = ids32(nodes);
     const int64_t bytes = ins_tree_workspace(handle(h), n_ids(seq_ids), s.data(), n.data());
     if (bytes < 0) check(INS_EINVAL);

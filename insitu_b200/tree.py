@@ -73,7 +73,9 @@ class DraftTree:
         return self.offsets[-1]
 
     def mask(self, device) -> torch.Tensor:
-        """The nodes' masks, (nodes, words) int64 bit patterns, on ``device``."""
+        """The nodes' masks, (nodes, words) int64 bit patterns, on ``device``.
+        They are copied once (the host waits for it), and then ready for calls
+        on every stream."""
         if self._mask.device != torch.device(device):
             self._mask = self._mask.to(device)
         return self._mask
