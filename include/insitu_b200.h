@@ -156,7 +156,10 @@ int ins_cache_set_scan_kernel(ins_cache *cache, int32_t mode);
  * staged rows are announced 16 larger than the copies that land, so its own
  * wait cannot complete. The waits give up, the launch still finishes, and
  * ins_cache_status returns INS_ETIMEOUT; no GPU fault is involved. item < 0
- * holds nothing back. */
+ * holds nothing back. ins_tree_scan's waits for its copies of cached rows take
+ * the same limit, at most 2^18 polls (about a second); there `item` is a CTA of the launch and `chunk` the number,
+ * among the tiles of cached rows that this CTA reads, of the one whose copies
+ * are announced 16 bytes larger. */
 int ins_cache_set_wait_test(ins_cache *cache, int32_t poll_limit, int32_t item, int32_t chunk,
                             int32_t head);
 

@@ -101,6 +101,13 @@ struct Staging {
     }
 };
 
+// Limits of the kernels' bounded waits and the copies held back in tests
+// (ins_cache_set_wait_test).
+struct WaitTest {
+    int32_t poll_limit = 1 << 22;
+    int32_t item = -1, chunk = 0;
+};
+
 // What the host knows of a cache's pages. A page is free (on free_pages), or
 // held by page_refs[page] sequences: the ingress opens pages for one
 // sequence, ins_cache_fork adds holders. Only pages full of rows are shared;
@@ -124,6 +131,7 @@ struct CacheBase {
     Staging stage_c;                    // positions of ins_seam
     Staging stage_p;                    // page operations and tree plans
     int64_t *launches = nullptr;        // the handle's kernel count
+    WaitTest wait;
 
     int64_t capacity() const { return (int64_t)cfg.max_pages_per_seq * cfg.page_tokens; }
     int32_t *table_row(int32_t seq) const { return h_page_table + (size_t)seq * (size_t)cfg.max_pages_per_seq; }

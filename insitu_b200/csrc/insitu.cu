@@ -373,6 +373,7 @@ int ins_cache_set_wait_test(ins_cache *c, int32_t poll_limit, int32_t item, int3
     c->chunk.hold_item = item;
     c->chunk.hold_chunk = chunk;
     c->chunk.hold_head = head;
+    c->wait = WaitTest{poll_limit, item, chunk};
     return INS_OK;
 }
 

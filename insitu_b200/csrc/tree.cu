@@ -42,6 +42,7 @@ struct TreeArgs {
     float *acc, *ml;                         // partials: [unit][rows][64], [unit][rows][2]
     int32_t *status;
     int32_t n_seqs, words, chunk, row_tiles_rows;
+    int32_t poll_limit, hold_cta, hold_tile; // tests: the tile whose copies are announced too large
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
@@ -56,10 +57,12 @@ __device__ __forceinline__ void bar_init_fence() {
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Waits for the phase of `parity`, at most 2^22 polls (about a second);
-// false: it gave up.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-    for (int i = 0; i < (1 << 22); ++i) {
+// Polls of a bounded wait: one that finds nothing lasts 4 us, so about a second.
+constexpr int WAIT_POLLS = 1 << 18;
+// Waits for the phase of `parity`, at most `limit` polls; false: it gave up
+// (this thread did: a warp has to agree before it goes on).
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int limit) {
+    for (int i = 0; i < limit; ++i) {
         uint32_t done;
         asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
                      : "=r"(done)
@@ -280,7 +283,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         if (j >= n_tiles) return;
         const int p0 = lo + j * FEW_TILE, rows16 = (min(FEW_TILE, hi - p0) + 15) & ~15;
         const uint32_t bar = bars + (n % STAGES) * 8, dst = ring + (n % STAGES) * stage;
-        if (lane == 0) bar_expect(bar, rows16 * (kbytes + vbytes + 4));
+        const bool held = (int)blockIdx.x == a.hold_cta && j == a.hold_tile;
+        if (lane == 0) bar_expect(bar, rows16 * (kbytes + vbytes + 4) + (held ? 16 : 0));
         __syncwarp();
         // one lane per run of rows inside a page; pages hold a multiple of 16 rows
         int at = 0;
@@ -319,7 +323,9 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
     for (int j = warp; j < n_tiles; j += NW, ++n) {
         __syncwarp();                                 // every lane has read the slot's previous tile
         issue(issued++);
-        if (!bar_wait(bars + (n % STAGES) * 8, (n / STAGES) & 1)) {
+        // the lanes poll one by one: the warp gives up as one, as what follows
+        // takes all of its lanes
+        if (__any_sync(FULL, !bar_wait(bars + (n % STAGES) * 8, (n / STAGES) & 1, a.poll_limit))) {
             lost = true;
             break;
         }
@@ -579,7 +585,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         // report it, and let the copies in flight land before the CTA goes
         if (lane == 0) atomicOr(a.status, ST_TIMEOUT);
         for (int k = n; k < issued; ++k)
-            if (warp + k * NW < n_tiles) bar_wait(bars + (k % STAGES) * 8, (k / STAGES) & 1);
+            if (warp + k * NW < n_tiles) bar_wait(bars + (k % STAGES) * 8, (k / STAGES) & 1, a.poll_limit);
     }
 
     // join the warps: each row's maximum, then the scaled sums
@@ -1009,7 +1015,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
     const int64_t end = run_start(cta + 1, all_tiles, gridDim.x);
     bool lost = false;                               // a wait gave up: the same for all lanes that wait together
     auto wait = [&](uint32_t bar, int phase) {
-        if (!lost && !bar_wait(bar, (uint32_t)phase & 1u)) {
+        if (!lost && !bar_wait(bar, (uint32_t)phase & 1u, a.poll_limit)) {
             lost = true;
             atomicOr(a.status, ST_TIMEOUT);
         }
@@ -1028,7 +1034,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
             int64_t next;
             const Segment s = segment_at(seqs, a.n_seqs, g, RU, t, end, cta, &next);
             const TreeSeq sq = seqs[s.seq];
-            const int len = sq.context + sq.nodes;
+            const int len = sq.context + sq.nodes, kt0 = kt;
             constexpr int KV4 = KB * 2, VV4 = VB * 2;            // 32-bit words of a row's codes
             const int32_t *pages = a.table + (int64_t)sq.seq * g.max_pages;
             // Bulk copies of this warp's 32 rows of tile s.lo + k, in the runs
@@ -1046,7 +1052,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                 if (s.lo + k >= s.hi || p0 >= len) return;
                 const int slot = (kr + k) % MANY_RING, rows16 = (min(32, len - p0) + 15) & ~15;
                 const uint32_t bar = row_bar(warp - 8, slot), dst = ring + slot * MANY_SLOT;
-                if (lane == 0) bar_expect(bar, rows16 * (8 * KB + 8 * VB + 4));
+                const bool held = cta == a.hold_cta && kt0 + k == a.hold_tile && warp == 8;
+                if (lane == 0) bar_expect(bar, rows16 * (8 * KB + 8 * VB + 4) + (held ? 16 : 0));
                 __syncwarp();
                 const int in0 = row_in_page(g, p0), first = min(rows16, g.P - in0);
                 const int at = lane ? first : 0, n = lane ? rows16 - first : first, in = lane ? 0 : in0;
@@ -1126,7 +1133,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
         }
         // copies that a lost wait left in flight land before the CTA goes
         if (lost)
-            for (int i = 0; i < MANY_RING; ++i) bar_wait(row_bar(warp - 8, i), uses >> i & 1u);
+            for (int i = 0; i < MANY_RING; ++i) bar_wait(row_bar(warp - 8, i), uses >> i & 1u, a.poll_limit);
     } else if (warp == 12) {
         // ---- this warp issues every product. All lanes walk the same steps
         // (so that operands stay in uniform registers: with one lane inside a
@@ -1186,7 +1193,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
         // nothing may be in flight when the tensor memory goes
         if (elect_one()) tc_commit(fin);
         __syncwarp();
-        if (!bar_wait(fin, 0)) atomicOr(a.status, ST_TIMEOUT);
+        if (!bar_wait(fin, 0, WAIT_POLLS)) atomicOr(a.status, ST_TIMEOUT);
         __syncwarp();
     } else {
         // ---- softmax: thread `row` of stream `i` owns one query row
@@ -1615,6 +1622,9 @@ int tree_body(CacheBase *c, int32_t B, const int32_t *seq, const int32_t *nodes,
     a.words = words;
     a.chunk = (int32_t)p.chunk;
     a.row_tiles_rows = p.rows;
+    a.poll_limit = std::min(c->wait.poll_limit, WAIT_POLLS);
+    a.hold_cta = c->wait.item;
+    a.hold_tile = c->wait.chunk;
     Plan plan;
     plan.add(p.seqs);
     // up to 8 rows the products are taken transposed: one node of 1,048,576

@@ -166,7 +166,8 @@ class PagedCache:
     def set_wait_test(self, poll_limit: int = 1 << 22, item: int = -1, chunk: int = 0,
                       head: int = 0) -> None:
         """Test hook of the online scan's bounded waits (ins_cache_set_wait_test):
-        the look-back of the fused kernel, the staged rows of the value pass."""
+        the look-back of the fused kernel, the staged rows of the value pass;
+        for ``tree_scan``, tile ``chunk`` of the rows that CTA ``item`` copies."""
         _lib.check(self._L.ins_cache_set_wait_test(self._h, poll_limit, item, chunk, head))
 
     def recomputed(self) -> int:

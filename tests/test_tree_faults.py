@@ -34,3 +34,35 @@ def test_a_dropped_trees_mask_stays_while_another_stream_reads_it(nodes):
     assert torch.equal(got.view(torch.int16), want.view(torch.int16))
     del zeros
     pc.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nodes", [1, 3, 6])
+@pytest.mark.parametrize("tile", [0, 1, 21])
+def test_a_wait_for_rows_that_runs_out_is_reported_and_the_context_survives(nodes, tile):
+    """One tile's copies are announced 16 bytes larger than they are, so the
+    wait for them cannot complete: it gives up after the lowered limit, the
+    launch ends, the status is INS_ETIMEOUT, and the next scan is what it was.
+    Every copy lands; nothing faults."""
+    from insitu_b200 import DraftTree
+    from insitu_b200._lib import DeviceTimeout
+    rng = np.random.default_rng(nodes)
+    pc = make(4, 2, 8, 4, 256, 60160, 1)
+    pc.put_rows([0], [60001], torch.from_numpy(random_rows(rng, pc, 60001)).to(pc.device))
+    q = torch.from_numpy(np.rint(rng.standard_normal((nodes, 32, 64)) * 16384).astype(np.int32)).to(pc.device)
+    tree = DraftTree([random_tree(rng, nodes)])
+    want = pc.tree_scan([0], q, tree)
+    pc.status()
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    for cta in (0, 77):
+        pc.set_wait_test(poll_limit=4096, item=cta, chunk=tile)
+        begin.record()
+        pc.tree_scan([0], q, tree)
+        end.record()
+        with pytest.raises(DeviceTimeout):
+            pc.status()
+        print(f"{nodes} nodes, tile {tile} of CTA {cta}: {begin.elapsed_time(end):.2f} ms")
+        pc.set_wait_test()
+        assert torch.equal(pc.tree_scan([0], q, tree).view(torch.int16), want.view(torch.int16))
+        pc.status()
+    pc.close()
