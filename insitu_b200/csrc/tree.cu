@@ -897,7 +897,10 @@ __device__ __forceinline__ bool weigh(uint32_t S, uint32_t P, float ref, float &
             acc[j & 1] = add_pair(acc[j & 1], pair64(__float_as_uint(e0), __float_as_uint(e1)));
             p[j] = pack_half2(e0, e1);
         }
-        if (c == 0 && !p_free()) return false;
+        if (c == 0 && !p_free()) {
+            tc_wait_load(x[1]);
+            return false;
+        }
         tc_store8(P + 8 * c, p);
         if (c < 7) tc_wait_load(x[(c + 1) & 1]);
     }
@@ -1029,7 +1032,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
         const uint32_t ring = sm0 + MANY_RING_AT + (warp - 8) * MANY_RING * MANY_SLOT;
         const float unit = exp2f((float)-g.norm_frac);
         int kt = 0, kr = 0;                                      // tiles so far; the ring slot of the segment's first
-        uint32_t uses = 0;                                       // bit i: the parity that ring slot i waits for next
+        // of ring slot i, bit i: the parity that its next wait is for; whether copies into it are on their way
+        uint32_t uses = 0, coming = 0;
         for (int seg = 0; t < end && !lost; ++seg) {
             int64_t next;
             const Segment s = segment_at(seqs, a.n_seqs, g, RU, t, end, cta, &next);
@@ -1054,6 +1058,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                 const uint32_t bar = row_bar(warp - 8, slot), dst = ring + slot * MANY_SLOT;
                 const bool held = cta == a.hold_cta && kt0 + k == a.hold_tile && warp == 8;
                 if (lane == 0) bar_expect(bar, rows16 * (8 * KB + 8 * VB + 4) + (held ? 16 : 0));
+                coming |= 1u << slot;
                 __syncwarp();
                 const int in0 = row_in_page(g, p0), first = min(rows16, g.P - in0);
                 const int at = lane ? first : 0, n = lane ? rows16 - first : first, in = lane ? 0 : in0;
@@ -1076,7 +1081,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                 if ((s.lo + k) * MANY_TILE + (warp - 8) * 32 < len) {
                     const int slot = (kr + k) % MANY_RING;
                     wait(row_bar(warp - 8, slot), uses >> slot);
-                    uses ^= 1u << slot;
+                    if (!lost) uses ^= 1u << slot, coming ^= 1u << slot;
                     const uint8_t *st = sm + (ring - sm0) + slot * MANY_SLOT;
                     const uint8_t *pk = st + lane * 8 * KB, *pv = st + 32 * 8 * KB + lane * 8 * VB;
 #pragma unroll
@@ -1133,7 +1138,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
         }
         // copies that a lost wait left in flight land before the CTA goes
         if (lost)
-            for (int i = 0; i < MANY_RING; ++i) bar_wait(row_bar(warp - 8, i), uses >> i & 1u, a.poll_limit);
+            for (int i = 0; i < MANY_RING; ++i)
+                if (coming >> i & 1u) bar_wait(row_bar(warp - 8, i), uses >> i & 1u, a.poll_limit);
     } else if (warp == 12) {
         // ---- this warp issues every product. All lanes walk the same steps
         // (so that operands stay in uniform registers: with one lane inside a

@@ -37,7 +37,7 @@ def test_a_dropped_trees_mask_stays_while_another_stream_reads_it(nodes):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("nodes", [1, 3, 6])
+@pytest.mark.parametrize("nodes", [1, 3, 6, 24, 64])
 @pytest.mark.parametrize("tile", [0, 1, 21])
 def test_a_wait_for_rows_that_runs_out_is_reported_and_the_context_survives(nodes, tile):
     """One tile's copies are announced 16 bytes larger than they are, so the
