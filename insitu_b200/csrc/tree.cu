@@ -57,6 +57,9 @@ __device__ __forceinline__ void bar_init_fence() {
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// Orders this thread's ordinary accesses to shared memory before later ones by
+// copies and tensor cores (once a barrier has passed).
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Polls of a bounded wait: one that finds nothing lasts 4 us, so about a second.
 constexpr int WAIT_POLLS = 1 << 18;
 // Waits for the phase of `parity`, at most `limit` polls; false: it gave up
@@ -243,6 +246,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
     if (lane == 0)
         for (int i = 0; i < STAGES; ++i) bar_init(bars + i * 8, 1);
     bar_init_fence();
+    fence_async();                                   // copies overwrite the centroids
     wait_prior_grid();
     __syncthreads();
 
@@ -732,7 +736,6 @@ __device__ __forceinline__ bool elect_one() {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
