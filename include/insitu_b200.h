@@ -468,7 +468,8 @@ int ins_cache_put_rows(ins_cache *cache, int32_t B, const int32_t *seq_ids, cons
  * ins_ingress rotates it, 16-byte aligned; out: device bf16 of that shape,
  * 16-byte aligned; workspace: device, ins_tree_workspace bytes for the same
  * cache, seq_ids and nodes (the lengths at the call), 16-byte aligned, free
- * again once the call's work is done. Any code widths. Stream-ordered; a
+ * again once the call's work is done. Any code widths and fraction bits, with
+ * a largest centroid in [2^-8, 2^4] in real units. Stream-ordered; a
  * bounded wait that gives up latches INS_ETIMEOUT for ins_cache_status. */
 int64_t ins_tree_workspace(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int32_t *nodes);
 int ins_tree_scan(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int32_t *nodes,

@@ -132,6 +132,7 @@ struct CacheBase {
     Staging stage_p;                    // page operations and tree plans
     int64_t *launches = nullptr;        // the handle's kernel count
     WaitTest wait;
+    double cent_max = 0.0;              // the largest centroid's magnitude, of keys and values
 
     int64_t capacity() const { return (int64_t)cfg.max_pages_per_seq * cfg.page_tokens; }
     int32_t *table_row(int32_t seq) const { return h_page_table + (size_t)seq * (size_t)cfg.max_pages_per_seq; }

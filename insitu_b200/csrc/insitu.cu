@@ -6,7 +6,9 @@
 // (cache/compressed.py:42-86). Kernels read device mirrors of it that every
 // mutating call refreshes with stream-ordered copies before its launch.
 
+#include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <string>
@@ -278,6 +280,9 @@ int ins_cache_create(const ins_config *cfg, const ins_tables *tb, int32_t device
         const int64_t lim = (1ll << 47) / cmax;
         c->g.q_lim = lim < (1ll << 30) ? lim : (1ll << 30);
     }
+    for (int i = 0; i < nk; ++i) c->cent_max = std::max(c->cent_max, std::fabs((double)tb->k_centroids[i]));
+    for (int i = 0; i < nv; ++i) c->cent_max = std::max(c->cent_max, std::fabs((double)tb->v_centroids[i]));
+    c->cent_max = std::ldexp(c->cent_max, -cfg->centroid_frac);
     c->device = device;
     auto cleanup = [&](int rc) {
         ins_cache_destroy(c);

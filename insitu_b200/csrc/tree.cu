@@ -13,10 +13,19 @@
 // is decoded from codes on the way: fp16 operands (a centroid, a query or a
 // probability is rounded to 11 bits, which moves the bf16 result by less than
 // its own rounding), fp32 sums, maxima and exponents.
+//
+// The products take the query as q/2^16 and the norms as norm/2^9 whatever
+// the cache's formats are: 32-bit queries stay below 2^15 then and 16-bit
+// norms up to 2^6, inside fp16's range with the weights' own factors. The
+// powers of two between these and the formats (1 for the default ones) go to
+// the scores and to the outputs in fp32 (TreeArgs::score_unit, out_unit);
+// k_tree_many, whose exponentials have no room for another multiplication (2 %
+// of its time), takes a score's down to its queries or up to its keys' norms.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "plan.cuh"
@@ -25,6 +34,8 @@ namespace ins {
 
 constexpr int TREE_MAX_NODES = 256;          // drafted tokens of one sequence
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float Q_UNIT = LOG2E / 65536.0f;   // of a query, in log2 units
+constexpr float NORM_UNIT = 1.0f / 512.0f;
 
 // One sequence of a call. Its work units are [unit0, next sequence's unit0):
 // (split of `chunk` tokens, row tile, KV head), the head innermost.
@@ -43,6 +54,8 @@ struct TreeArgs {
     int32_t *status;
     int32_t n_seqs, words, chunk, row_tiles_rows;
     int32_t poll_limit, hold_cta, hold_tile; // tests: the tile whose copies are announced too large
+    // what the products' fixed units leave to the formats: for the scores (k_tree_many: its two factors), the outputs
+    float score_unit, q_scale, k_scale, out_unit;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
@@ -158,7 +171,7 @@ __device__ __forceinline__ int find_seq(const TreeSeq *seqs, int n, int i) {
 //
 // The running maximum moves only when a score exceeds it by more than 2^8
 // (LAG, in the exponent's base): until then exp2 stays below 256 and times a
-// norm below 2^14, inside fp16's range, so a rescale of the accumulators is
+// norm (at most 2^6) below 2^14, inside fp16's range, so a rescale of the accumulators is
 // rare and the maximum needs no exchange of lanes at every step.
 //
 // Up to 8 rows (HALF) the products are taken transposed, S^T = K Q^T and
@@ -275,7 +288,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
                 const int4 v = ok ? p[ks] : make_int4(0, 0, 0, 0);
-                const float u = LOG2E * exp2f((float)-g.qk_frac);
+                const float u = Q_UNIT;
                 qf[m][ks][half] = pack_half2((float)v.x * u, (float)v.y * u);
                 qf[m][ks][half + 2] = pack_half2((float)v.z * u, (float)v.w * u);
             }
@@ -316,7 +329,6 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
         m_ref[m][0] = m_ref[m][1] = NONE;
         l[m][0] = l[m][1] = 0.0f;
     }
-    const float nunit = exp2f((float)-g.norm_frac);
     // this warp's norms of a tile: 16 tokens' (key, value) in each 128 bytes
     uint8_t *norms = sm + L::NORMS_AT + warp * 512;
     const uint32_t lane4 = lane * 4, value8 = 128 + lane % 16 * 8;
@@ -341,7 +353,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
             const int tok = lane + 32 * i;
             const uint32_t w = *reinterpret_cast<const uint32_t *>(sn + tok * 4);
             *reinterpret_cast<float2 *>(norms + tok * 8) =
-                make_float2(norm_value(w & 0xffffu, nunit), norm_value(w >> 16, nunit));
+                make_float2(norm_value(w & 0xffffu, NORM_UNIT) * a.score_unit, norm_value(w >> 16, NORM_UNIT));
         }
         __syncwarp();
         const int p0 = lo + j * FEW_TILE;
@@ -644,7 +656,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
                 sum += f * jml[(w * R + r) * 2 + 1];
             }
         if (sq.splits == 1) {
-            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;   // a row that sees nothing is zero
+            const float inv = sum > 0.0f ? a.out_unit / sum : 0.0f;   // a row that sees nothing is zero
             const int node = (row0 + r) / G, qh = (row0 + r) % G;
             __nv_bfloat162 *dst = reinterpret_cast<__nv_bfloat162 *>(
                 a.out + (((int64_t)(sq.node0 + node) * g.n_kv + head) * G + qh) * D + c4 * 4);
@@ -1033,7 +1045,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
         const int row = tid - 256;
         const uint32_t lane4 = lane * 4;
         const uint32_t ring = sm0 + MANY_RING_AT + (warp - 8) * MANY_RING * MANY_SLOT;
-        const float unit = exp2f((float)-g.norm_frac);
         int kt = 0, kr = 0;                                      // tiles so far; the ring slot of the segment's first
         // of ring slot i, bit i: the parity that its next wait is for; whether copies into it are on their way
         uint32_t uses = 0, coming = 0;
@@ -1103,7 +1114,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                 cn = live ? cn : 0;                              // past the end: a zero norm makes a zero row
                 const int st = kt % MANY_STAGES;
                 if (kt >= MANY_STAGES) wait(empty(st), kt / MANY_STAGES - 1);
-                const float kn = norm_value(cn & 0xffffu, unit), vn = norm_value(cn >> 16, unit);
+                const float kn = norm_value(cn & 0xffffu, NORM_UNIT) * a.k_scale, vn = norm_value(cn >> 16, NORM_UNIT);
                 auto codes = [&](const uint32_t *w, int bits, int j) -> uint32_t {   // pair j's entry, this lane's copy
                     if (bits == 4) return entry_at(w[j / 4], j % 4, lane4);
                     if (bits == 2) return entry_at((j & 1 ? w[j / 8] >> 4 : w[j / 8]) & 0x0f0f0f0fu, j % 8 / 2, lane4);
@@ -1223,7 +1234,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
             // are done, or (!ROWS) half of the one tile, once both streams' are.
             if (!ROWS && seg) wait(seg_done, seg - 1);
             {
-                const float u = LOG2E * exp2f((float)-g.qk_frac);
+                const float u = Q_UNIT * a.q_scale;
 #pragma unroll
                 for (int x = 0; x < (ROWS ? 8 : 4); ++x) {
                     const int at = (ROWS ? 1024 * i + row + 128 * x : tid + 256 * x), r = at / 8, c = at % 8;
@@ -1336,7 +1347,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_tree_many(Geo g, TreeArgs a
                 }
                 if (!mine || qr >= rows_all) continue;
                 if (s.slot < 0) {
-                    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                    const float inv = l > 0.0f ? a.out_unit / l : 0.0f;
                     uint4 *dst = reinterpret_cast<uint4 *>(
                         a.out + (((int64_t)(sq.node0 + qr / g.H) * g.n_kv + s.head) * g.H + qr % g.H) * D + 32 * c);
 #pragma unroll
@@ -1414,7 +1425,7 @@ __global__ void __launch_bounds__(128) k_tree_join(Geo g, TreeArgs a, int32_t R,
             wt[r * splits + s] = f;
         }
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const float inv = sum > 0.0f ? a.out_unit / sum : 0.0f;
         for (int s = lane; s < splits; s += 32) wt[r * splits + s] *= inv;
     }
     __syncthreads();
@@ -1448,6 +1459,10 @@ namespace {
 // 384 : 298; 3b/3b, 6 sequences to 9,001 tokens (about 20) 45.5 : 41.7. Above
 // 64 rows k_tree_few decodes each row three times and more.
 constexpr int MANY_FROM = 32, MANY_SURE = 64, MANY_TILES = 12;
+// Its keys (centroid times norm, below 2^4 times 2^6) can take a factor of up
+// to 2^5 of the scores' before they leave fp16; beyond, k_tree_few.
+constexpr int MANY_SHIFT = 5;
+int score_shift(const Geo &g) { return 16 + 9 - g.qk_frac - g.norm_frac; }
 
 // How a call is cut: rows a tile, tokens a split, and what that takes.
 struct TreePlan {
@@ -1484,7 +1499,7 @@ int make_plan(const CacheBase *c, int32_t B, const int32_t *seq, const int32_t *
     }
     if (all > INT32_MAX / (g.n_kv * g.H)) return fail(INS_EBADLEN, "too many nodes in one call");
     if (p.seqs.empty()) return INS_OK;
-    const bool paired = (g.kb == 4 && g.vb == 2) || (g.kb == 3 && g.vb == 3);
+    const bool paired = ((g.kb == 4 && g.vb == 2) || (g.kb == 3 && g.vb == 3)) && score_shift(g) <= MANY_SHIFT;
     int64_t kv_tiles = 0;
     for (const TreeSeq &s : p.seqs) kv_tiles += g.n_kv * ((s.context + s.nodes + MANY_TILE - 1) / MANY_TILE);
     if (paired && (most > MANY_SURE || (most > MANY_FROM && kv_tiles > (int64_t)MANY_TILES * sms))) {
@@ -1609,6 +1624,9 @@ int tree_body(CacheBase *c, int32_t B, const int32_t *seq, const int32_t *nodes,
         return INS_OK;
     }
     if (p.seqs.empty()) return INS_OK;
+    // centroids are fp16 in real units, times a norm in k_tree_many
+    if (c->g.qk_frac < 0 || c->g.qk_frac > 31 || c->cent_max > 16.0 || (c->cent_max > 0.0 && c->cent_max < 1.0 / 256))
+        return fail(INS_EINVAL, "tree scan: qk_frac in [0, 31] and a largest centroid in [2^-8, 2^4] are supported");
     for (const TreeSeq &t : p.seqs)
         if (t.nodes > 64 * words) return fail(INS_EINVAL, "the mask's words are too few for a tree's nodes");
     if (!mask || !q || !out) return fail(INS_EINVAL, "tree scan: NULL buffer");
@@ -1634,6 +1652,10 @@ int tree_body(CacheBase *c, int32_t B, const int32_t *seq, const int32_t *nodes,
     a.poll_limit = std::min(c->wait.poll_limit, WAIT_POLLS);
     a.hold_cta = c->wait.item;
     a.hold_tile = c->wait.chunk;
+    a.score_unit = std::ldexp(1.0f, score_shift(c->g));
+    a.q_scale = std::min(a.score_unit, 1.0f);
+    a.k_scale = std::max(a.score_unit, 1.0f);
+    a.out_unit = std::ldexp(1.0f, 9 - c->g.norm_frac);
     Plan plan;
     plan.add(p.seqs);
     // up to 8 rows the products are taken transposed: one node of 1,048,576
