@@ -397,7 +397,9 @@ int64_t ins_scan_recomputed_total(ins_cache *cache, void *stream);
  * 2. The caller exchanges the maxima; shard r's m_in is the maximum over
  *    shards before it (-2^47 for the first), same layout.
  * 3. ins_scan_part, with the arguments of step 1: writes one composite per
- *    item to `part` (device, ins_part_bytes(B) bytes).
+ *    item to `part` (device, ins_part_bytes(B) bytes). Refused (EINVAL) after
+ *    another scan, or a reset, compaction or truncation of one of its
+ *    sequences; rows added since do not matter.
  * 4. The caller gathers the shards' parts, in causal order, into one device
  *    buffer; ins_merge_parts folds them and writes `out` and `stats` as
  *    ins_scan would for the whole sequences. */

@@ -2,6 +2,7 @@
 // reporting, the per-call upload ring, and the host's page bookkeeping.
 #pragma once
 
+#include <algorithm>
 #include <climits>
 #include <cstring>
 #include <new>
@@ -132,6 +133,10 @@ struct CacheBase {
     Staging stage_p;                    // page operations and tree plans
     int64_t *launches = nullptr;        // the handle's kernel count
     WaitTest wait;
+    // the sequences whose scores an ins_scan_maxima took, while ins_scan_part
+    // may still use them
+    std::vector<int32_t> split_seq;
+    bool split_armed = false;
     double cent_max = 0.0;              // the largest centroid's magnitude, of keys and values
 
     int64_t capacity() const { return (int64_t)cfg.max_pages_per_seq * cfg.page_tokens; }
@@ -141,6 +146,10 @@ struct CacheBase {
         free_pages.pop_back();
         page_refs[(size_t)pg] = 1;
         return pg;
+    }
+    // Rows of `seq` have gone or moved (rows only added change nothing).
+    void rows_changed(int32_t seq) {
+        if (split_armed && std::find(split_seq.begin(), split_seq.end(), seq) != split_seq.end()) split_armed = false;
     }
     void release_page(int32_t pg) {
         if (--page_refs[(size_t)pg] == 0) free_pages.push_back(pg);

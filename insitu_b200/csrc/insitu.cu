@@ -35,11 +35,9 @@ struct ins_cache : ins::CacheBase {
     unsigned long long *d_redo_total = nullptr;   // items the sequential kernel recomputed, running
     ChunkScratch chunk;                 // scratch of the context-parallel scan
     uint64_t gen = 0;                   // bumped by every call that rewrites `chunk`
-    struct {                            // context split: phase 1 waiting for phase 2
-        bool armed = false;
+    struct {                            // context split: phase 1 waiting for phase 2 (split_armed, split_seq)
         uint64_t gen = 0;
         int32_t B = 0;
-        std::vector<int32_t> seq;
         std::vector<int64_t> T;
         const int32_t *q_rot = nullptr;
         int32_t rs = 0;                 // rows-per-thread instantiation phase 1 used
@@ -396,6 +394,7 @@ int ins_cache_reset(ins_cache *c, int32_t seq) {
             pg = -1;
         }
         c->h_seq_lens[s] = 0;
+        c->rows_changed(s);
     }
     if (int rc = push_mirrors(c, 0, lo, hi)) return rc;
     CK(cudaStreamSynchronize(0));
@@ -1002,14 +1001,14 @@ int ins_scan_maxima(ins_cache *c, int32_t B, const int32_t *seq_ids, const int64
                                 "codes, the default fixed-point format)");
     DeviceGuard dg(c->device);
     cudaStream_t s = (cudaStream_t)stream;
-    c->split.armed = false;
+    c->split_armed = false;
     const int64_t *d_T;
     const int32_t *d_seq;
-    if (int rc = stage_scan_args(c, B, seq_ids, lengths, s, &c->split.seq, &c->split.T, &d_T, &d_seq))
+    if (int rc = stage_scan_args(c, B, seq_ids, lengths, s, &c->split_seq, &c->split.T, &d_T, &d_seq))
         return rc;
     ++c->gen;
     if (int rc = split_maxima(c, variant, B, d_seq, d_T, c->split.T.data(), q_rot, maxima, s)) return rc;
-    c->split.armed = true;
+    c->split_armed = true;
     c->split.gen = c->gen;
     c->split.B = B;
     c->split.q_rot = q_rot;
@@ -1022,17 +1021,17 @@ int ins_scan_part(ins_cache *c, int32_t B, const int32_t *seq_ids, const int64_t
     if (B <= 0 || !seq_ids || !q_rot || !m_in || !part) return fail(INS_EINVAL, "scan_part arguments");
     if (((uintptr_t)part & 7u) || ((uintptr_t)m_in & 7u)) return fail(INS_EINVAL, "part/m_in must be 8-byte aligned");
     auto &sp = c->split;
-    bool same = sp.armed && sp.gen == c->gen && sp.B == B && sp.q_rot == q_rot;
+    bool same = c->split_armed && sp.gen == c->gen && sp.B == B && sp.q_rot == q_rot;
     for (int32_t i = 0; same && i < B; ++i) {
         const int32_t sq = seq_ids[i];
         const int64_t T = lengths ? lengths[i] : (sq >= 0 && sq < c->cfg.max_seqs ? c->h_seq_lens[sq] : -1);
-        same = sq == sp.seq[i] && T == sp.T[i];
+        same = sq == c->split_seq[i] && T == sp.T[i];
     }
     if (!same)
         return fail(INS_EINVAL, "ins_scan_part must follow ins_scan_maxima on this cache with the same "
-                                "sequences, lengths and q_rot, with no scan in between");
+                                "sequences, lengths and q_rot, with no scan in between and no change of their rows");
     DeviceGuard dg(c->device);
-    sp.armed = false;
+    c->split_armed = false;
     return split_part(c, chunk_variant(c->g, c->g.H), m_in, part, (cudaStream_t)stream);
 }
 

@@ -416,6 +416,7 @@ int compact_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *bas
             dropped.push_back(tab[p]);
             tab[p] = -1;
         }
+        if (j.first < j.end || j.end < c->h_seq_lens[seq[b]]) c->rows_changed(seq[b]);
         c->h_seq_lens[seq[b]] = (int32_t)j.end;
         if (j.p0 >= j.p1) continue;
         // a replaced page's rows before the first moved one come along

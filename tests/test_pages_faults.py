@@ -31,3 +31,41 @@ def test_a_fork_whose_source_is_also_a_target_is_refused(spare):
     pc.truncate([0, 1], 0)
     assert pc.free_pages == 2 + spare
     pc.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("change", ["truncate", "compact", "reset"])
+def test_a_context_split_does_not_outlive_its_rows(change):
+    """Between the phases rows are dropped and as many others appended: the
+    maxima are of rows that are gone, so the second phase is refused. Changes
+    of other sequences, and rows only added, leave it."""
+    from insitu_b200 import Geometry, PagedCache, QuantConfig
+    rng = np.random.default_rng(3)
+    pc = PagedCache(QuantConfig(key_bits=4, value_bits=2), geo=Geometry(2, 4, 64), max_seqs=3, capacity=4096)
+    wire = lambda s, *shape: torch.from_numpy(np.rint(rng.standard_normal(shape) * s * 65536).astype(np.int32)).cuda()
+    q = wire(0.25, 1, 8, 64)
+    for s in (0, 1):
+        pc.ingress([s] * 3000, wire(1, 3000, 2, 64), wire(1, 3000, 2, 64))
+    maxima = pc.scan_maxima([0], q, lengths=[3000])
+    pc.truncate([1], 2000)
+    pc.compact([1], [list(range(0, 2000, 3))])
+    pc.fork([0], [2])
+    pc.ingress([0] * 10, wire(1, 10, 2, 64), wire(1, 10, 2, 64))
+    want = pc.scan_part([0], torch.full_like(maxima, pc.S_LO), lengths=[3000])
+    maxima = pc.scan_maxima([0], q, lengths=[3000])
+    if change == "truncate":
+        pc.truncate([0], 2900)
+    elif change == "compact":
+        pc.compact([0], [[i for i in range(3010) if i % 50]])
+    else:
+        pc.reset(0)
+    pc.ingress([0] * 3010, wire(1, 3010, 2, 64), wire(1, 3010, 2, 64)) if change == "reset" else \
+        pc.ingress([0] * 200, wire(1, 200, 2, 64), wire(1, 200, 2, 64))
+    with pytest.raises(ValueError):
+        pc.scan_part([0], torch.full_like(maxima, pc.S_LO), lengths=[3000])
+    again = pc.scan_maxima([2], q, lengths=[3000])          # the fork has kept the rows
+    got = pc.scan_part([2], torch.full_like(again, pc.S_LO), lengths=[3000])
+    torch.cuda.synchronize()
+    assert got.shape == want.shape
+    pc.status()
+    pc.close()
