@@ -58,27 +58,35 @@ struct Staging {
     void *d = nullptr;
     int64_t *launches = nullptr;        // the cache's kernel count (an upload may be a launch)
 
+    // Makes room for uploads of `bytes`: what can fail of a reserve, for a call
+    // that has to know before it changes anything.
+    int grow(size_t bytes) {
+        if (bytes <= cap) return INS_OK;
+        size_t want = cap ? cap : 4096;
+        while (want < bytes) want *= 2;
+        for (Slot &o : ring) {
+            if (!o.done) CK(cudaEventCreateWithFlags(&o.done, cudaEventDisableTiming));
+            CK(cudaEventSynchronize(o.done));
+            if (o.h) cudaFreeHost(o.h);
+            if (o.d) cudaFree(o.d);
+            o.h = o.d = nullptr;
+        }
+        cap = 0;
+        for (Slot &o : ring)
+            if (cudaHostAlloc(&o.h, want, cudaHostAllocDefault) != cudaSuccess ||
+                cudaMalloc(&o.d, want) != cudaSuccess) {
+                cudaGetLastError();
+                return fail(INS_ENOMEM, "allocation of " + std::to_string(want) + " B of upload buffers failed");
+            }
+        cap = want;
+        return INS_OK;
+    }
     int reserve(size_t bytes) {
+        if (int rc = grow(bytes)) return rc;
         cur = (cur + 1) % NSLOT;
         Slot &sl = ring[cur];
         if (!sl.done) CK(cudaEventCreateWithFlags(&sl.done, cudaEventDisableTiming));
         CK(cudaEventSynchronize(sl.done));
-        if (bytes > cap) {
-            size_t want = cap ? cap : 4096;
-            while (want < bytes) want *= 2;
-            for (Slot &o : ring) {
-                if (o.done) CK(cudaEventSynchronize(o.done));
-                if (o.h) cudaFreeHost(o.h);
-                if (o.d) cudaFree(o.d);
-                o.h = o.d = nullptr;
-            }
-            cap = 0;
-            for (Slot &o : ring) {
-                CK(cudaHostAlloc(&o.h, want, cudaHostAllocDefault));
-                CK(cudaMalloc(&o.d, want));
-            }
-            cap = want;
-        }
         h = sl.h;
         d = sl.d;
         return INS_OK;

@@ -224,6 +224,12 @@ struct Moves {
         pages.insert(pages.end(), row + p0, row + p1 + 1);
         return off;
     }
+    // Room for what the vectors have reserved, before anything changes.
+    int ready(CacheBase *c) const {
+        if ((int64_t)units.capacity() * c->g.n_kv > INT32_MAX) return fail(INS_EBADLEN, "too many rows in one call");
+        return Plan::ready(c, units.capacity() * sizeof(MoveUnit) + entries.capacity() * sizeof(int2) +
+                                  (kept.size() + pages.capacity()) * sizeof(int32_t) + 64);
+    }
     int launch(CacheBase *c, cudaStream_t s) const {
         Plan plan;
         if (units.empty()) {
@@ -238,7 +244,6 @@ struct Moves {
         }
         plan.add(units);
         const size_t entries_at = plan.add(entries), kept_at = plan.add(kept), pages_at = plan.add(pages);
-        if ((int64_t)units.size() * c->g.n_kv > INT32_MAX) return fail(INS_EBADLEN, "too many rows in one call");
         return plan.run(c, s, [&](const auto &src) {
             *c->launches += 1;
             return launch_after(k_move_rows<std::decay_t<decltype(src)>>, (unsigned)(units.size() * c->g.n_kv),
@@ -280,12 +285,13 @@ int fork_body(CacheBase *c, int32_t B, const int32_t *src, const int32_t *dst, c
                                      std::to_string(c->free_pages.size()) + " free");
     Moves m;
     const size_t row = (size_t)c->cfg.max_pages_per_seq;
-    for (int32_t b = 0; b < B; ++b) {
-        const int64_t n = lengths ? lengths[b] : c->h_seq_lens[src[b]], full = n / P;
-        m.entries.reserve(m.entries.size() + (size_t)full + 1);
-    }
-    m.units.reserve((size_t)B);
-    m.pages.reserve((size_t)B * 2);
+    size_t n_entries = 0;
+    for (int32_t b = 0; b < B; ++b)
+        n_entries += (size_t)pages_for(c, lengths ? lengths[b] : c->h_seq_lens[src[b]]);
+    m.entries.reserve(n_entries);
+    m.units.reserve((size_t)need);
+    m.pages.reserve((size_t)need * 2);
+    if (int rc = m.ready(c)) return rc;
     // nothing above changed the cache; nothing below can fail before the launch
     for (int32_t b = 0; b < B; ++b) {
         const int64_t n = lengths ? lengths[b] : c->h_seq_lens[src[b]], full = n / P;
@@ -384,18 +390,21 @@ int compact_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *bas
     }
     const size_t row = (size_t)c->cfg.max_pages_per_seq;
     // every allocation the plan needs happens before the cache changes
-    size_t n_pages = 0, n_units = 0;
-    for (const Job &j : jobs) {
+    size_t n_pages = 0, n_units = 0, n_listed = 0, n_dropped = 0;
+    for (int32_t b = 0; b < B; ++b) {
+        const Job &j = jobs[(size_t)b];
         n_pages += (size_t)(j.p1 - j.p0);
-        n_units += (size_t)((j.end - j.p0 * P) / MOVE_ROWS + 2);
+        n_units += j.p0 >= j.p1 ? 0 : j.fresh ? (size_t)((j.end - j.p0 * P + MOVE_ROWS - 1) / MOVE_ROWS) : 1;
+        const size_t from_p0 = (size_t)(pages_for(c, c->h_seq_lens[seq[b]]) - j.p0);
+        n_dropped += from_p0;
+        n_listed += j.p0 < j.p1 ? from_p0 + (size_t)(j.p1 - j.p0) : 0;
     }
     std::vector<int32_t> dropped;
-    size_t old_pages = 0;
-    for (int32_t b = 0; b < B; ++b) old_pages += (size_t)pages_for(c, c->h_seq_lens[seq[b]]);
     m.units.reserve(n_units);
     m.entries.reserve(n_pages);
-    m.pages.reserve(old_pages + n_pages);
-    dropped.reserve(old_pages);
+    m.pages.reserve(n_listed);
+    dropped.reserve(n_dropped);
+    if (int rc = m.ready(c)) return rc;
     bool any_kept = false;
     for (int32_t b = 0; b < B; ++b) {
         const Job &j = jobs[(size_t)b];
@@ -502,6 +511,7 @@ int put_rows_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *n,
     for (int32_t b = 0; b < B; ++b) tiles += (n[b] + ROW_TILE - 1) / ROW_TILE;
     if (tiles * ((c->g.n_kv + ROW_HEADS - 1) / ROW_HEADS) > INT32_MAX)
         return fail(INS_EBADLEN, "too many rows in one call");
+    if (int rc = Plan::ready(c, std::max((size_t)need * sizeof(int2), (size_t)B * sizeof(RowSpan)) + 64)) return rc;
     tiles = total = 0;
     const size_t row = (size_t)c->cfg.max_pages_per_seq;
     for (int32_t b = 0; b < B; ++b) {

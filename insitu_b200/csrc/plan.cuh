@@ -31,12 +31,18 @@ class Plan {
     template <typename T>
     size_t add(const T *v, size_t n) {
         const size_t at = (size_ + alignof(T) - 1) / alignof(T) * alignof(T);
-        parts_.push_back(Part{at, v, n * sizeof(T)});
+        parts_[n_++] = Part{at, v, n * sizeof(T)};
         size_ = at + n * sizeof(T);
         return at;
     }
     template <typename T>
     size_t add(const std::vector<T> &v) { return add(v.data(), v.size()); }
+
+    // Makes sure that run() will find its upload buffers for a plan of up to
+    // `bytes`: run() then fails only where the device does.
+    static int ready(CacheBase *c, size_t bytes) {
+        return bytes > (size_t)PARAM_UPLOAD_MAX ? c->stage_p.grow(bytes) : INS_OK;
+    }
 
     // Calls `launch(src)` with the plan as PlanInline<512>, PlanInline<3840>
     // or PlanPtr; launch returns a cudaError_t.
@@ -58,8 +64,8 @@ class Plan {
         size_t bytes;
     };
     void write(uint8_t *to) const {
-        for (const Part &p : parts_)
-            if (p.bytes) std::memcpy(to + p.at, p.from, p.bytes);
+        for (int i = 0; i < n_; ++i)
+            if (parts_[i].bytes) std::memcpy(to + parts_[i].at, parts_[i].from, parts_[i].bytes);
     }
     template <int N, typename F>
     int inlined(F &&launch) const {
@@ -68,7 +74,8 @@ class Plan {
         CK(launch(p));
         return INS_OK;
     }
-    std::vector<Part> parts_;
+    Part parts_[4];                          // as many as any plan has
+    int n_ = 0;
     size_t size_ = 0;
 };
 
