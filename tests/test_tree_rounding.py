@@ -168,6 +168,27 @@ def test_queries_of_all_32_bits(nodes, norm_frac, qk_frac):
     run(4, 2, 4, 300, nodes, large, 2.0 ** 29, seed=nodes, norm_frac=norm_frac, qk_frac=qk_frac)
 
 
+def near_one(rng, shape):
+    return np.clip(np.rint(512 + 60 * rng.standard_normal(shape)), 1, 32767)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kb,vb", [(4, 2), (3, 3), (3, 2)])
+@pytest.mark.parametrize("nodes", [1, 3, 6, 12, 24, 64])
+@pytest.mark.parametrize("scale", [0.0, 0.25, 4.0, 60.0])
+def test_scores_of_every_size(kb, vb, nodes, scale):
+    """From the plain mean to one token that takes all the weight, maxima
+    rising late and often; the widths that a cache has by default among them."""
+    run(kb, vb, 4, 3000, nodes, near_one, scale * 65536, seed=nodes)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nodes", [1, 3, 6, 12, 24, 64])
+@pytest.mark.parametrize("groups", [1, 8])
+def test_norms_of_either_sign_and_every_size(nodes, groups):
+    run(4, 2, groups, 700, nodes, large, 0.01 * 65536, seed=nodes)
+
+
 @pytest.mark.gpu
 def test_formats_that_the_products_do_not_cover_are_refused():
     from insitu_b200 import DraftTree
