@@ -97,8 +97,10 @@ class AttentionLayer:
     def forward(self, x, positions=None):
         """Rows of x are decode tokens, in order (a prefill when there are
         several). Returns y (tokens, hidden) fp32 on the device and the
-        attention output (tokens, num_heads * head_dim) int64 Q(acc_frac)."""
+        attention output (tokens, num_heads * head_dim) int64 Q(acc_frac).
+        Nodes of a ``verify`` that no ``accept`` kept are dropped first."""
         pc = self.dec.pc
+        self._drop_drafted()
         x = torch.as_tensor(x).to(pc.device, torch.float32)
         if x.ndim == 1:
             x = x[None]
@@ -126,6 +128,15 @@ class AttentionLayer:
         return y, merged
 
     # -- drafted trees -----------------------------------------------------------
+    def _drop_drafted(self):
+        """Drops the rows of a verify that no accept has followed, while they
+        are the cache's last ones."""
+        if self._drafted is None:
+            return
+        (T, n), self._drafted = self._drafted, None
+        if self.dec.pc.length(self.seq) == T + n:
+            self.dec.pc.truncate([self.seq], [T])
+
     def _qkv_wire(self, x, positions):
         """Projections and the seam of x's rows: the wire q, k, v on the device."""
         n = x.shape[0]
@@ -139,7 +150,8 @@ class AttentionLayer:
         position is its depth after the context, and it attends the context
         and its ancestors (``tree_scan``, the floating-point form of the
         cache's attention). The nodes' rows stay cached until ``accept`` says
-        which of them to keep. Returns y (nodes, hidden) fp32 and the
+        which of them to keep; the next ``verify`` or ``forward`` without it
+        keeps none. Returns y (nodes, hidden) fp32 and the
         attention output (nodes, num_heads, head_dim) bf16."""
         pc = self.dec.pc
         if len(tree.counts) != 1 or tree.depths is None:
@@ -148,6 +160,7 @@ class AttentionLayer:
         n = x.shape[0]
         if n != tree.counts[0]:
             raise ValueError(f"{n} inputs for a tree of {tree.counts[0]} nodes")
+        self._drop_drafted()
         T = pc.length(self.seq)
         wq, wk, wv, conv = self._qkv_wire(x, T + tree.depths - 1)
         self.last_wire, self._last_conv = (wq, wk, wv), conv

@@ -66,3 +66,29 @@ def test_a_wait_for_rows_that_runs_out_is_reported_and_the_context_survives(node
         assert torch.equal(pc.tree_scan([0], q, tree).view(torch.int16), want.view(torch.int16))
         pc.status()
     pc.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("then", ["forward", "verify"])
+def test_drafted_nodes_that_no_accept_kept_are_not_context(then):
+    """A verify whose nodes all fell, then the next step without an accept of
+    nothing: the siblings' rows are no tokens of the sequence."""
+    from insitu_b200 import DraftTree
+    from test_tree_layer import make_layer
+    rng = np.random.default_rng(8)
+    xs, drafted, x = (rng.standard_normal((n, 256)).astype(np.float32) for n in (40, 5, 1))
+    layer, plain = make_layer(), make_layer()
+    for m in (layer, plain):
+        m.forward(xs)
+    layer.verify(drafted, DraftTree([[-1, 0, 0, -1, 3]]))
+    if then == "forward":
+        got, want = layer.forward(x)[0], plain.forward(x)[0]
+    else:
+        one = DraftTree([[-1]])
+        got, want = layer.verify(x, one)[0], plain.verify(x, one)[0]
+        layer.accept([0])
+        plain.accept([0])
+    assert layer.dec.pc.length(0) == 41
+    assert torch.equal(got, want) and torch.equal(layer.dec.pc.rows([0]), plain.dec.pc.rows([0]))
+    layer.close()
+    plain.close()
