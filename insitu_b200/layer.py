@@ -166,8 +166,9 @@ class AttentionLayer:
         self.last_wire, self._last_conv = (wq, wk, wv), conv
         self._conv_n += conv[:2]
         torch.maximum(self._conv_max, conv[2:].view(torch.float64), out=self._conv_max)
-        out = pc.tree_scan([self.seq], pc.ingress([self.seq] * n, wk, wv, wq), tree)
-        self._drafted = (T, n)
+        q_rot = pc.ingress([self.seq] * n, wk, wv, wq)
+        self._drafted = (T, n)             # (the rows are there, whatever the scan says)
+        out = pc.tree_scan([self.seq], q_rot, tree)
         return project(self.w_o, out.reshape(n, self.hq * self.d).to(torch.float32), self.b_o, rounded=True), out
 
     def accept(self, path) -> None:

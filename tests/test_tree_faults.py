@@ -92,3 +92,29 @@ def test_drafted_nodes_that_no_accept_kept_are_not_context(then):
     assert torch.equal(got, want) and torch.equal(layer.dec.pc.rows([0]), plain.dec.pc.rows([0]))
     layer.close()
     plain.close()
+
+
+@pytest.mark.gpu
+def test_a_verify_whose_scan_fails_leaves_no_rows_behind(monkeypatch):
+    """Its rows are appended before the scan: an error there (no memory for the
+    partial sums) must not make them context."""
+    from insitu_b200 import DraftTree
+    from test_tree_layer import make_layer
+    rng = np.random.default_rng(8)
+    xs, drafted, x = (rng.standard_normal((n, 256)).astype(np.float32) for n in (40, 5, 1))
+    layer, plain = make_layer(), make_layer()
+    for m in (layer, plain):
+        m.forward(xs)
+
+    def no_memory(*args):
+        raise torch.cuda.OutOfMemoryError("no memory")
+
+    monkeypatch.setattr(layer.dec.pc, "tree_scan", no_memory)
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        layer.verify(drafted, DraftTree([[-1, 0, 0, -1, 3]]))
+    monkeypatch.undo()
+    got, want = layer.forward(x)[0], plain.forward(x)[0]
+    assert layer.dec.pc.length(0) == 41
+    assert torch.equal(got, want) and torch.equal(layer.dec.pc.rows([0]), plain.dec.pc.rows([0]))
+    layer.close()
+    plain.close()
