@@ -112,15 +112,7 @@ class AttentionLayer:
             pos = positions            # stays on the device; the seam kernel checks it
         else:
             pos = np.asarray(positions, np.int64)
-        q, k, v = project(self.w_qkv, x, self.b_qkv, rounded=True).split(self._split, dim=1)
-        q = q.reshape(n, self.hq, self.d)
-        k = k.reshape(n, self.hk, self.d)
-        v = v.reshape(n, self.hk, self.d)
-        wq, wk, wv, conv = self.seam(q, k, v, pos, host_stats=False)
-        self.last_wire = (wq, wk, wv)
-        self._last_conv = conv
-        self._conv_n += conv[:2]
-        torch.maximum(self._conv_max, conv[2:].view(torch.float64), out=self._conv_max)
+        wq, wk, wv = self._qkv_wire(x, pos)
         out, self.last_stats = self.dec.prefill_attend(self.seq, wq, wk, wv, mode=self.softmax)
         merged = out.reshape(n, self.hq * self.d)
         acc = merged.to(torch.float64) / float(1 << self.fmt.qk_frac)      # Q.to_float
@@ -138,11 +130,17 @@ class AttentionLayer:
             self.dec.pc.truncate([self.seq], [T])
 
     def _qkv_wire(self, x, positions):
-        """Projections and the seam of x's rows: the wire q, k, v on the device."""
+        """Projections and the seam of x's rows: the wire q, k, v on the device.
+        Their conversion statistics join the layer's."""
         n = x.shape[0]
         q, k, v = project(self.w_qkv, x, self.b_qkv, rounded=True).split(self._split, dim=1)
-        return self.seam(q.reshape(n, self.hq, self.d), k.reshape(n, self.hk, self.d), v.reshape(n, self.hk, self.d),
-                         positions, host_stats=False)
+        wq, wk, wv, conv = self.seam(q.reshape(n, self.hq, self.d), k.reshape(n, self.hk, self.d),
+                                     v.reshape(n, self.hk, self.d), positions, host_stats=False)
+        self.last_wire = (wq, wk, wv)
+        self._last_conv = conv
+        self._conv_n += conv[:2]
+        torch.maximum(self._conv_max, conv[2:].view(torch.float64), out=self._conv_max)
+        return wq, wk, wv
 
     def verify(self, x, tree):
         """The nodes of a drafted tree (an ``insitu_b200.tree.DraftTree`` of one
@@ -162,10 +160,7 @@ class AttentionLayer:
             raise ValueError(f"{n} inputs for a tree of {tree.counts[0]} nodes")
         self._drop_drafted()
         T = pc.length(self.seq)
-        wq, wk, wv, conv = self._qkv_wire(x, T + tree.depths - 1)
-        self.last_wire, self._last_conv = (wq, wk, wv), conv
-        self._conv_n += conv[:2]
-        torch.maximum(self._conv_max, conv[2:].view(torch.float64), out=self._conv_max)
+        wq, wk, wv = self._qkv_wire(x, T + tree.depths - 1)
         q_rot = pc.ingress([self.seq] * n, wk, wv, wq)
         self._drafted = (T, n)             # (the rows are there, whatever the scan says)
         out = pc.tree_scan([self.seq], q_rot, tree)
