@@ -148,7 +148,8 @@ int ins_cache_set_scan_kernel(ins_cache *cache, int32_t mode);
 /* A test of the scans' failure path, with no reference counterpart and no
  * use outside tests: every bounded wait of the online scan's look-back (fused
  * kernel) and of its value pass's staged rows (separate launches) gives up
- * after `poll_limit` polls (default 2^22, about a second), and tile `chunk`
+ * after `poll_limit` polls (default 2^22, about a second of the look-back's
+ * and some 17 of those for staged rows, 4 us each), and tile `chunk`
  * of item `item` (sequence b, KV head h: item b * n_kv + h, in the order of
  * the scan's seq_ids) is held back: with the fused kernel the word it
  * publishes for query head `head` is withheld, so the tiles after it wait

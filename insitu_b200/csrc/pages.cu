@@ -5,8 +5,8 @@
 // freeing pages costs no device work; what the device does is move rows.
 // A row of one KV head is three pieces in its region's planes (K codes, V
 // codes, norms), 52 bytes at 4b/2b: every kernel here reads and writes each
-// moved row once, and is bound by those bytes or, at a few rows, by its one
-// launch.
+// moved row once, and takes its one launch's time at a few rows, and at many
+// the instructions that address pieces of 8 bytes.
 #include <algorithm>
 
 #include "plan.cuh"
@@ -33,8 +33,10 @@ constexpr int MOVE_THREADS = 256;
 // sources rise faster than destinations (source(d) >= d), so a row that a
 // chunk writes is no later chunk's source, and pages may be compacted in
 // place. Units that run side by side never write a page another one reads.
-// Bound by the rows' bytes: 65,536 kept rows of 131,072 into pages of their
-// own (8 heads, 4b/2b) read and write 54 MB in 24 us, 2.3 TB/s.
+// 65,536 kept rows of 131,072 into pages of their own (8 heads, 4b/2b) read and
+// write 54 MB in 24 us, 2.3 TB/s: a third of what the memory does, which is 26 %
+// busy, as the issue slots are 63 %: each 8 bytes take a division and a 64-bit
+// address. In place the chunks follow one another: 3.4 ms.
 template <class Src>
 __global__ void __launch_bounds__(MOVE_THREADS) k_move_rows(Geo g, uint8_t *__restrict__ pool,
                                                             int32_t *__restrict__ table, uint32_t kept_at,
@@ -122,9 +124,10 @@ constexpr int ROW_TILE = 32, ROW_HEADS = 8;
 // written) plane by plane, 8 bytes a thread; the caller's buffer
 // ([rows][n_kv][row_bytes], the packed rows of CompressedCache.buf,
 // cache/compressed.py:42-52) row by row, so both sides are contiguous runs;
-// shared memory holds the tile in the buffer's order. Bound by the bytes:
-// 65,536 rows of 8 heads (4b/2b) out take 30 us, 131,072 in 51 us, 1.8 and
-// 2.1 TB/s of reads and writes.
+// shared memory holds the tile in the buffer's order. 65,536 rows of 8 heads
+// (4b/2b) out take 30 us, 131,072 in 51 us, 1.8 and 2.1 TB/s of reads and
+// writes: bound by instructions (66 % of the issue slots; the divisions that
+// find a piece's row and head), as the pool's and the buffer's orders differ.
 template <bool PUT, class Src>
 __global__ void __launch_bounds__(256) k_copy_rows(Geo g, uint8_t *__restrict__ pool,
                                                    const int32_t *__restrict__ table, uint8_t *__restrict__ buf,

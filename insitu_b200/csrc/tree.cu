@@ -180,8 +180,9 @@ __device__ __forceinline__ int find_seq(const TreeSeq *seqs, int n, int i) {
 // P^T changes from a result's layout to an operand's by two 8 x 8 transposes.
 //
 // Bound by instructions: of the 16 tokens' 2,048 codes a warp's step makes 32
-// table addresses and 24 loads, and some 200 instructions in all. One token
-// of 1,048,576 (8 KV heads of 4 query heads, 4b/2b) takes 151 us: 2.9 TB/s of
+// table addresses and 24 loads, and some 190 instructions in all (other code
+// widths decode a code at a time: 3b/2b 641 us where 4b/2b takes 139). One token
+// of 1,048,576 (8 KV heads of 4 query heads, 4b/2b) takes 139 us: 3.1 TB/s of
 // the 436 MB of codes and norms. With the products the other way round,
 // 4-byte value entries and 16 warps of 128 registers it took 198 us.
 
@@ -692,8 +693,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_tree_few(Geo g, TreeArgs a, cons
 // parts are joined by k_tree_join: at most two partial slots a CTA.
 //
 // 64 nodes on each of 16 sequences of 32,768 tokens (8 KV heads of 4 query
-// heads: 256 rows an item, 275 GFLOP) take 434 us, 0.63 PFLOP/s: 239 us of it
-// are the exponentials (XU pipe 63 % busy), the rest the waits of a stream
+// heads: 256 rows an item, 275 GFLOP) take 416 us, 0.66 PFLOP/s: 239 us of it
+// are the exponentials (XU pipe 66 % busy), the rest the waits of a stream
 // whose next scores are not there yet. A third score buffer would fill them,
 // but tensor memory has no columns left.
 
@@ -1453,10 +1454,11 @@ namespace {
 // to do, as its start costs more (fewer units of work, tensor memory, the
 // join of 128-row slots) and its tiles less. Measured, 8 KV heads of 4 query
 // heads, 4b/2b, k_tree_few against k_tree_many: 9 nodes (36 rows) of one
-// sequence, 2,304 tokens (1 tile an SM) 21.8 : 22.8 us, 18,800 (8) 27.3 : 31.5,
-// 65,536 (28) 55.1 : 55.0, 131,072 (55) 92.5 : 88.2, 16 sequences of 32,768
-// (222) 375 : 295; 16 nodes (64 rows) 27.4 : 32.3, 55.0 : 56.4, 92.5 : 89.3,
-// 384 : 298; 3b/3b, 6 sequences to 9,001 tokens (about 20) 45.5 : 41.7. Above
+// sequence, 2,304 tokens (1 tile an SM) 22.0 : 21.7 us, 18,800 (8) 27.1 : 28.8,
+// 65,536 (28) 53.0 : 51.2, 131,072 (55) 88.1 : 83.3, 16 sequences of 32,768
+// (222) 365 : 280; 16 nodes (64 rows) 20.3 : 18.1, 27.1 : 29.6, 52.9 : 52.1,
+// 88.5 : 84.4, 376 : 287; 3b/3b, 6 sequences to 9,001 tokens (about 20), 16
+// nodes 45.4 : 37.0. Above
 // 64 rows k_tree_few decodes each row three times and more.
 constexpr int MANY_FROM = 32, MANY_SURE = 64, MANY_TILES = 12;
 // Its keys (centroid times norm, below 2^4 times 2^6) can take a factor of up
@@ -1505,8 +1507,8 @@ int make_plan(const CacheBase *c, int32_t B, const int32_t *seq, const int32_t *
     if (paired && (most > MANY_SURE || (most > MANY_FROM && kv_tiles > (int64_t)MANY_TILES * sms))) {
         p.many = true;
         // 256-row tiles share each decoded row between both streams: above 128
-        // rows 128 : 166 us with 128-row tiles (64 nodes, 131,072 tokens); with
-        // 128 rows or fewer one stream would idle, 93 : 110 us (32 nodes)
+        // rows 122 us, with 128-row tiles 154 (64 nodes, 131,072 tokens); with
+        // 128 rows or fewer one stream would idle, 88 : 105 us (32 nodes)
         p.rows = most > 128 ? 256 : 128;
         for (TreeSeq &s : p.seqs) {
             const int64_t rts = ((int64_t)s.nodes * g.H + p.rows - 1) / p.rows;
@@ -1530,7 +1532,7 @@ int make_plan(const CacheBase *c, int32_t B, const int32_t *seq, const int32_t *
     }
     // Rows a tile: two 16-row fragments share each decoded token where there
     // are more than 16 rows. At 16 rows (4 nodes, 131,072 tokens) one fragment
-    // takes 41.9 us, two 55.8; at 17 to 32 one fragment would decode twice.
+    // takes 38.9 us, two 54.0; at 17 to 32 one fragment would decode twice.
     p.rows = most > 16 ? 32 : 16;
     auto units_at = [&](int64_t chunk) {
         int64_t u = 0;
@@ -1592,9 +1594,9 @@ int launch_few(CacheBase *c, const TreePlan &p, const Plan &plan, const TreeArgs
 template <int KB, int VB>
 int launch_few_rows(CacheBase *c, const TreePlan &p, bool half, const Plan &plan, const TreeArgs &a, cudaStream_t s) {
     // Warps: five a scheduler where 96 registers hold their state (1 token of
-    // 1M rows: 20 warps 151 us, 23 warps of 80 registers 153; 3b/3b 195, 209),
-    // three where 32 rows take 168 (8 nodes of 1M: 12 warps 317 us, 14 spill:
-    // 540). 8-bit rows make a stage 8.4 KB: 8 warps of them fit.
+    // 1M rows: 20 warps 139 us, 23 warps of 80 registers 143; 3b/3b 200, 211),
+    // three where 32 rows take 168 (8 nodes of 1M: 12 warps 302 us, 14 spill:
+    // 468). 8-bit rows make a stage 8.4 KB: 8 warps of them fit.
     constexpr int N1 = KB ? 20 : 8, N2 = KB ? 12 : 8;
     if (p.rows == 32) return launch_few<KB, VB, 2, false, N2>(c, p, plan, a, s);
     if (half) return launch_few<KB, VB, 1, true, N1>(c, p, plan, a, s);
@@ -1659,7 +1661,7 @@ int tree_body(CacheBase *c, int32_t B, const int32_t *seq, const int32_t *nodes,
     Plan plan;
     plan.add(p.seqs);
     // up to 8 rows the products are taken transposed: one node of 1,048,576
-    // tokens 150 us, by the 16-row variant 195
+    // tokens 139 us, by the 16-row variant 185
     bool half = true;
     for (const TreeSeq &t : p.seqs) half &= t.nodes * c->g.H <= 8;
     const int kb = c->g.kb, vb = c->g.vb;
