@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
 #include <vector>
@@ -244,8 +245,8 @@ at::Tensor tree_scan(int64_t h, at::IntArrayRef seq_ids, at::IntArrayRef nodes, 
     c10::cuda::CUDAGuard guard(q.device());
     used_here(mask);
     const std::vector<int32_t> s = ids32(seq_ids), n = ids32(nodes);
-    const int64_t bytes = ins_tree_workspace(handle(h), n_ids(seq_ids), s.data(), n.data());
-    if (bytes < 0) check(INS_EINVAL);
+    // (what refuses the size refuses the scan too, which says why by its status)
+    const int64_t bytes = std::max<int64_t>(0, ins_tree_workspace(handle(h), n_ids(seq_ids), s.data(), n.data()));
     at::Tensor out = at::empty(q.sizes(), q.options().dtype(at::kBFloat16));
     at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
     check(ins_tree_scan(handle(h), n_ids(seq_ids), s.data(), n.data(),

@@ -118,3 +118,20 @@ def test_a_verify_whose_scan_fails_leaves_no_rows_behind(monkeypatch):
     assert torch.equal(got, want) and torch.equal(layer.dec.pc.rows([0]), plain.dec.pc.rows([0]))
     layer.close()
     plain.close()
+
+
+@pytest.mark.gpu
+def test_a_refusal_has_its_own_error():
+    """A tree of more nodes than the sequence has rows is a matter of length,
+    as the scans' lengths are; a sequence that is not there is an argument."""
+    from insitu_b200 import DraftTree
+    from insitu_b200._lib import ArgumentError, CapacityError
+    pc = make(4, 2, 2, 4, 16, 64, 2)
+    pc.put_rows([0], [2], torch.zeros((2, 2, 52), dtype=torch.uint8, device=pc.device))
+    q = torch.zeros((3, 8, 64), dtype=torch.int32, device=pc.device)
+    tree = DraftTree([[-1, 0, 1]])
+    with pytest.raises(CapacityError, match="fewer than its tree"):
+        pc.tree_scan([0], q, tree)
+    with pytest.raises(ArgumentError, match="out of range"):
+        pc.tree_scan([5], q, tree)
+    pc.close()
