@@ -148,8 +148,8 @@ int ins_cache_set_scan_kernel(ins_cache *cache, int32_t mode);
 /* A test of the scans' failure path, with no reference counterpart and no
  * use outside tests: every bounded wait of the online scan's look-back (fused
  * kernel) and of its value pass's staged rows (separate launches) gives up
- * after `poll_limit` polls (default 2^22, about a second of the look-back's
- * and some 17 of those for staged rows, 4 us each), and tile `chunk`
+ * after `poll_limit` polls (default 2^22, of which waits for copies take at
+ * most 2^18, about a second), and tile `chunk`
  * of item `item` (sequence b, KV head h: item b * n_kv + h, in the order of
  * the scan's seq_ids) is held back: with the fused kernel the word it
  * publishes for query head `head` is withheld, so the tiles after it wait
@@ -158,7 +158,7 @@ int ins_cache_set_scan_kernel(ins_cache *cache, int32_t mode);
  * wait cannot complete. The waits give up, the launch still finishes, and
  * ins_cache_status returns INS_ETIMEOUT; no GPU fault is involved. item < 0
  * holds nothing back. ins_tree_scan's waits for its copies of cached rows take
- * the same limit, at most 2^18 polls (about a second); there `item` is a CTA of the launch and `chunk` the number,
+ * the same limit; there `item` is a CTA of the launch and `chunk` the number,
  * among the tiles of cached rows that this CTA reads, of the one whose copies
  * are announced 16 bytes larger. */
 int ins_cache_set_wait_test(ins_cache *cache, int32_t poll_limit, int32_t item, int32_t chunk,

@@ -18,6 +18,9 @@ namespace ins {
 constexpr int D = 64;                // head_dim this build supports
 constexpr int MAX_ROUNDS = 8;        // rotation rounds carried in the sign masks
 constexpr uint32_t FULL = 0xffffffffu;
+// Polls of a bounded wait on an mbarrier (4 us each where they find nothing):
+// about a second.
+constexpr int WAIT_POLLS = 1 << 18;
 
 // Device status bits, latched by kernels and read by ins_cache_status().
 enum : int32_t { ST_RANGE = 1, ST_TIMEOUT = 2, ST_INTERNAL = 4, ST_SPLIT = 8, ST_POSITION = 16 };

@@ -1315,8 +1315,9 @@ __device__ __forceinline__ void mbar_arrive_tx(uint64_t *bar, uint32_t bytes) {
                  ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
 }
 // Waits for phase `parity` of the barrier to complete; gives up (false) after
-// a bounded number of polls, each of which the hardware may suspend briefly.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, int limit = 1 << 22) {
+// a bounded number of polls, each of which the hardware suspends: one that
+// finds nothing lasts 4 us.
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, int limit = WAIT_POLLS) {
     const uint32_t addr = smem_addr(bar);
     for (int it = 0; it < limit; ++it) {
         uint32_t done;
@@ -2670,7 +2671,7 @@ inline int prepare_chunked(ChunkScratch &cs, const Geo &g, const DevTables *tb, 
     a.status = d_status;
     a.item_done = cs.idone;
     a.scan_done = cs.sdone;
-    a.poll_limit = cs.poll_limit;
+    a.poll_limit = std::min(cs.poll_limit, WAIT_POLLS);
     a.hold_rec = cs.hold_item < 0 || cs.hold_item >= n_items || cs.hold_chunk >= cs.max_chunks
                      ? -1
                      : (int64_t)cs.hold_item * cs.max_chunks + cs.hold_chunk;

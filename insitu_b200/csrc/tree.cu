@@ -73,8 +73,6 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 // Orders this thread's ordinary accesses to shared memory before later ones by
 // copies and tensor cores (once a barrier has passed).
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// Polls of a bounded wait: one that finds nothing lasts 4 us, so about a second.
-constexpr int WAIT_POLLS = 1 << 18;
 // Waits for the phase of `parity`, at most `limit` polls; false: it gave up
 // (this thread did: a warp has to agree before it goes on).
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int limit) {
