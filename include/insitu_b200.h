@@ -479,8 +479,37 @@ int ins_tree_scan(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int
                   const uint64_t *mask, int32_t words, const int32_t *q_rot, void *out,
                   void *workspace, int64_t workspace_bytes, void *stream);
 
-/* Element types of ins_sample's logits. */
+/* Attention of chunks of new tokens, in floating point: the causal form of
+ * ins_tree_scan (the reference scans causal prefixes in integers,
+ * ops/attention.py:517-871, which ins_scan does for a chunk). Sequence
+ * seq_ids[i]'s last counts[i] cached tokens (0 up to all; already appended by
+ * an ingress) are a chunk; each attends itself and the tokens before it, under
+ * a window (window > 0; 0: none) only those of the last `window` positions,
+ * its own among them, and the sequence's first `sinks` tokens. A position is a
+ * row's place in the cache. Outputs, numerics, buffers and their alignment are
+ * ins_tree_scan's; q_rot and out hold sum counts tokens, workspace
+ * ins_chunk_workspace bytes for the same cache and arguments (the lengths at
+ * the call). Sequences of up to 2^30 tokens; the same sequence may be named
+ * several times. Stream-ordered; a bounded wait that gives up latches
+ * INS_ETIMEOUT for ins_cache_status. */
+int64_t ins_chunk_workspace(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int32_t *counts,
+                            int32_t window, int32_t sinks);
+int ins_chunk_scan(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int32_t *counts,
+                   int32_t window, int32_t sinks, const int32_t *q_rot, void *out, void *workspace,
+                   int64_t workspace_bytes, void *stream);
+
+/* Element types of logits, and of keys and values in floating point. */
 enum { INS_F32 = 0, INS_F16 = 1, INS_BF16 = 2 };
+
+/* Rows [t0[i], t0[i] + n[i]) of seq_ids[i], one sequence after another, as
+ * keys and values in real units: k and v, device, [sum n][n_kv][d] of `dtype`,
+ * 16-byte aligned. rotated != 0: as the cache holds them, norm *
+ * centroid[code] (the basis of q_rot and of the scans' outputs); 0: turned
+ * back by the rotation's inverse, the model's own keys (after RoPE) and
+ * values. Sums are fp32, rounded once to dtype (float16 overflows to infinity
+ * above 65,504). */
+int ins_cache_dense(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int64_t *t0,
+                    const int64_t *n, void *k, void *v, int32_t dtype, int32_t rotated, void *stream);
 
 /* One sampled token per row of logits (no reference counterpart: its driver
  * takes the argmax on the host). With z_i = x_i / temperature and w_i =
@@ -505,6 +534,40 @@ int ins_sample(int32_t rows, int32_t vocab, const void *logits, int32_t dtype, i
                const float *uniform, int64_t uniform_stride, const float *temperature,
                const int32_t *top_k, const float *top_p, const float *min_p, int64_t *tokens,
                float *logprobs, void *stream);
+
+/* Penalties, bias and mask on rows of logits, before a draw. Row i's tokens
+ * so far are the first lengths[h] of the tokens' row h = of[i] (i where `of` is
+ * NULL), of which the first prompts[h] were asked and the others said, and its
+ * n_drafted drafted ones, said. With c how often a token has been said,
+ *   y = (asked or said) ? (x > 0 ? x / repetition : x * repetition) : x
+ *   y = y - frequency * c - presence * (c > 0) + bias
+ * and -inf where the mask's bit of the token is 0 (bit t % 32 of word t / 32),
+ * computed in fp32 and rounded once. Entries outside [0, vocab) are no tokens;
+ * an `of` outside [0, histories) names no tokens. Each pointer may be NULL (no
+ * tokens; every column of `tokens`; no prompt; 1, 0, 0; none). All buffers are
+ * on the device. */
+typedef struct ins_penalties {
+    const int64_t *tokens;                     /* [histories] rows of `history`, tokens_stride apart */
+    int64_t tokens_stride;
+    int32_t history, histories;
+    const int32_t *lengths, *prompts;          /* [histories] */
+    const int32_t *of;                         /* [rows] */
+    const int64_t *drafted;                    /* [rows] rows of n_drafted, drafted_stride apart */
+    int64_t drafted_stride;
+    const float *repetition, *presence, *frequency;   /* [rows] */
+    const float *bias;                         /* rows of vocab, bias_stride apart (0: one for all) */
+    int64_t bias_stride;
+    const int32_t *mask;                       /* rows of (vocab + 31) / 32 words, mask_stride apart (0: one) */
+    int64_t mask_stride;
+    int32_t n_drafted, reserved0;
+} ins_penalties;
+
+/* out (rows of vocab elements, out_stride >= vocab apart) is the changed
+ * logits, of their type; it may be the logits themselves (the same pointer and
+ * stride), and may not overlap them otherwise. vocab in [1, 262144]; stride as
+ * in ins_sample. Runs on the device of the current context, stream-ordered. */
+int ins_penalize(int32_t rows, int32_t vocab, const void *logits, int32_t dtype, int64_t stride, void *out,
+                 int64_t out_stride, const ins_penalties *penalties, void *stream);
 
 /* The last error message recorded on this thread ("" if none). */
 const char *ins_last_error(void);

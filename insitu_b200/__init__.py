@@ -17,6 +17,9 @@ and adds what a serving loop needs next to them:
 
     DraftTree           trees of drafted tokens, attended by PagedCache.tree_scan
     Sampler             tokens from logits: temperature, top-k, top-p, min-p
+    Penalties           penalties of the tokens so far, biases and masks on logits
+    (PagedCache)        chunk_scan: causal attention of chunks of new tokens,
+                        under a window and sinks; dense: rows read back
     (PagedCache)        fork, compact, truncate, rows, put_rows: page operations
 """
 
@@ -24,7 +27,7 @@ from .config import FixedFormat, Geometry, QuantConfig
 
 __all__ = ["FixedFormat", "Geometry", "QuantConfig", "Rotation", "KVQuantizer", "CompressedKV",
            "KVCache", "CompressedCache", "CompressedAttention", "AttentionStats",
-           "DecodeAttention", "PagedCache", "AttentionLayer", "DraftTree", "Sampler"]
+           "DecodeAttention", "PagedCache", "AttentionLayer", "DraftTree", "Sampler", "Penalties"]
 
 
 def __getattr__(name):
@@ -54,6 +57,9 @@ def __getattr__(name):
     if name == "Sampler":
         from .sampling import Sampler
         return Sampler
+    if name == "Penalties":
+        from .penalties import Penalties
+        return Penalties
     if name == "PagedCache":
         from .engine import PagedCache
         return PagedCache

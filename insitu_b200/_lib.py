@@ -21,8 +21,11 @@ UNITS = {
     "csrc/insitu.cu": COMMON + ("csrc/kernels.cuh", "csrc/scan_chunked.cuh", "csrc/scan_fused.cuh",
                                 "csrc/project.cuh"),
     "csrc/pages.cu": COMMON + ("csrc/plan.cuh",),
+    "csrc/chunk.cu": COMMON + ("csrc/plan.cuh", "csrc/attend.cuh"),
+    "csrc/dense.cu": COMMON + ("csrc/plan.cuh",),
+    "csrc/penalize.cu": COMMON,
     "csrc/sample.cu": COMMON,
-    "csrc/tree.cu": COMMON + ("csrc/plan.cuh",),
+    "csrc/tree.cu": COMMON + ("csrc/plan.cuh", "csrc/attend.cuh"),
 }
 SOURCES = tuple(dict.fromkeys(s for unit, headers in UNITS.items() for s in (unit, *headers)))
 HEADER = os.path.join(ROOT, "include", "insitu_b200.h")
@@ -99,6 +102,17 @@ class SeamCfg(C.Structure):
                 ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("rope_frac", C.c_int32),
                 ("max_position", C.c_int32)]
 
+
+class PenaltiesArgs(C.Structure):
+    """ins_penalties."""
+    _fields_ = [("tokens", C.c_void_p), ("tokens_stride", C.c_int64), ("history", C.c_int32),
+                ("histories", C.c_int32), ("lengths", C.c_void_p), ("prompts", C.c_void_p), ("of", C.c_void_p),
+                ("drafted", C.c_void_p), ("drafted_stride", C.c_int64), ("repetition", C.c_void_p),
+                ("presence", C.c_void_p), ("frequency", C.c_void_p), ("bias", C.c_void_p),
+                ("bias_stride", C.c_int64), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
+                ("n_drafted", C.c_int32), ("reserved0", C.c_int32)]
+
+
 # every symbol the header declares, for the load check
 SYMBOLS = ("ins_abi_version", "ins_bytes_per_token", "ins_cache_create", "ins_cache_destroy",
            "ins_cache_reset", "ins_cache_length", "ins_cache_capacity", "ins_ingress", "ins_rotate",
@@ -111,7 +125,8 @@ SYMBOLS = ("ins_abi_version", "ins_bytes_per_token", "ins_cache_create", "ins_ca
            "ins_scan_recomputed_total", "ins_cache_set_scan_kernel", "ins_cache_set_wait_test",
            "ins_project", "ins_cache_free_pages", "ins_cache_fork", "ins_cache_compact",
            "ins_cache_truncate", "ins_cache_rows", "ins_cache_put_rows", "ins_sample",
-           "ins_tree_workspace", "ins_tree_scan")
+           "ins_tree_workspace", "ins_tree_scan", "ins_chunk_workspace", "ins_chunk_scan",
+           "ins_cache_dense", "ins_penalize")
 
 
 def nvcc() -> str:
@@ -275,6 +290,11 @@ def lib():
     L.ins_tree_workspace.argtypes = [vp, i32, vp, vp]
     L.ins_tree_workspace.restype = i64
     L.ins_tree_scan.argtypes = [vp, i32, vp, vp, vp, i32, vp, vp, vp, i64, vp]
+    L.ins_chunk_workspace.argtypes = [vp, i32, vp, vp, i32, i32]
+    L.ins_chunk_workspace.restype = i64
+    L.ins_chunk_scan.argtypes = [vp, i32, vp, vp, i32, i32, vp, vp, vp, i64, vp]
+    L.ins_cache_dense.argtypes = [vp, i32, vp, vp, vp, vp, vp, i32, i32, vp]
+    L.ins_penalize.argtypes = [i32, i32, vp, i32, i64, vp, i64, C.POINTER(PenaltiesArgs), vp]
     L.ins_last_error.restype = C.c_char_p
     _lib = L
     return L

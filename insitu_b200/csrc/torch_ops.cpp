@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/insitu_b200.h"
@@ -256,6 +257,151 @@ at::Tensor tree_scan(int64_t h, at::IntArrayRef seq_ids, at::IntArrayRef nodes, 
     return out;
 }
 
+// ins_chunk_scan: attention of each sequence's last counts[i] cached tokens,
+// causal, under a window and sinks (window 0: none); q (sum counts, q_heads,
+// 64) int32 -> the same shape in bf16.
+at::Tensor chunk_scan(int64_t h, at::IntArrayRef seq_ids, at::IntArrayRef counts, int64_t window, int64_t sinks,
+                      const at::Tensor &q, int64_t q_heads) {
+    check_i32(q, "q", q_heads, 64);
+    TORCH_CHECK_VALUE(counts.size() == seq_ids.size(), "insitu: seq_ids and counts disagree on their number");
+    int64_t total = 0;
+    for (const int64_t n : counts) {
+        TORCH_CHECK_VALUE(n >= 0 && n <= INT32_MAX, "insitu: a token count out of range");
+        total += n;
+    }
+    TORCH_CHECK_VALUE(q.size(0) == total, "insitu: q must hold ", total, " tokens, got ", q.size(0));
+    TORCH_CHECK_VALUE(window >= 0 && window <= INT32_MAX && sinks >= 0 && sinks <= INT32_MAX,
+                      "insitu: a window or a number of sinks out of range");
+    c10::cuda::CUDAGuard guard(q.device());
+    const std::vector<int32_t> s = ids32(seq_ids), n = ids32(counts);
+    // (what refuses the size refuses the scan too, which says why by its status)
+    const int64_t bytes = std::max<int64_t>(
+        0, ins_chunk_workspace(handle(h), n_ids(seq_ids), s.data(), n.data(), (int32_t)window, (int32_t)sinks));
+    at::Tensor out = at::empty(q.sizes(), q.options().dtype(at::kBFloat16));
+    at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+    check(ins_chunk_scan(handle(h), n_ids(seq_ids), s.data(), n.data(), (int32_t)window, (int32_t)sinks,
+                         q.data_ptr<int32_t>(), out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
+                         at::cuda::getCurrentCUDAStream().stream()));
+    return out;
+}
+
+int32_t element_type(at::ScalarType st) {
+    TORCH_CHECK_VALUE(st == at::kFloat || st == at::kHalf || st == at::kBFloat16,
+                      "insitu: the type must be float32, float16 or bfloat16, got ", st);
+    return st == at::kFloat ? INS_F32 : st == at::kHalf ? INS_F16 : INS_BF16;
+}
+
+// ins_cache_dense into new (sum n, n_kv, 64) tensors k and v of `type`'s type.
+std::tuple<at::Tensor, at::Tensor> dense(int64_t h, const at::Tensor &anchor, at::IntArrayRef seq_ids,
+                                         at::IntArrayRef t0, at::IntArrayRef n, int64_t n_kv, at::ScalarType type,
+                                         bool rotated) {
+    c10::cuda::CUDAGuard guard(anchor.device());
+    TORCH_CHECK_VALUE(t0.size() == seq_ids.size() && n.size() == seq_ids.size(),
+                      "insitu: seq_ids, t0 and n disagree on their number");
+    const int32_t dtype = element_type(type);
+    int64_t total = 0;
+    for (const int64_t x : n) {
+        TORCH_CHECK_VALUE(x >= 0 && x <= INT32_MAX, "insitu: a row count out of range");
+        total += x;
+    }
+    at::Tensor k = at::empty({total, n_kv, 64}, anchor.options().dtype(type)), v = at::empty_like(k);
+    const std::vector<int32_t> s = ids32(seq_ids);
+    check(ins_cache_dense(handle(h), n_ids(seq_ids), s.data(), t0.data(), n.data(), k.data_ptr(), v.data_ptr(), dtype,
+                          rotated, at::cuda::getCurrentCUDAStream().stream()));
+    return {k, v};
+}
+
+// ins_penalize: out = the logits under penalties, bias and mask; settings are
+// device tensors of one value a row, or none.
+void penalize(const at::Tensor &logits, const c10::optional<at::Tensor> &tokens,
+                    const c10::optional<at::Tensor> &lengths, const c10::optional<at::Tensor> &prompts,
+                    const c10::optional<at::Tensor> &of, const c10::optional<at::Tensor> &drafted,
+                    const c10::optional<at::Tensor> &repetition, const c10::optional<at::Tensor> &presence,
+                    const c10::optional<at::Tensor> &frequency, const c10::optional<at::Tensor> &bias,
+                    const c10::optional<at::Tensor> &mask, const at::Tensor &out) {
+    TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && (logits.size(1) < 2 || logits.stride(1) == 1),
+                      "insitu: logits must be a (rows, vocab) CUDA tensor with adjacent columns");
+    const int32_t dtype = element_type(logits.scalar_type());
+    const int64_t n = logits.size(0), vocab = logits.size(1), words = (vocab + 31) / 32;
+    TORCH_CHECK_VALUE(vocab >= 1 && vocab <= (1 << 18) && n <= (1 << 27), "insitu: vocab must be in [1, 262144], got ",
+                      vocab);
+    // a matrix with adjacent columns; returns its row stride
+    auto matrix = [&](const at::Tensor &t, at::ScalarType type, const char *name) {
+        TORCH_CHECK_VALUE(t.device() == logits.device() && t.scalar_type() == type && t.dim() == 2 &&
+                              (t.size(1) < 2 || t.stride(1) == 1),
+                          "insitu: ", name, " must be a 2-D ", type, " tensor with adjacent columns on logits' device");
+        return t.size(0) > 1 ? t.stride(0) : 0;
+    };
+    // one value for each of `m` rows
+    auto vector = [&](const c10::optional<at::Tensor> &t, at::ScalarType type, int64_t m, const char *name) -> void * {
+        if (!t.has_value()) return nullptr;
+        TORCH_CHECK_VALUE(t->device() == logits.device() && t->scalar_type() == type && t->is_contiguous() &&
+                              t->dim() == 1 && t->size(0) == m,
+                          "insitu: ", name, " must be a contiguous ", type, " tensor of ", m,
+                          " values on logits' device");
+        return t->data_ptr();
+    };
+    // one row for all rows of logits, or one each
+    auto shared = [&](const at::Tensor &t, int64_t columns, const char *name) {
+        TORCH_CHECK_VALUE(t.size(1) == columns && (t.size(0) == 1 || t.size(0) == n), "insitu: ", name,
+                          " must hold 1 or ", n, " rows of ", columns, ", got ", t.sizes());
+    };
+    ins_penalties p{};
+    if (tokens.has_value()) {
+        p.tokens_stride = matrix(*tokens, at::kLong, "tokens");
+        p.tokens = tokens->data_ptr<int64_t>();
+        TORCH_CHECK_VALUE(tokens->size(0) <= INT32_MAX && tokens->size(1) <= INT32_MAX, "insitu: too many tokens");
+        TORCH_CHECK_VALUE(of.has_value() || tokens->size(0) == n, "insitu: tokens hold ", tokens->size(0),
+                          " rows; logits hold ", n);
+        p.histories = (int32_t)tokens->size(0);
+        p.history = (int32_t)tokens->size(1);
+        p.lengths = static_cast<int32_t *>(vector(lengths, at::kInt, p.histories, "lengths"));
+        p.prompts = static_cast<int32_t *>(vector(prompts, at::kInt, p.histories, "prompts"));
+        p.of = static_cast<int32_t *>(vector(of, at::kInt, n, "of"));
+    } else {
+        TORCH_CHECK_VALUE(!lengths.has_value() && !prompts.has_value() && !of.has_value(),
+                          "insitu: lengths, prompts and of need tokens");
+    }
+    if (drafted.has_value()) {
+        p.drafted_stride = matrix(*drafted, at::kLong, "drafted");
+        TORCH_CHECK_VALUE(drafted->size(0) == n && drafted->size(1) <= INT32_MAX, "insitu: drafted hold ",
+                          drafted->size(0), " rows; logits hold ", n);
+        p.drafted = drafted->data_ptr<int64_t>();
+        p.n_drafted = (int32_t)drafted->size(1);
+    }
+    if (bias.has_value()) {
+        p.bias_stride = matrix(*bias, at::kFloat, "bias");
+        shared(*bias, vocab, "bias");
+        p.bias = bias->data_ptr<float>();
+    }
+    if (mask.has_value()) {
+        p.mask_stride = matrix(*mask, at::kInt, "mask");
+        shared(*mask, words, "mask");
+        p.mask = mask->data_ptr<int32_t>();
+    }
+    p.repetition = static_cast<float *>(vector(repetition, at::kFloat, n, "repetition"));
+    p.presence = static_cast<float *>(vector(presence, at::kFloat, n, "presence"));
+    p.frequency = static_cast<float *>(vector(frequency, at::kFloat, n, "frequency"));
+    c10::cuda::CUDAGuard guard(logits.device());
+    for (const auto *t : {&repetition, &presence, &frequency})
+        if (t->has_value()) used_here(**t);
+    TORCH_CHECK_VALUE(out.device() == logits.device() && out.scalar_type() == logits.scalar_type() &&
+                          out.sizes() == logits.sizes() && (vocab < 2 || out.stride(1) == 1) &&
+                          (n < 2 || out.stride(0) >= vocab),
+                      "insitu: out must be a tensor of logits' shape, type and device whose rows do not overlap");
+    if (n > 0 && (out.data_ptr() != logits.data_ptr() || (n > 1 && out.stride(0) != logits.stride(0)))) {
+        auto span = [&](const at::Tensor &t) {
+            const auto *from = static_cast<const char *>(t.data_ptr());
+            return std::make_pair(from, from + ((n - 1) * t.stride(0) + vocab) * t.element_size());
+        };
+        const auto a = span(out), b = span(logits);
+        TORCH_CHECK_VALUE(a.second <= b.first || b.second <= a.first,
+                          "insitu: out must be logits itself, or lie wholly before or after it in memory");
+    }
+    check(ins_penalize((int32_t)n, (int32_t)vocab, logits.data_ptr(), dtype, logits.stride(0), out.data_ptr(),
+                       n > 1 ? out.stride(0) : vocab, &p, at::cuda::getCurrentCUDAStream().stream()));
+}
+
 // ins_sample: one token per row of logits (rows, vocab); the settings are
 // device tensors of one value a row, or none.
 std::tuple<at::Tensor, at::Tensor> sample(const at::Tensor &logits, const at::Tensor &uniform,
@@ -306,6 +452,11 @@ TORCH_LIBRARY(insitu, m) {
     m.def("rows(int handle, Tensor anchor, int[] seq_ids, int[] t0, int[] n, int n_kv, int row_bytes) -> Tensor");
     m.def("put_rows(int handle, int[] seq_ids, int[] n, Tensor rows) -> ()");
     m.def("tree_scan(int handle, int[] seq_ids, int[] nodes, Tensor mask, Tensor q, int q_heads) -> Tensor");
+    m.def("chunk_scan(int handle, int[] seq_ids, int[] counts, int window, int sinks, Tensor q, int q_heads) -> Tensor");
+    m.def("dense(int handle, Tensor anchor, int[] seq_ids, int[] t0, int[] n, int n_kv, ScalarType type, "
+          "bool rotated) -> (Tensor, Tensor)");
+    m.def("penalize(Tensor logits, Tensor? tokens, Tensor? lengths, Tensor? prompts, Tensor? of, Tensor? drafted, "
+          "Tensor? repetition, Tensor? presence, Tensor? frequency, Tensor? bias, Tensor? mask, Tensor(a!) out) -> ()");
     m.def("sample(Tensor logits, Tensor uniform, Tensor? temperature, Tensor? top_k, Tensor? top_p, "
           "Tensor? min_p) -> (Tensor, Tensor)");
     m.def("ingress(int handle, int[] seq_ids, Tensor k, Tensor v, Tensor? q, int n_kv, int q_heads, "
@@ -328,5 +479,8 @@ TORCH_LIBRARY_IMPL(insitu, CUDA, m) {
     m.impl("rows", rows);
     m.impl("put_rows", put_rows);
     m.impl("tree_scan", tree_scan);
+    m.impl("chunk_scan", chunk_scan);
+    m.impl("dense", dense);
+    m.impl("penalize", penalize);
     m.impl("sample", sample);
 }

@@ -353,6 +353,41 @@ class PagedCache:
         except (RuntimeError, ValueError) as e:
             _raise_mapped(e)
 
+    def chunk_scan(self, seq_ids, q_rot, counts, *, window: int | None = None, sinks: int = 0) -> torch.Tensor:
+        """Causal attention of a chunk of new tokens of each sequence
+        (ins_chunk_scan), in floating point as ``tree_scan``. The chunk is the
+        sequence's last ``counts`` cached tokens (one number, or one a
+        sequence; 1 is a decode token), appended by ``ingress``, whose rotated
+        queries ``q_rot`` (tokens, n_kv*groups, d) are. ``window``: a token
+        attends the last ``window`` positions, its own among them, and the
+        sequence's first ``sinks`` tokens; None: every position up to its own.
+        Returns q_rot's shape in bfloat16."""
+        g = self.geo
+        q = self._dev_i32(q_rot, (g.num_heads, g.head_dim))
+        ids = _list(seq_ids)
+        if window is not None and window < 1:
+            raise ValueError(f"window={window} must be at least 1, or None")
+        try:
+            return self._ops.chunk_scan(self._h.value or 0, ids, _ids(counts, len(ids)), window or 0, sinks, q,
+                                        g.num_heads)
+        except (RuntimeError, ValueError) as e:
+            _raise_mapped(e)
+
+    def dense(self, seq_ids, t0=0, n=None, *, dtype=torch.bfloat16, rotated: bool = False):
+        """Rows [t0, t0 + n) of each sequence (to its end by default), one
+        sequence after another, as keys and values in floating point
+        (ins_cache_dense): k and v, (sum n, n_kv, d) each, in ``dtype`` (float32,
+        float16, bfloat16). ``rotated``: in the basis that the cache holds, that
+        of ``q_rot``; else the model's own (keys after RoPE)."""
+        ids = _list(seq_ids)
+        first = _ids(t0, len(ids))
+        count = [self.length(s) - f for s, f in zip(ids, first)] if n is None else _ids(n, len(ids))
+        try:
+            return self._ops.dense(self._h.value or 0, self._anchor, ids, first, count, self.geo.n_kv_heads, dtype,
+                                   rotated)
+        except (RuntimeError, ValueError) as e:
+            _raise_mapped(e)
+
     # -- page operations ------------------------------------------------------------
     @property
     def free_pages(self) -> int:

@@ -28,19 +28,18 @@ _SETTINGS = {
 }
 
 
-class Sampler:
-    """Settings of a batch of rows; calling it draws one token a row.
+class RowSettings:
+    """Settings of a batch of rows, each a number, or a 1-D tensor or sequence
+    of one value a row. They are checked here, so a call reads nothing back
+    from the device."""
 
-    ``temperature`` (0 takes the largest logit), ``top_k`` (0: off), ``top_p``
-    and ``min_p`` are numbers, or 1-D tensors or sequences of one value a row.
-    They are checked here, so a call reads nothing back from the device. One
-    ``Sampler`` may be used on several streams."""
+    SETTINGS: dict = {}
 
-    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    def __init__(self, **values):
         self._rows = None
         self._per_row, self._scalar, self._filled = {}, {}, {}
-        for name, value in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
-            dtype, neutral, valid, words = _SETTINGS[name]
+        for name, value in values.items():
+            dtype, neutral, valid, words = self.SETTINGS[name]
             t = torch.as_tensor(value)
             if t.dim() > 1:
                 raise ValueError(f"{name} must be a number or one value a row")
@@ -67,7 +66,7 @@ class Sampler:
         if self._rows not in (None, n):
             raise ValueError(f"the settings are for {self._rows} rows; logits hold {n}")
         out = []
-        for name in _SETTINGS:
+        for name in self.SETTINGS:
             t = self._per_row.get(name)
             if t is not None:
                 if t.device != device:
@@ -76,11 +75,25 @@ class Sampler:
                 t = self._filled.get(name)
                 if t is None or t.device != device or t.numel() < n:
                     rows = max(256, 1 << (n - 1).bit_length())
-                    t = torch.full((rows,), self._scalar[name], dtype=_SETTINGS[name][0]).to(device)
+                    t = torch.full((rows,), self._scalar[name], dtype=self.SETTINGS[name][0]).to(device)
                     self._filled[name] = t
                 t = t[:n]
             out.append(t)
         return out
+
+
+class Sampler(RowSettings):
+    """Settings of a batch of rows; calling it draws one token a row.
+
+    ``temperature`` (0 takes the largest logit), ``top_k`` (0: off), ``top_p``
+    and ``min_p`` are numbers, or 1-D tensors or sequences of one value a row.
+    They are checked here, so a call reads nothing back from the device. One
+    ``Sampler`` may be used on several streams."""
+
+    SETTINGS = _SETTINGS
+
+    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        super().__init__(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
 
     def __call__(self, logits: torch.Tensor, uniform: torch.Tensor):
         """``logits`` (rows, vocab) float32, float16 or bfloat16 on the GPU,

@@ -80,6 +80,28 @@ class DraftTree:
             self._mask = self._mask.to(device)
         return self._mask
 
+    def paths(self, drafted, device=None) -> torch.Tensor:
+        """The drafted tokens that stand before what each node's logits say: its
+        ancestors' and its own, (nodes, longest path) int64, filled up with -1.
+        ``drafted``: the tokens of all nodes. What ``Penalties`` adds to a
+        sequence's tokens; the sequence of each node is ``sequences``."""
+        if self.parents is None:
+            raise ValueError("a tree from masks has no paths")
+        tokens = drafted.tolist() if torch.is_tensor(drafted) else [int(t) for t in drafted]
+        if len(tokens) != len(self):
+            raise ValueError(f"{len(tokens)} drafted tokens for {len(self)} nodes")
+        rows = []
+        for first, tree in zip(self.offsets, self.parents):
+            for i, p in enumerate(tree):
+                rows.append((rows[first + p] if p >= 0 else []) + [tokens[first + i]])
+        longest = max(map(len, rows), default=0)
+        return torch.tensor([r + [-1] * (longest - len(r)) for r in rows], dtype=torch.int64,
+                            device=device).reshape(len(rows), longest)
+
+    def sequences(self, device=None) -> torch.Tensor:
+        """Which tree of the batch each node belongs to, (nodes,) int32."""
+        return torch.tensor([b for b, n in enumerate(self.counts) for _ in range(n)], dtype=torch.int32, device=device)
+
     def accept(self, b: int, drafted, sampled, first: int) -> tuple[list, int]:
         """The path of tree ``b`` that sampling confirms. ``drafted``: the
         tokens of its nodes; ``sampled``: the token drawn at each node (what
