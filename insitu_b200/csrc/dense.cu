@@ -17,142 +17,300 @@
 namespace ins {
 
 // Rows [t0, t0 + n) of `seq`, at row `row` of the outputs; the span's tiles of
-// DENSE_TILE rows are tiles [tile, next span's tile).
+// 32 rows are tiles [tile, next span's tile).
 struct DenseSpan {
     int32_t seq, t0, n, tile;
     int64_t row;
 };
 
-constexpr int DENSE_TILE = 32, DENSE_THREADS = 256;
+constexpr int DENSE_WARPS = 8, DENSE_THREADS = DENSE_WARPS * 32;
 
-template <typename T>
-__device__ __forceinline__ void store8(T *dst, const float (&x)[8]);
-template <>
-__device__ __forceinline__ void store8(float *dst, const float (&x)[8]) {
-    reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+// Two floats at once (one instruction for both).
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
 }
-template <>
-__device__ __forceinline__ void store8(__half *dst, const float (&x)[8]) {
-    __half2 h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(h);
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+    float2 r;
+    asm("{ .reg .b64 x, y, m; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 m, {%6, %6}; "
+        "fma.rn.f32x2 x, y, m, x; mov.b64 {%0, %1}, x; }"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(-1.0f));
+    return r;
 }
-template <>
-__device__ __forceinline__ void store8(__nv_bfloat16 *dst, const float (&x)[8]) {
-    __nv_bfloat162 h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(h);
-}
-
-// The centroids of 8 codes of `bits` bits from byte `at` of a row on.
-template <int BITS>
-__device__ __forceinline__ void centroids8(const uint8_t *at, int bits_any, const float *cent, float (&y)[8]) {
-    const int bits = BITS ? BITS : bits_any;
-    uint64_t w = 0;
-    if constexpr (BITS == 4) w = *reinterpret_cast<const uint32_t *>(at);
-    else if constexpr (BITS == 2) w = *reinterpret_cast<const uint16_t *>(at);
-    else
-        for (int i = 0; i < bits; ++i) w |= (uint64_t)at[i] << (8 * i);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = cent[(uint32_t)(w >> (i * bits)) & ((1u << bits) - 1u)];
+__device__ __forceinline__ float2 mul2(float2 a, float s) {
+    float2 r;
+    asm("{ .reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %4}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x; }"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(s));
+    return r;
 }
 
-// Four threads a vector; thread t holds channels 8 t + i and 32 + 8 t + i (a
-// store of 16 bytes is then a contiguous run of the four). Stages 1, 2, 4 and
-// 32 of the butterfly stay in a thread, 8 and 16 exchange with threads t ^ 1
-// and t ^ 2.
-__device__ __forceinline__ void hadamard(float (&a)[8], float (&b)[8], int t) {
+// The butterfly's stages of distances FROM to 32 channels over a vector (v[i]:
+// channels 2 i and 2 i + 1).
+template <int FROM>
+__device__ __forceinline__ void butterfly(float2 (&v)[32]) {
+    if constexpr (FROM == 1) {
 #pragma unroll
-    for (int h = 1; h < 8; h *= 2)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (!(i & h)) {
-                const float x = a[i], y = a[i + h], u = b[i], v = b[i + h];
-                a[i] = x + y, a[i + h] = x - y, b[i] = u + v, b[i + h] = u - v;
-            }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float x = a[i], y = b[i];
-        a[i] = x + y, b[i] = x - y;
+        for (int i = 0; i < 32; ++i) v[i] = make_float2(v[i].x + v[i].y, v[i].x - v[i].y);
     }
 #pragma unroll
-    for (int h = 1; h < 4; h *= 2) {
-        const float s = t & h ? -1.0f : 1.0f;
+    for (int h = FROM > 1 ? FROM / 2 : 1; h < 32; h *= 2)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            a[i] = fmaf(s, a[i], __shfl_xor_sync(FULL, a[i], h));
-            b[i] = fmaf(s, b[i], __shfl_xor_sync(FULL, b[i], h));
+        for (int i = 0; i < 32; ++i)
+            if (!(i & h)) {
+                const float2 x = v[i], y = v[i + h];
+                v[i] = add2(x, y), v[i + h] = sub2(x, y);
+            }
+}
+
+// Tables in shared memory that decode several codes at a time, and take the
+// butterfly's first stages with them (TURN): of a width of 4 bits a byte's two
+// channels, of 3 bits six bits' two, of 2 bits a byte's four. A copy for each
+// lane that reads at the same time (16 of 8 bytes, 8 of 16), so that no two
+// meet in a bank. At 4b/2b both tables' entries alternate, 256 bytes apart, so
+// that one byte permute makes an address of a byte of codes. Other widths: a
+// table of single centroids.
+template <int BITS, int STRIDE>
+struct DenseTable {
+    static constexpr int ENTRIES = BITS == 4 ? 256 : BITS == 3 ? 64 : BITS == 2 ? 256 : 256;
+    static constexpr int BYTES = BITS == 0 ? 1024 : ENTRIES * STRIDE;
+    static constexpr int STAGES = BITS == 2 ? 2 : BITS ? 1 : 0;      // of the butterfly, if TURN
+    static __device__ __forceinline__ void fill(uint8_t *sm, const int64_t *cent, int count, bool turn) {
+        if constexpr (BITS == 0) {
+            for (int i = threadIdx.x; i < count; i += DENSE_THREADS) reinterpret_cast<float *>(sm)[i] = (float)cent[i];
+        } else {
+            // one thread an entry's copy
+            constexpr int W = BITS == 2 ? 4 : 2, COPIES = 32 / W;
+            for (int i = threadIdx.x; i < ENTRIES * COPIES; i += DENSE_THREADS) {
+                const int e = i / COPIES;
+                float c[W];
+#pragma unroll
+                for (int k = 0; k < W; ++k) c[k] = (float)cent[e >> (BITS * k) & ((1 << BITS) - 1)];
+                if (turn) {
+#pragma unroll
+                    for (int h = 1; h < W; h *= 2)
+#pragma unroll
+                        for (int k = 0; k < W; ++k)
+                            if (!(k & h)) {
+                                const float x = c[k], y = c[k + h];
+                                c[k] = x + y, c[k + h] = x - y;
+                            }
+                }
+                float *to = reinterpret_cast<float *>(sm + e * STRIDE) + i % COPIES * W;
+#pragma unroll
+                for (int k = 0; k < W; ++k) to[k] = c[k];
+            }
         }
     }
+};
+
+// A row's codes, as 8-byte words from global memory.
+template <int BITS>
+struct DenseCodes {
+    static constexpr int WORDS = BITS ? BITS : 8;
+    uint2 w[WORDS];
+    __device__ __forceinline__ void load(const uint8_t *row, int bits) {
+        if constexpr (BITS == 4 || BITS == 2) {
+#pragma unroll
+            for (int i = 0; i < BITS / 2; ++i) {
+                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(row) + i);
+                w[2 * i] = make_uint2(x.x, x.y), w[2 * i + 1] = make_uint2(x.z, x.w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i)
+                if (BITS || i < bits) w[i] = __ldg(reinterpret_cast<const uint2 *>(row) + i);
+        }
+    }
+    __device__ __forceinline__ uint32_t word(int i) const { return i & 1 ? w[i / 2].y : w[i / 2].x; }
+    // `bits` bits from bit `at` on (both constants once unrolled)
+    __device__ __forceinline__ uint32_t field(int at, int bits) const {
+        const int i = at / 32, sh = at % 32;
+        const uint32_t x = sh + bits <= 32 ? word(i) >> sh : __funnelshift_r(word(i), word(i + 1), sh);
+        return x & ((1u << bits) - 1u);
+    }
+    template <int B>
+    __device__ __forceinline__ void singles(const uint8_t *sm, float2 (&v)[32]) const {
+        if constexpr (B <= WORDS) {
+            const float *cent = reinterpret_cast<const float *>(sm);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = make_float2(cent[field(2 * i * B, B)], cent[field((2 * i + 1) * B, B)]);
+        }
+    }
+    // byte `i` times 256, plus what is below 256
+    __device__ __forceinline__ uint32_t entry(int i, uint32_t plus) const {
+        return __byte_perm(word(i / 4), plus, 0x5504 | i % 4 << 4);
+    }
+    __device__ __forceinline__ void decode(const uint8_t *sm, int bits, int lane, float2 (&v)[32]) const {
+        if constexpr (BITS == 2) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float4 x = *reinterpret_cast<const float4 *>(sm + entry(i, 128 + lane % 8 * 16));
+                v[2 * i] = make_float2(x.x, x.y), v[2 * i + 1] = make_float2(x.z, x.w);
+            }
+        } else if constexpr (BITS == 4) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = *reinterpret_cast<const float2 *>(sm + entry(i, lane % 16 * 8));
+        } else if constexpr (BITS != 0) {
+            const uint8_t *mine = sm + lane % 16 * 8;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                v[i] = *reinterpret_cast<const float2 *>(mine + field(2 * BITS * i, 2 * BITS) * 128);
+        } else {
+            switch (bits) {
+                case 1: singles<1>(sm, v); break;
+                case 2: singles<2>(sm, v); break;
+                case 3: singles<3>(sm, v); break;
+                case 4: singles<4>(sm, v); break;
+                case 5: singles<5>(sm, v); break;
+                case 6: singles<6>(sm, v); break;
+                case 7: singles<7>(sm, v); break;
+                default: singles<8>(sm, v); break;
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ uint32_t dense_pair(float2 x, __half *) {
+    const __half2 h = __floats2half2_rn(x.x, x.y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t dense_pair(float2 x, __nv_bfloat16 *) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// One CTA per 32 rows of a span, all KV heads. Bound by the bytes: 52 read and
-// 256 or 512 written a row and head.
+template <int KB, int VB>
+struct DenseLayout {
+    static constexpr bool BOTH = KB == 4 && VB == 2;
+    static constexpr int STRIDE = BOTH ? 256 : 128;
+    static constexpr int K_BYTES = DenseTable<KB, STRIDE>::BYTES;
+    // (at 4b/2b the values' entries begin at byte 128 of the keys', which their addresses add)
+    static constexpr int V_AT = BOTH ? 128 : K_BYTES;
+    static constexpr int SIGNS_AT = K_BYTES + (BOTH ? 0 : DenseTable<VB, STRIDE>::BYTES);
+    static constexpr int STAGE_AT = SIGNS_AT + 256;
+};
+
+// A warp takes 32 rows of a KV head, a thread a row, in turn with the next
+// task's codes already on their way. A thread holds its whole vector, so the
+// butterfly needs no exchange; the finished vectors go through shared memory
+// (rows padded by 16 bytes) so that eight lanes write each 128 bytes.
 template <int KB, int VB, typename T, class Src>
-__global__ void __launch_bounds__(DENSE_THREADS) k_dense(Geo g, const DevTables *__restrict__ tb,
-                                                         const uint8_t *__restrict__ pool,
-                                                         const int32_t *__restrict__ table, T *__restrict__ k,
-                                                         T *__restrict__ v, int32_t n_spans, int32_t rounds,
-                                                         float unit, const __grid_constant__ Src src) {
-    __shared__ float cent[2][256];
-    __shared__ int64_t at[DENSE_TILE];
-    __shared__ int32_t in_page[DENSE_TILE];
-    const int tid = threadIdx.x, t = tid % 4;
-    for (int i = tid; i < (1 << g.kb); i += DENSE_THREADS) cent[0][i] = (float)tb->k_cent[i];
-    for (int i = tid; i < (1 << g.vb); i += DENSE_THREADS) cent[1][i] = (float)tb->v_cent[i];
+__global__ void __launch_bounds__(DENSE_THREADS, sizeof(T) == 4 ? 1 : 2)
+    k_dense(Geo g, const DevTables *__restrict__ tb, const uint8_t *__restrict__ pool,
+            const int32_t *__restrict__ table, T *__restrict__ k, T *__restrict__ v, int32_t n_spans, int64_t tasks,
+            int32_t rounds, float unit, const __grid_constant__ Src src) {
+    using L = DenseLayout<KB, VB>;
+    using KT = DenseTable<KB, L::STRIDE>;
+    using VT = DenseTable<VB, L::STRIDE>;
+    constexpr int LINE = D * (int)sizeof(T) + 16;
+    extern __shared__ __align__(128) uint8_t sm[];
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    uint8_t *const stage = sm + L::STAGE_AT + warp * 32 * LINE;
+    KT::fill(sm, tb->k_cent, 1 << g.kb, rounds > 0);
+    VT::fill(sm + L::V_AT, tb->v_cent, 1 << g.vb, rounds > 0);
+    // the last signs, as the sign bits of a vector's words of type T
+    uint32_t *const signs = reinterpret_cast<uint32_t *>(sm + L::SIGNS_AT);
+    if (tid < 64) {
+        const uint64_t m = rounds > 0 ? tb->sign_mask[0] : 0;
+        if (sizeof(T) == 4) signs[tid] = (uint32_t)(m >> tid & 1) << 31;
+        else if (tid < 32) signs[tid] = (uint32_t)(m >> (2 * tid) & 1) << 15 | (uint32_t)(m >> (2 * tid + 1) & 1) << 31;
+    }
     wait_prior_grid();
-    const DenseSpan *spans = reinterpret_cast<const DenseSpan *>(src.data());
-    int lo = 0, hi = n_spans - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (spans[mid].tile <= (int)blockIdx.x) lo = mid;
-        else hi = mid - 1;
-    }
-    const DenseSpan sp = spans[lo];
-    const int r0 = (blockIdx.x - sp.tile) * DENSE_TILE, n = min(DENSE_TILE, sp.n - r0);
-    if (tid < n) {
-        const int p = sp.t0 + r0 + tid;
-        at[tid] = (int64_t)table[(int64_t)sp.seq * g.max_pages + p / g.P] * g.page_bytes;
-        in_page[tid] = p % g.P;
-    }
     __syncthreads();
-    const int all = n * g.n_kv;
-    // whole warps go around, as the butterfly exchanges lanes
-    for (int i = tid / 4; i / 8 * 8 < all; i += DENSE_THREADS / 4) {
-        const bool live = i < all;
-        const int r = live ? i / g.n_kv : 0, head = live ? i % g.n_kv : 0;
-        const uint8_t *region = pool + at[r] + head * g.head_bytes;
-        const uint32_t norms = *reinterpret_cast<const uint32_t *>(region + nplane_off(g) + (int64_t)in_page[r] * 4);
-        const int64_t to = ((sp.row + r0 + r) * g.n_kv + head) * D + 8 * t;
-        auto vector = [&](auto width, const uint8_t *row, int bits, const float *c, int16_t norm, T *dst) {
-            constexpr int BITS = decltype(width)::value;
-            float a[8], b[8];
-            centroids8<BITS>(row + t * bits, bits, c, a);
-            centroids8<BITS>(row + (4 + t) * bits, bits, c, b);
-            const float scale = (float)norm * unit;
+    const DenseSpan *spans = reinterpret_cast<const DenseSpan *>(src.data());
+    // a task's rows: `n` of them, the first at row `row` of the outputs
+    struct Task {
+        int64_t row;
+        int32_t n, head;
+    };
+    DenseCodes<KB> kc;
+    DenseCodes<VB> vc;
+    uint32_t norms = 0;
+    auto load = [&](int64_t task) {
+        Task t{0, 0, 0};
+        if (task >= tasks) return t;
+        const int tile = (int)(task / g.n_kv);
+        t.head = (int)(task - (int64_t)tile * g.n_kv);
+        int lo = 0, hi = n_spans - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (spans[mid].tile <= tile) lo = mid;
+            else hi = mid - 1;
+        }
+        const DenseSpan sp = spans[lo];
+        const int r0 = (tile - sp.tile) * 32;
+        t.n = min(32, sp.n - r0);
+        t.row = sp.row + r0;
+        const int p = sp.t0 + r0 + min(lane, t.n - 1);
+        const int page = g.p_log2 >= 0 ? p >> g.p_log2 : p / g.P, in = p - page * g.P;
+        const uint8_t *region = pool + region_off(g, table[(int64_t)sp.seq * g.max_pages + page], t.head);
+        kc.load(region + (int64_t)in * g.kbytes, g.kb);
+        vc.load(region + vplane_off(g) + (int64_t)in * g.vbytes, g.vb);
+        norms = __ldg(reinterpret_cast<const uint32_t *>(region + nplane_off(g)) + in);
+        return t;
+    };
+    const int64_t stride = (int64_t)gridDim.x * DENSE_WARPS;
+    int64_t task = (int64_t)blockIdx.x * DENSE_WARPS + warp;
+    Task t = load(task);
+    while (task < tasks) {
+        const float ks = (float)(int16_t)(norms & 0xffffu) * unit, vs = (float)(int16_t)(norms >> 16) * unit;
+        const Task now = t;
+        auto finish = [&](float2 (&z)[32], auto stages, float scale, T *dst) {
+            constexpr int DONE = decltype(stages)::value;
             for (int rd = rounds - 1; rd >= 0; --rd) {
-                hadamard(a, b, t);
+                if (rd == rounds - 1) butterfly<1 << DONE>(z);
+                else butterfly<1>(z);
+                if (rd == 0) break;                              // the last signs go on after the rounding
                 const uint64_t m = tb->sign_mask[rd];
-                const uint32_t ma = (uint32_t)(m >> (8 * t)), mb = (uint32_t)(m >> (32 + 8 * t));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    a[j] = __uint_as_float(__float_as_uint(a[j]) ^ (ma >> j << 31));
-                    b[j] = __uint_as_float(__float_as_uint(b[j]) ^ (mb >> j << 31));
+                for (int i = 0; i < 32; ++i)
+                    z[i] = make_float2(m >> (2 * i) & 1 ? -z[i].x : z[i].x, m >> (2 * i + 1) & 1 ? -z[i].y : z[i].y);
+            }
+            __syncwarp();                                        // the stage's last vectors have been read
+            uint32_t *to = reinterpret_cast<uint32_t *>(stage + lane * LINE);
+            const uint4 *sign = reinterpret_cast<const uint4 *>(signs);
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = dense_pair(mul2(z[4 * c + j], scale), dst);
+                    const uint4 s = sign[c];
+                    reinterpret_cast<uint4 *>(to)[c] = make_uint4(w[0] ^ s.x, w[1] ^ s.y, w[2] ^ s.z, w[3] ^ s.w);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    const float2 a = mul2(z[2 * c], scale), b = mul2(z[2 * c + 1], scale);
+                    const uint4 s = sign[c];
+                    reinterpret_cast<uint4 *>(to)[c] =
+                        make_uint4(__float_as_uint(a.x) ^ s.x, __float_as_uint(a.y) ^ s.y, __float_as_uint(b.x) ^ s.z,
+                                   __float_as_uint(b.y) ^ s.w);
                 }
             }
+            __syncwarp();
+            constexpr int CHUNKS = D * (int)sizeof(T) / 16, ROWS = 32 / CHUNKS;   // of 16 bytes a row; rows at a time
+            T *out = dst + (now.row * g.n_kv + now.head) * D;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) a[j] *= scale, b[j] *= scale;
-            if (!live) return;
-            store8(dst + to, a);
-            store8(dst + to + 32, b);
+            for (int r0 = 0; r0 < 32; r0 += ROWS) {
+                const int r = r0 + lane / CHUNKS, c = lane % CHUNKS;
+                if (r < now.n)
+                    __stcs(reinterpret_cast<uint4 *>(out + (int64_t)r * g.n_kv * D) + c,
+                           *reinterpret_cast<const uint4 *>(stage + r * LINE + c * 16));
+            }
         };
-        vector(std::integral_constant<int, KB>(), region + (int64_t)in_page[r] * g.kbytes, g.kb, cent[0],
-               (int16_t)(norms & 0xffffu), k);
-        vector(std::integral_constant<int, VB>(), region + vplane_off(g) + (int64_t)in_page[r] * g.vbytes, g.vb,
-               cent[1], (int16_t)(norms >> 16), v);
+        float2 x[32];
+        kc.decode(sm, g.kb, lane, x);
+        finish(x, std::integral_constant<int, KT::STAGES>(), ks, k);
+        vc.decode(L::BOTH ? sm : sm + L::V_AT, g.vb, lane, x);
+        task += stride;
+        t = load(task);
+        finish(x, std::integral_constant<int, VT::STAGES>(), vs, v);
     }
 }
 
@@ -162,6 +320,8 @@ template <typename T>
 int launch_dense(CacheBase *c, const Plan &plan, int32_t n_spans, int64_t tiles, void *k, void *v, bool rotated,
                  cudaStream_t s) {
     const Geo &g = c->g;
+    int sms = 148;
+    CK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c->device));
     // a round of the rotation multiplies by 2^-rot_shift (or rot_inv / 2^15), and H H = 64
     const int rounds = rotated ? 0 : g.rounds;
     const double back = (g.rot_shift >= 0 ? std::ldexp(1.0, g.rot_shift) : 32768.0 / g.rot_inv) / 64.0;
@@ -171,10 +331,18 @@ int launch_dense(CacheBase *c, const Plan &plan, int32_t n_spans, int64_t tiles,
         auto fn = g.kb == 4 && g.vb == 2   ? k_dense<4, 2, T, S>
                   : g.kb == 3 && g.vb == 3 ? k_dense<3, 3, T, S>
                                            : k_dense<0, 0, T, S>;
+        const size_t tables = g.kb == 4 && g.vb == 2   ? DenseLayout<4, 2>::STAGE_AT
+                              : g.kb == 3 && g.vb == 3 ? DenseLayout<3, 3>::STAGE_AT
+                                                       : DenseLayout<0, 0>::STAGE_AT;
+        const size_t smem = tables + DENSE_THREADS * (D * sizeof(T) + 16);
+        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        const int64_t tasks = tiles * g.n_kv, ctas = (tasks + DENSE_WARPS - 1) / DENSE_WARPS;
+        const unsigned grid = (unsigned)std::min<int64_t>(ctas, (int64_t)sms * (sizeof(T) == 4 ? 1 : 2));
         *c->launches += 1;
-        return launch_after(fn, (unsigned)tiles, (unsigned)DENSE_THREADS, 0, s, g, (const DevTables *)c->d_tables,
+        return launch_after(fn, grid, (unsigned)DENSE_THREADS, smem, s, g, (const DevTables *)c->d_tables,
                             (const uint8_t *)c->d_pool, (const int32_t *)c->d_page_table, (T *)k, (T *)v, n_spans,
-                            (int32_t)rounds, unit, src);
+                            tasks, (int32_t)rounds, unit, src);
     });
 }
 
@@ -192,7 +360,7 @@ int dense_body(CacheBase *c, int32_t B, const int32_t *seq, const int64_t *t0, c
                                          " cached tokens");
         if (n[b] == 0) continue;
         spans.push_back(DenseSpan{seq[b], (int32_t)t0[b], (int32_t)n[b], (int32_t)tiles, total});
-        tiles += (n[b] + DENSE_TILE - 1) / DENSE_TILE;
+        tiles += (n[b] + 31) / 32;
         total += n[b];
         if (tiles > INT32_MAX) return fail(INS_EBADLEN, "too many rows in one call");
     }

@@ -15,13 +15,15 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "cache.h"
 
 namespace ins {
 
-constexpr int PEN_THREADS = 256;
+constexpr int PEN_THREADS = 256, PEN_BYTES = 32768;      // logits of a slice, at most
 constexpr int PEN_MAX_VOCAB = 1 << 18;
+constexpr int PEN_LIST = 4096;               // tokens with a count that a slice can list
 constexpr uint32_t PEN_ASKED = 1u << 31;     // in a count: the token is in the prompt
 
 struct PenaltyArgs {
@@ -35,68 +37,219 @@ struct PenaltyArgs {
     const float *bias;
     const uint32_t *mask;
     int64_t bias_stride, mask_stride;
-    int32_t vocab, slice, history, histories, n_drafted;
+    int32_t vocab, slices, slice_log2;       // CTAs a row, each for 2^slice_log2 tokens
+    int32_t history, histories, n_drafted;
+};
+
+// Eight logits as 16-byte vectors: two of floats, one of halves.
+template <typename T>
+struct Eight {
+    static constexpr int N = sizeof(T) / 2;
+    uint4 v[N];
+    __device__ __forceinline__ T *at() { return reinterpret_cast<T *>(v); }
 };
 
 __device__ __forceinline__ float pen_f32(float x) { return x; }
 __device__ __forceinline__ float pen_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float pen_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ T pen_to(float x);
-template <>
-__device__ __forceinline__ float pen_to(float x) { return x; }
-template <>
-__device__ __forceinline__ __half pen_to(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 pen_to(float x) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ void pen_set(float &to, float x) { to = x; }
+__device__ __forceinline__ void pen_set(__half &to, float x) { to = __float2half_rn(x); }
+__device__ __forceinline__ void pen_set(__nv_bfloat16 &to, float x) { to = __float2bfloat16_rn(x); }
 
+// -inf in the elements whose bit is 0.
+__device__ __forceinline__ void forbid(Eight<float> &e, uint32_t bits) {
+    uint32_t *w = reinterpret_cast<uint32_t *>(e.v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = bits >> i & 1u ? w[i] : 0xff800000u;
+}
+template <typename T>
+__device__ __forceinline__ void forbid(Eight<T> &e, uint32_t bits) {
+    constexpr uint32_t none = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    uint32_t *w = reinterpret_cast<uint32_t *>(e.v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t keep = (bits >> (2 * i) & 1u) * 0xffffu | (bits >> (2 * i + 1) & 1u) * 0xffff0000u;
+        w[i] = (w[i] & keep) | (none & ~keep);
+    }
+}
+
+// Eight elements from an address of any alignment (to its element): the
+// 16-byte vectors around them, shifted together. `off`: the address modulo 16,
+// the same for the whole row.
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T *from, uint32_t off) {
+    Eight<T> e;
+    const uint4 *p = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(from) - off);
+    uint4 x = __ldcs(p);
+#pragma unroll
+    for (int i = 0; i < Eight<T>::N; ++i) {
+        if (off == 0) {
+            e.v[i] = x;
+            if (i + 1 < Eight<T>::N) x = __ldcs(p + i + 1);
+            continue;
+        }
+        const uint4 y = __ldcs(p + i + 1);
+        uint32_t a, b, c, d, f;                      // the words that hold the 16 bytes
+        switch (off / 4) {
+            case 0: a = x.x, b = x.y, c = x.z, d = x.w, f = y.x; break;
+            case 1: a = x.y, b = x.z, c = x.w, d = y.x, f = y.y; break;
+            case 2: a = x.z, b = x.w, c = y.x, d = y.y, f = y.z; break;
+            default: a = x.w, b = y.x, c = y.y, d = y.z, f = y.w; break;
+        }
+        const uint32_t sh = off % 4 * 8;
+        e.v[i] = make_uint4(__funnelshift_r(a, b, sh), __funnelshift_r(b, c, sh), __funnelshift_r(c, d, sh),
+                            __funnelshift_r(d, f, sh));
+        x = y;
+    }
+    return e;
+}
+
+// A thread changes PEN_GROUPS groups of eight logits, the groups where its
+// result's rows are aligned to 16 bytes, and single ones at a slice's ends. It
+// loads them before the tokens are counted, so that their latency passes
+// meanwhile.
 template <typename T>
 __global__ void __launch_bounds__(PEN_THREADS) k_penalize(const PenaltyArgs a) {
-    extern __shared__ __align__(16) uint32_t counts[];          // [slice] counts, then a bit each
+    // [slice] counts, then values; a bit each; up to PEN_LIST tokens that have one
+    extern __shared__ __align__(16) uint32_t counts[];
+    __shared__ int listed;
+    constexpr int GROUPS = PEN_BYTES / (8 * (int)sizeof(T)) / PEN_THREADS;
     wait_prior_grid();
-    const int slices = (a.vocab + a.slice - 1) / a.slice;
-    const int64_t row = blockIdx.x / slices;
-    const int first = (int)(blockIdx.x % slices) * a.slice, n = min(a.slice, a.vocab - first);
+    const int64_t row = blockIdx.x / a.slices;
+    const int slice = 1 << a.slice_log2, first = (int)(blockIdx.x % a.slices) << a.slice_log2;
+    const int n = min(slice, a.vocab - first);
     const int tid = threadIdx.x;
+    const T *x = static_cast<const T *>(a.logits) + row * a.stride + first;
+    T *y = static_cast<T *>(a.out) + row * a.out_stride + first;
+    const int head = min(n, (int)((16 - ((uintptr_t)y & 15)) & 15) / (int)sizeof(T));
+    const int body = (n - head) / 8;
+    const uint32_t off = (uint32_t)((uintptr_t)(x + head) & 15);
+    const uint32_t *mask = a.mask ? a.mask + row * a.mask_stride + first / 32 : nullptr;
+    // bits i to i + 7 of a row of words
+    auto eight_bits = [&](const uint32_t *w, int i) -> uint32_t {
+        if (head == 0) return reinterpret_cast<const uint8_t *>(w)[i / 8];      // i is a multiple of 8
+        const uint32_t lo = w[i / 32], hi = w[(i + 7) / 32];
+        return __funnelshift_r(lo, hi, i % 32) & 0xffu;
+    };
+    Eight<T> e[GROUPS];
+    uint32_t allowed[GROUPS];
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+        const int i = head + 8 * (tid + k * PEN_THREADS);
+        allowed[k] = 0xffu;
+        if (tid + k * PEN_THREADS < body) {
+            e[k] = load_eight(x + i, off);
+            if (mask) allowed[k] = eight_bits(mask, i);
+        }
+    }
+
     const float r = a.repetition ? a.repetition[row] : 1.0f;
     const float presence = a.presence ? a.presence[row] : 0.0f, frequency = a.frequency ? a.frequency[row] : 0.0f;
     const bool counted = r != 1.0f || presence != 0.0f || frequency != 0.0f;
-    uint32_t *any = counts + a.slice;
+    uint32_t *any = counts + slice;
+    uint16_t *list = reinterpret_cast<uint16_t *>(any + slice / 32);
     if (counted) {
-        for (int i = tid; i < a.slice + a.slice / 32; i += PEN_THREADS) counts[i] = 0;
+        if (tid == 0) listed = 0;
+        for (int i = tid; i < (slice + slice / 32) / 4; i += PEN_THREADS)
+            reinterpret_cast<uint4 *>(counts)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        auto add = [&](int64_t token, bool asked) {
-            const int64_t at = token - first;
-            if (at < 0 || at >= n) return;                       // another slice's, or no token at all
-            if (asked) atomicOr(&counts[at], PEN_ASKED);
-            else atomicAdd(&counts[at], 1u);
-            atomicOr(&any[at / 32], 1u << (at % 32));
+        // A warp adds up to 8 tokens a lane: all counts first, then the tokens
+        // that had none before join the list.
+        auto add = [&](const int64_t (&id)[8], int i, int step, int prompt) {
+            uint32_t fresh = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (id[k] >= first && id[k] < first + n) {       // else another slice's, or no token at all
+                    uint32_t *count = &counts[(int)id[k] - first];
+                    const uint32_t old = i + k * step < prompt ? atomicOr(count, PEN_ASKED) : atomicAdd(count, 1u);
+                    fresh |= (old == 0) << k;
+                }
+            if (!__any_sync(FULL, fresh)) return;
+            int total = __popc(fresh), at = total;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int before = __shfl_up_sync(FULL, at, o);
+                if (tid % 32 >= o) at += before;
+            }
+            int base = 0;
+            if (tid % 32 == 31) base = atomicAdd(&listed, at);
+            at += __shfl_sync(FULL, base, 31) - total;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (fresh >> k & 1u) {
+                    if (at < PEN_LIST) list[at] = (uint16_t)((int)id[k] - first);
+                    ++at;
+                }
         };
         const int64_t h = a.of ? a.of[row] : row;
         if (a.tokens && h >= 0 && h < a.histories) {
             const int len = a.lengths ? max(0, min(a.lengths[h], a.history)) : a.history;
             const int prompt = a.prompts ? a.prompts[h] : 0;
             const int64_t *t = a.tokens + h * a.tokens_stride;
-            for (int i = tid; i < len; i += PEN_THREADS) add(t[i], i < prompt);
+            for (int i = tid; i - tid < len; i += 8 * PEN_THREADS) {
+                int64_t id[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) id[k] = i + k * PEN_THREADS < len ? t[i + k * PEN_THREADS] : -1;
+                add(id, i, PEN_THREADS, prompt);
+            }
         }
-        for (int i = tid; i < a.n_drafted; i += PEN_THREADS) add(a.drafted[row * a.drafted_stride + i], false);
+        for (int i = tid; i - tid < a.n_drafted; i += PEN_THREADS) {
+            int64_t id[8] = {-1, -1, -1, -1, -1, -1, -1, -1};
+            if (i < a.n_drafted) id[0] = a.drafted[row * a.drafted_stride + i];
+            add(id, 0, 0, 0);
+        }
         __syncthreads();
-    }
-    const T *x = static_cast<const T *>(a.logits) + row * a.stride;
-    T *y = static_cast<T *>(a.out) + row * a.out_stride;
-    const float *bias = a.bias ? a.bias + row * a.bias_stride : nullptr;
-    const uint32_t *mask = a.mask ? a.mask + row * a.mask_stride : nullptr;
-    auto change = [&](float v, int i) {
-        if (counted && (any[(i - first) / 32] >> ((i - first) % 32) & 1u)) {
-            const uint32_t c = counts[i - first], said = c & ~PEN_ASKED;
+        // each such token's value takes its count's place, before any result is written
+        auto value = [&](int i, float v) {
+            const uint32_t said = counts[i] & ~PEN_ASKED;
             v = v > 0.0f ? __fdiv_rn(v, r) : v * r;
             if (said) v = v - frequency * (float)said - presence;
+            counts[i] = __float_as_uint(v);
+            atomicOr(&any[i / 32], 1u << (i % 32));
+        };
+        if (listed <= PEN_LIST) {
+            for (int j = tid; j < listed; j += 4 * PEN_THREADS) {
+                int i[4];
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) i[k] = j + k * PEN_THREADS < listed ? list[j + k * PEN_THREADS] : -1;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = i[k] >= 0 ? pen_f32(x[i[k]]) : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (i[k] >= 0) value(i[k], v[k]);
+            }
+        } else {
+            for (int i = tid; i < n; i += PEN_THREADS)
+                if (counts[i]) value(i, pen_f32(x[i]));
         }
-        if (bias) v += bias[i];
-        if (mask && !(mask[i / 32] >> (i % 32) & 1u)) v = -INFINITY;
-        return v;
+        __syncthreads();
+    }
+    const float *bias = a.bias ? a.bias + row * a.bias_stride + first : nullptr;
+    // element i, whose logit is v and whose bit of `any` is `has`
+    auto change = [&](float v, int i, bool has) {
+        if (has) v = __uint_as_float(counts[i]);
+        return bias ? v + bias[i] : v;
     };
-    for (int i = first + tid; i < first + n; i += PEN_THREADS) y[i] = pen_to<T>(change(pen_f32(x[i]), i));
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+        if (tid + k * PEN_THREADS >= body) break;
+        const int i = head + 8 * (tid + k * PEN_THREADS);
+        const uint32_t has = counted ? eight_bits(any, i) : 0u;
+        if (bias || has) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pen_set(e[k].at()[j], change(pen_f32(e[k].at()[j]), i + j, has >> j & 1u));
+        }
+        if (allowed[k] != 0xffu) forbid(e[k], allowed[k]);
+#pragma unroll
+        for (int j = 0; j < Eight<T>::N; ++j) __stcs(reinterpret_cast<uint4 *>(y + i) + j, e[k].v[j]);
+    }
+    if (tid < n - 8 * body) {                                    // at most 7 of the head, 7 of the tail
+        const int i = tid < head ? tid : tid + 8 * body;
+        float v = change(pen_f32(x[i]), i, counted && (any[i / 32] >> (i % 32) & 1u));
+        if (mask && !(mask[i / 32] >> (i % 32) & 1u)) v = -INFINITY;
+        pen_set(y[i], v);
+    }
 }
 
 namespace {
@@ -106,14 +259,16 @@ int launch_penalize(PenaltyArgs a, int32_t rows, cudaStream_t s) {
     int dev = 0, sms = 148;
     CK(cudaGetDevice(&dev));
     CK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    int slices = (a.vocab + 16383) / 16384;
-    while ((int64_t)rows * slices < 4 * sms && a.vocab / slices > 4096) slices *= 2;
-    a.slice = ((a.vocab + slices - 1) / slices + 31) / 32 * 32;
-    slices = (a.vocab + a.slice - 1) / a.slice;
-    if ((int64_t)rows * slices > INT32_MAX) return fail(INS_EBADLEN, "penalties: too many rows in one call");
-    const size_t smem = ((size_t)a.slice + a.slice / 32) * sizeof(uint32_t);
+    // Slices of up to 32 KB of logits, smaller ones where they leave SMs idle.
+    const int64_t least = 4 * (int64_t)sms;
+    a.slice_log2 = sizeof(T) == 4 ? 13 : 14;
+    while (a.slice_log2 > 11 && (int64_t)rows * ((a.vocab - 1 >> a.slice_log2) + 1) < least) --a.slice_log2;
+    a.slices = (a.vocab - 1 >> a.slice_log2) + 1;
+    if ((int64_t)rows * a.slices > INT32_MAX) return fail(INS_EBADLEN, "penalties: too many rows in one call");
+    const size_t slice = (size_t)1 << a.slice_log2;
+    const size_t smem = (slice + slice / 32) * sizeof(uint32_t) + PEN_LIST * sizeof(uint16_t);
     CK(cudaFuncSetAttribute(k_penalize<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    CK(launch_after(k_penalize<T>, (unsigned)(rows * slices), (unsigned)PEN_THREADS, smem, s, a));
+    CK(launch_after(k_penalize<T>, (unsigned)(rows * a.slices), (unsigned)PEN_THREADS, smem, s, a));
     return INS_OK;
 }
 
@@ -144,7 +299,7 @@ extern "C" int ins_penalize(int32_t rows, int32_t vocab, const void *logits, int
         const PenaltyArgs a{logits, out, stride, out_stride, p->tokens, p->drafted, p->tokens_stride,
                             p->drafted_stride, p->lengths, p->prompts, p->of, p->repetition, p->presence,
                             p->frequency, p->bias, reinterpret_cast<const uint32_t *>(p->mask), p->bias_stride,
-                            p->mask_stride, vocab, 0, p->history, p->histories, p->drafted ? p->n_drafted : 0};
+                            p->mask_stride, vocab, 0, 0, p->history, p->histories, p->drafted ? p->n_drafted : 0};
         cudaStream_t s = (cudaStream_t)stream;
         if (dtype == INS_F32) return launch_penalize<float>(a, rows, s);
         if (dtype == INS_F16) return launch_penalize<__half>(a, rows, s);
