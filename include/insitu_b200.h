@@ -487,9 +487,9 @@ int ins_tree_scan(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int
  * a window (window > 0; 0: none) only those of the last `window` positions,
  * its own among them, and the sequence's first `sinks` tokens. A position is a
  * row's place in the cache. Outputs, numerics, buffers and their alignment are
- * ins_tree_scan's; q_rot and out hold sum counts tokens, workspace
- * ins_chunk_workspace bytes for the same cache and arguments (the lengths at
- * the call). Sequences of up to 2^30 tokens; the same sequence may be named
+ * ins_tree_scan's; q_rot and out hold sum counts tokens, workspace (128-byte
+ * aligned) ins_chunk_workspace bytes for the same cache and arguments (the
+ * lengths at the call). Sequences of up to 2^30 tokens; the same sequence may be named
  * several times. Stream-ordered; a bounded wait that gives up latches
  * INS_ETIMEOUT for ins_cache_status. */
 int64_t ins_chunk_workspace(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int32_t *counts,

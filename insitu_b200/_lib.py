@@ -21,7 +21,7 @@ UNITS = {
     "csrc/insitu.cu": COMMON + ("csrc/kernels.cuh", "csrc/scan_chunked.cuh", "csrc/scan_fused.cuh",
                                 "csrc/project.cuh"),
     "csrc/pages.cu": COMMON + ("csrc/plan.cuh",),
-    "csrc/chunk.cu": COMMON + ("csrc/plan.cuh", "csrc/attend.cuh"),
+    "csrc/chunk.cu": COMMON + ("csrc/plan.cuh", "csrc/attend.cuh", "csrc/chunk_tiles.cuh"),
     "csrc/dense.cu": COMMON + ("csrc/plan.cuh",),
     "csrc/penalize.cu": COMMON,
     "csrc/sample.cu": COMMON,

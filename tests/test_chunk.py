@@ -119,6 +119,14 @@ def test_long_contexts(n, groups, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kb,vb", [(4, 2), (2, 4)])
+@pytest.mark.parametrize("context,n,window", [(0, 4500, None), (700, 3300, None), (3000, 2500, 300), (0, 3000, 64)])
+def test_more_row_tiles_than_the_gpu_has_room_for(kb, vb, context, n, window):
+    """Each SM takes many units, of a few tiles and of many."""
+    run(kb, vb, 4, 4, 256, [context, 5], [n, 1200], window=window, sinks=4, seed=n)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [1, 12, 60, 400])
 @pytest.mark.parametrize("scale", [0.0, 4.0, 60.0])
 def test_peaked_and_flat_scores(n, scale):
