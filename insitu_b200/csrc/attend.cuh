@@ -808,6 +808,8 @@ __device__ __forceinline__ void tc_wait_load(uint32_t (&r)[16]) {
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::
                      "memory");
 }
+__device__ __forceinline__ void tc_load(uint32_t (&r)[16], uint32_t at) { tc_load16(r, at); }
+__device__ __forceinline__ void tc_load(uint32_t (&r)[32], uint32_t at) { tc_load32(r, at); }
 __device__ __forceinline__ void tc_store8(uint32_t at, const uint32_t *r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]),
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -866,6 +868,11 @@ __device__ __forceinline__ uint64_t pair64(uint32_t lo, uint32_t hi) {
 __device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
 __device__ __forceinline__ float2 split64(uint64_t v) {

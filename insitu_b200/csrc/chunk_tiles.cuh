@@ -10,11 +10,11 @@
 //
 // k_chunk_tiles: one CTA an SM, persistent, takes units (a row tile of a KV
 // head, or a piece of its KV tiles) from a ticket in order of falling size. One
-// warp loads, one issues the products S = Q K^T and O += P V, two groups of four
-// warps (a stream each, 128 rows, a thread a row) turn S into P. P replaces S in
-// tensor memory, so that there is room for three score buffers of 128 columns
-// next to two outputs of 64: while both streams work on a buffer each, the third
-// already holds the scores of the one that finishes first.
+// warp loads, two groups of eight warps (a stream each: 128 rows, two threads a
+// row) turn S = Q K^T into P, one warp issues the products S and one a stream O +=
+// P V. P replaces S in tensor memory, so that there is room for three score buffers
+// of 128 columns next to two outputs of 64: while both streams work on a buffer
+// each, the third already holds the scores of the one that finishes first.
 #pragma once
 
 #include "attend.cuh"
@@ -52,9 +52,9 @@ struct ChunkView {
 };
 
 constexpr int TL_ROWS = 256, TL_TILE = 128, TL_IMAGE = TL_TILE * 128;      // an image: 128 rows of 64 fp16
-constexpr int TL_STAGES = 4, TL_THREADS = 10 * 32;
+constexpr int TL_STAGES = 4, TL_THREADS = 20 * 32;
 constexpr int TL_Q_AT = 0, TL_KV_AT = 2 * 2 * TL_IMAGE, TL_UNIT_AT = TL_KV_AT + TL_STAGES * 2 * TL_IMAGE;
-constexpr int TL_BARS_AT = TL_UNIT_AT + 128, TL_SMEM = TL_BARS_AT + 256;
+constexpr int TL_HALVES_AT = TL_UNIT_AT + 128, TL_BARS_AT = TL_HALVES_AT + 2048, TL_SMEM = TL_BARS_AT + 256;
 
 struct TilesArgs {
     const DevTables *tb;
@@ -196,43 +196,83 @@ struct TilesUnit {
     int32_t slot;                            // partial slot, -1: all of the row tile's KV tiles
 };
 
-// P = exp2(S - ref) of a row in fp16 pairs, with a factor of 2^7 (as sum has):
-// with LAG it stays below 2^15, and fp16 keeps weights down to 2^-31 of the
-// maximum. True if some row of the warp exceeds its ref by more than LAG (P and
-// sum are then not valid).
+// P = exp2(S - ref) of 64 columns of a row in fp16 pairs, with a factor of 2^7
+// (as sum has). Under the row's own maximum they sum to 2^13 at most; true if
+// they exceed 2^15 (P and sum are then not valid: ref is too low). Up to there
+// every weight is inside fp16, which keeps them down to 2^-31 of the maximum,
+// and no comparison of scores is needed.
 template <bool MASKED, class Row>
-__device__ __forceinline__ bool weigh_row(uint32_t S, float ref, float &sum, uint32_t (&p)[64], const Row &row, int t0) {
+__device__ __forceinline__ bool weigh_half(uint32_t S, float ref, float &sum, uint32_t (&p)[32], const Row &row, int t0) {
     const float sub = (ref > -INFINITY ? -ref : 0.0f) + 7.0f;
     const uint64_t sub2 = pair64(__float_as_uint(sub), __float_as_uint(sub));
-    uint32_t x[2][16];
     uint64_t acc[2] = {0, 0};
-    float top = -INFINITY, top1 = -INFINITY;
-    tc_load16(x[0], S);
-    tc_wait_load(x[0]);
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        uint32_t(&y)[16] = x[c & 1];
-        if (c < 7) tc_load16(x[(c + 1) & 1], S + 16 * (c + 1));
+    for (int c = 0; c < 2; ++c) {
+        uint32_t x[32];
+        tc_load32(x, S + 32 * c);
+        tc_wait_load(x);
         if (MASKED) {
-            const uint32_t see = row.bits(t0 + 16 * c);
+            const uint32_t see = row.bits(t0 + 32 * c);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) y[j] = (see >> j) & 1 ? y[j] : 0xff800000u;
+            for (int j = 0; j < 32; ++j) x[j] = (see >> j) & 1 ? x[j] : 0xff800000u;
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            top = fmaxf(top, __uint_as_float(y[2 * j]));
-            top1 = fmaxf(top1, __uint_as_float(y[2 * j + 1]));
-            const float2 v = split64(add_pair(pair64(y[2 * j], y[2 * j + 1]), sub2));
+        for (int j = 0; j < 16; ++j) {
+            const float2 v = split64(add_pair(pair64(x[2 * j], x[2 * j + 1]), sub2));
             const float e0 = ex2(v.x), e1 = ex2(v.y);
             acc[j & 1] = add_pair(acc[j & 1], pair64(__float_as_uint(e0), __float_as_uint(e1)));
-            p[8 * c + j] = pack_half2(e0, e1);
+            p[16 * c + j] = pack_half2(e0, e1);
         }
-        if (c < 7) tc_wait_load(x[(c + 1) & 1]);
     }
-    top = fmaxf(top, top1);
     const float2 v = split64(add_pair(acc[0], acc[1]));
     sum = v.x + v.y;
-    return __any_sync(FULL, top > ref + LAG);
+    return sum > 32768.0f;
+}
+// The largest of a row's 64 columns that it sees, and of `m`.
+template <class Row>
+__device__ __noinline__ float largest_half(uint32_t S, float m, const Row row, int t0) {
+    uint32_t x[32];
+#pragma unroll 1
+    for (int c = 0; c < 2; ++c) {
+        tc_load32(x, S + 32 * c);
+        tc_wait_load(x);
+        hide<true>(x, row, t0 + 32 * c);
+        m = largest(x, m);
+    }
+    return m;
+}
+// 32 output columns times f.
+__device__ __noinline__ void scale_half(uint32_t O, float f) {
+    uint32_t x[32];
+    tc_load32(x, O);
+    tc_wait_load(x);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(__uint_as_float(x[j]) * f);
+    tc_store16(O, x);
+    tc_store16(O + 16, x + 16);
+    tc_wait_st();
+}
+// True for both warps of a pair if `x` is for one of their threads. They wait
+// for one another: each comes here as often as the other.
+__device__ __forceinline__ bool pair_any(int pair, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{ .reg .pred p, q; setp.ne.u32 p, %1, 0; barrier.cta.red.or.pred q, %2, 64, p; selp.u32 %0, 1, 0, q; }"
+        : "=r"(r)
+        : "r"((uint32_t)x), "r"(1 + pair)
+        : "memory");
+    return r;
+}
+
+// bar_wait of a whole warp: the first look is all that most waits need.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, int phase, int limit) {
+    uint32_t done;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(done)
+                 : "r"(bar), "r"((uint32_t)phase & 1u)
+                 : "memory");
+    if (__all_sync(FULL, done)) return true;
+    return __all_sync(FULL, bar_wait(bar, (uint32_t)phase & 1u, limit));
 }
 
 template <class Src>
@@ -247,27 +287,25 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
     auto kv_empty = [&](int i) { return bars + 32 + 8 * i; };
     auto q_full = [&](int i) { return bars + 64 + 8 * i; };
     auto q_empty = [&](int i) { return bars + 80 + 8 * i; };
-    auto p_ready = [&](int i) { return bars + 96 + 8 * i; };
-    auto pv_done = [&](int i) { return bars + 112 + 8 * i; };
-    // of stream i in score buffer b: one barrier for both would be two phases
-    // ahead of a stream that is late, and a parity does not tell them apart
-    auto s_ready = [&](int i, int b) { return bars + 128 + 8 * (2 * b + i); };
-    const uint32_t fin = bars + 176;
-    volatile uint32_t *tmem_at = reinterpret_cast<uint32_t *>(sm + TL_BARS_AT + 192);
+    // of step k, k % 6: its stream is k % 2, its score buffer k % 3
+    auto s_ready = [&](int k) { return bars + 96 + 8 * k; };
+    auto p_ready = [&](int k) { return bars + 144 + 8 * k; };
+    auto pv_done = [&](int k) { return bars + 192 + 8 * k; };
+    const uint32_t fin = bars + 240;
+    volatile uint32_t *tmem_at = reinterpret_cast<uint32_t *>(sm + TL_BARS_AT + 248);
     TilesUnit *unit_sm = reinterpret_cast<TilesUnit *>(sm + TL_UNIT_AT);
     static_assert(2 * sizeof(TilesUnit) <= 128, "two units");
 
     if (tid == 0) {
-        for (int i = 0; i < TL_STAGES; ++i) bar_init(kv_full(i), 1), bar_init(kv_empty(i), 1);
+        for (int i = 0; i < TL_STAGES; ++i) bar_init(kv_full(i), 1), bar_init(kv_empty(i), 2);
         for (int i = 0; i < 2; ++i) {
-            bar_init(q_full(i), 1), bar_init(q_empty(i), 9);
-            bar_init(p_ready(i), 4), bar_init(pv_done(i), 1);
-            for (int b = 0; b < 3; ++b) bar_init(s_ready(i, b), 1);
+            bar_init(q_full(i), 1), bar_init(q_empty(i), 19);
         }
-        bar_init(fin, 1);
+        for (int k = 0; k < 6; ++k) bar_init(s_ready(k), 1), bar_init(p_ready(k), 8), bar_init(pv_done(k), 1);
+        bar_init(fin, 3);
         bar_init_fence();
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32((void *)tmem_at))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -280,7 +318,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
     if (*tmem_at != tmem || (sm0 & 1023)) {          // never: reported, not worked around
         if (tid == 0) atomicOr(a.status, ST_INTERNAL);
         __syncthreads();
-        if (warp == 8)
+        if (warp == 16)
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(*tmem_at) : "memory");
         return;
     }
@@ -288,18 +326,17 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
 
     bool lost = false;                               // a wait gave up: the same for all lanes of a warp
     auto wait = [&](uint32_t bar, int phase) {
-        if (!lost && !bar_wait(bar, (uint32_t)phase & 1u, a.poll_limit)) {
+        if (!warp_wait(bar, phase, a.poll_limit)) {
             lost = true;
-            atomicOr(a.status, ST_TIMEOUT);
+            if (lane == 0) atomicOr(a.status, ST_TIMEOUT);
         }
-        lost = __any_sync(FULL, lost);
     };
 
-    if (warp == 9) {
+    if (warp == 19) {
         // ---- loads
         const ChunkSeq *seqs = reinterpret_cast<const ChunkSeq *>(src.data());
         int kt = 0, n = 0;                           // KV tiles, units so far
-        for (;; ++n) {
+        for (;;) {
             int u = 0;
             if (lane == 0) u = atomicAdd(a.ticket, 1);
             u = __shfl_sync(FULL, u, 0);
@@ -319,6 +356,11 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
             const int head = item % g.n_kv, rt = sq.rts - 1 - item / g.n_kv;
             const RowTile t = row_tile(view, sq, g.H, rt);
             const int lo = (int)((int64_t)t.tiles * piece / sq.splits), hi = (int)((int64_t)t.tiles * (piece + 1) / sq.splits);
+            if (lo == hi) {                          // a piece of a row tile of few tiles: nothing
+                for (int r = lane; r < TL_ROWS; r += 32)
+                    *reinterpret_cast<float2 *>(a.ml + ((int64_t)u * TL_ROWS + r) * 2) = make_float2(-INFINITY, 0.0f);
+                continue;
+            }
             if (lane == 0) {
                 TilesUnit &w = unit_sm[slot];
                 w.end = 0;
@@ -345,98 +387,86 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
                 }
                 __syncwarp();
             }
+            ++n;
             if (lost) break;
         }
         // copies in flight land before the CTA goes
         if (lost) {
             for (int k = max(0, kt - TL_STAGES); k < kt; ++k)
                 bar_wait(kv_full(k % TL_STAGES), (k / TL_STAGES) & 1, a.poll_limit);
-            for (int k = max(0, n - 1); k <= n; ++k) bar_wait(q_full(k & 1), (k / 2) & 1, a.poll_limit);
+            for (int k = max(0, n - 2); k < n; ++k) bar_wait(q_full(k & 1), (k / 2) & 1, a.poll_limit);
         }
-    } else if (warp == 8) {
-        // ---- products. All lanes walk the same steps, one elected lane issues.
-        // Step k (of all units, one after another) is stream k % 2's of a KV tile
-        // and uses score buffer k % 3. Score products run up to three steps ahead
-        // of value products, into the next unit at most (whose queries are there
-        // while this one's are).
-        constexpr uint32_t iqk = tc_idesc(128, false), ipv = tc_idesc(64, true);
-        const uint64_t q_desc = tc_desc(sm0 + TL_Q_AT), k_desc = tc_desc(sm0 + TL_KV_AT),
-                       v_desc = tc_desc(sm0 + TL_KV_AT + TL_IMAGE);
-        int qn = 0, qs = 0, qk = 0, q_tile = 0;      // score products: unit, step in it, step, KV tile
-        int pn = 0, pk = 0, p_tile = 0;              // value products: unit, step, KV tile
-        int steps[2] = {0, 0};                       // of unit n, at n % 2
-        int seen[2] = {0, 0};                        // value products of a stream that are known to be done
-        bool open = false, end = false;
-        auto pv_wait = [&](int k) {                  // until step k's value product is done
-            const int i = k & 1;
-            if ((i ? seen[1] : seen[0]) > (k >> 1)) return;
-            wait(pv_done(i), k >> 1);
-            if (i) seen[1] = (k >> 1) + 1;
-            else seen[0] = (k >> 1) + 1;
-        };
-        auto feed = [&] {
-            while (!lost && !end && qn <= pn + 1 && qk < pk + 3) {
-                if (!open) {
-                    wait(q_full(qn & 1), qn >> 1);
-                    if (lost) return;
-                    const volatile TilesUnit *w = unit_sm + (qn & 1);
-                    end = __shfl_sync(FULL, w->end, 0) != 0;
-                    if (end) return;
-                    const int s = __shfl_sync(FULL, 2 * (w->hi - w->lo), 0);
-                    if (qn & 1) steps[1] = s;
-                    else steps[0] = s;
-                    open = true;
-                    qs = 0;
-                }
-                if (qs == ((qn & 1) ? steps[1] : steps[0])) {
-                    if (elect_one()) tc_commit(q_empty(qn & 1));
-                    __syncwarp();
-                    open = false;
-                    ++qn;
-                    continue;
-                }
-                const int i = qs & 1, b = qk % 3, st = q_tile % TL_STAGES;
-                if (i == 0) wait(kv_full(st), q_tile / TL_STAGES);
-                if (qk >= 3) pv_wait(qk - 3);
-                if (lost) return;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t q = q_desc + (uint64_t)((2 * (qn & 1) + i) * (TL_IMAGE >> 4));
+    } else if (warp >= 16) {
+        // ---- products: one warp issues the score products, one a stream its value
+        // products. All lanes walk the same steps, one elected lane issues. Step k
+        // (of all units, one after another) is stream k % 2's of a KV tile and uses
+        // score buffer k % 3.
+        int kt = 0, k6 = 0, use = 0;                 // KV tiles so far; the next step: k % 6, k / 6
+        if (warp == 16) {
+            constexpr uint32_t idesc = tc_idesc(128, false);
+            const uint64_t q_desc = tc_desc(sm0 + TL_Q_AT), k_desc = tc_desc(sm0 + TL_KV_AT);
+            for (int n = 0; !lost; ++n) {
+                wait(q_full(n & 1), n >> 1);
+                if (lost) break;
+                const TilesUnit un = unit_sm[n & 1];
+                if (un.end) break;
+                const uint64_t q = q_desc + (uint64_t)((n & 1) * (2 * TL_IMAGE >> 4));
+                for (int j = un.lo; j < un.hi && !lost; ++j, ++kt) {
+                    const int st = kt % TL_STAGES;
+                    wait(kv_full(st), kt / TL_STAGES);
                     const uint64_t k = k_desc + (uint64_t)(st * (2 * TL_IMAGE >> 4));
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) tc_mma_ss(tmem + 128 * b, q + 2 * x, k + 2 * x, iqk, x > 0);
-                    tc_commit(s_ready(i, b));
-                }
-                __syncwarp();
-                ++qs, ++qk;
-                q_tile += i;
-            }
-        };
-        for (;; ++pn) {
-            feed();
-            if (lost || (end && pn == qn)) break;
-            const int all = (pn & 1) ? steps[1] : steps[0];
-            for (int s = 0; s < all && !lost; ++s) {
-                feed();
-                if (lost) break;
-                const int i = s & 1, b = pk % 3, st = p_tile % TL_STAGES;
-                if (pk >= 2) pv_wait(pk - 2);
-                wait(p_ready(i), pk >> 1);
-                if (lost) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t v = v_desc + (uint64_t)(st * (2 * TL_IMAGE >> 4));
+                    for (int i = 0; i < 2; ++i) {
+                        // its buffer's last step was k - 3
+                        if (!lost && (use || k6 >= 3)) wait(pv_done(k6 >= 3 ? k6 - 3 : k6 + 3), k6 >= 3 ? use : use - 1);
+                        if (lost) break;
+                        tc_fence_after();
+                        if (elect_one()) {
 #pragma unroll
-                    for (int x = 0; x < 8; ++x)
-                        tc_mma_ts(tmem + 384 + 64 * i, tmem + 128 * b + 8 * x, v + 128 * x, ipv, s >= 2 || x > 0);
-                    if (i == 1) tc_commit(kv_empty(st));
-                    tc_commit(pv_done(i));
+                            for (int x = 0; x < 4; ++x)
+                                tc_mma_ss(tmem + 128 * (k6 % 3), q + (uint64_t)(i * (TL_IMAGE >> 4)) + 2 * x, k + 2 * x, idesc,
+                                          x > 0);
+                            tc_commit(s_ready(k6));
+                        }
+                        __syncwarp();
+                        k6 = k6 == 5 ? 0 : k6 + 1;
+                        use += k6 == 0;
+                    }
                 }
+                if (elect_one()) tc_commit(q_empty(n & 1));
                 __syncwarp();
-                ++pk;
-                p_tile += i;
             }
-            if (lost) break;
+        } else {
+            const int i = warp - 17;
+            constexpr uint32_t idesc = tc_idesc(64, true);
+            const uint64_t v_desc = tc_desc(sm0 + TL_KV_AT + TL_IMAGE);
+            k6 = i;
+            for (int n = 0; !lost; ++n) {
+                wait(q_full(n & 1), n >> 1);
+                if (lost) break;
+                const TilesUnit un = unit_sm[n & 1];
+                if (un.end) break;
+                for (int j = un.lo; j < un.hi && !lost; ++j, ++kt) {
+                    const int st = kt % TL_STAGES;
+                    wait(kv_full(st), kt / TL_STAGES);
+                    if (!lost) wait(p_ready(k6), use);
+                    if (lost) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t v = v_desc + (uint64_t)(st * (2 * TL_IMAGE >> 4));
+#pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            tc_mma_ts(tmem + 384 + 64 * i, tmem + 128 * (k6 % 3) + 8 * x, v + 128 * x, idesc,
+                                      j > un.lo || x > 0);
+                        tc_commit(pv_done(k6));
+                        tc_commit(kv_empty(st));
+                    }
+                    __syncwarp();
+                    k6 = k6 >= 4 ? k6 - 4 : k6 + 2;
+                    use += k6 < 2;
+                }
+                if (lane == 0) bar_arrive(q_empty(n & 1));
+            }
         }
         // nothing may be in flight when the tensor memory goes
         if (elect_one()) tc_commit(fin);
@@ -444,14 +474,20 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
         if (!bar_wait(fin, 0, WAIT_POLLS)) atomicOr(a.status, ST_TIMEOUT);
         __syncwarp();
     } else {
-        // ---- softmax: thread `row` of stream `i` owns one query row
-        const int i = warp / 4, row = tid - 128 * i;
+        // ---- softmax: of a query row (`row` of stream `i`) two threads own 64
+        // columns of scores each (half `h`), so that four warps of each scheduler
+        // hide one another's latencies. A wait that gave up is known to both warps
+        // of a pair at their next meeting, where they leave together.
+        const int i = warp / 8, h = warp / 4 % 2, row = tid % 128, pair = 4 * i + warp % 4;
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;   // lane 32 (warp % 4), in bits 16 up
-        const uint32_t O = tmem + lanes + 384 + 64 * i;
-        int m = 0, b = i;                                    // this stream's steps so far; the next one's buffer
-        for (int n = 0; !lost; ++n) {
+        const uint32_t O = tmem + lanes + 384 + 64 * i + 32 * h;
+        float *const mine = reinterpret_cast<float *>(sm + TL_HALVES_AT) + (2 * i + h) * 128 + row;
+        float *const other = reinterpret_cast<float *>(sm + TL_HALVES_AT) + (2 * i + 1 - h) * 128 + row;
+        int k6 = i, use = 0;                                 // the stream's next step k: k % 6, k / 6
+        int last = 0, last_use = 0;                          // its last one
+        for (int n = 0;; ++n) {
             wait(q_full(n & 1), n >> 1);
-            if (lost) break;
+            if (pair_any(pair, lost)) break;
             const TilesUnit un = unit_sm[n & 1];
             if (un.end) break;
             const int r = 128 * i + row;
@@ -459,68 +495,72 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
             const int p = min(un.p_lo + r / g.H, un.p_hi);
             const ChunkView::Row sees{p, p + 1 - view.window, view.sinks};
             float ref = -INFINITY, l = 0.0f;
-            for (int j = un.lo; j < un.hi && !lost; ++j, ++m) {
-                const int t0 = (j < un.early ? j : j + un.jump) * TL_TILE;
-                const uint32_t S = tmem + lanes + 128 * b;
-                wait(s_ready(i, b), m / 3);          // step 2 m + i, its buffer's every sixth
-                b = b == 0 ? 2 : b - 1;
-                if (lost) break;
+            bool left = false;
+            for (int j = un.lo; j < un.hi; ++j) {
+                const int tile = (j < un.early ? j : j + un.jump) * TL_TILE, t0 = tile + 64 * h;
+                const bool whole = tile + TL_TILE - 1 <= un.p_lo &&
+                                   (tile > un.p_hi - view.window || tile + TL_TILE <= view.sinks);
+                const uint32_t S = tmem + lanes + 128 * (k6 % 3);
+                wait(s_ready(k6), use);
                 tc_fence_after();
-                // O is this stream's again once its last value product is done
-                bool have = m == 0;
-                auto o_free = [&] {
-                    if (!have) wait(pv_done(i), m - 1);
-                    have = true;
-                };
                 if (any_row) {
                     float sum = 0.0f;
-                    uint32_t w[64];
-                    auto step = [&](auto masked) {
-                        constexpr bool M = decltype(masked)::value;
-                        // the exponentials are taken under the maximum so far, and
-                        // again in the rare case that it was too low
-                        bool over = true;
-                        if (j > un.lo) over = weigh_row<M>(S, ref, sum, w, sees, t0);
-                        if (over) {
-                            o_free();
-                            tc_fence_after();
-                            raise<M>(S, O, j > un.lo, ref, l, sees, t0);
-                            weigh_row<M>(S, ref, sum, w, sees, t0);
-                        }
+                    uint32_t w[32];
+                    bool over = lost || j == un.lo;
+                    auto weigh = [&] {
+                        if (whole) over |= weigh_half<false>(S + 64 * h, ref, sum, w, sees, t0);
+                        else over |= weigh_half<true>(S + 64 * h, ref, sum, w, sees, t0);
                     };
-                    if (t0 + TL_TILE - 1 <= un.p_lo && (t0 > un.p_hi - view.window || t0 + TL_TILE <= view.sinks))
-                        step(std::false_type());
-                    else step(std::true_type());
+                    // the exponentials are taken under the maximum so far, and again in
+                    // the rare case that it was too low
+                    if (!over) weigh();
+                    if (pair_any(pair, over)) {
+                        // O is this stream's once its last value product is done
+                        if (j > un.lo && !lost) wait(pv_done(last), last_use);
+                        tc_fence_after();
+                        if (pair_any(pair, lost)) {
+                            left = true;
+                            break;
+                        }
+                        *mine = largest_half(S + 64 * h, ref, sees, t0);
+                        pair_any(pair, false);
+                        const float now = fmaxf(*mine, *other), f = now > -INFINITY ? ex2(ref - now) : 1.0f;
+                        ref = now;
+                        l *= f;
+                        if (j > un.lo) scale_half(O, f);
+                        weigh();
+                        pair_any(pair, false);               // all scores have been read: P may replace them
+                    }
                     l += sum;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tc_store16(S + 16 * c, w + 16 * c);
+                    tc_store16(S + 32 * h, w);
+                    tc_store16(S + 32 * h + 16, w + 16);
                     tc_wait_st();
+                } else if (lost) {
+                    left = true;
+                    break;
                 }
-                o_free();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(p_ready(i));
+                if (lane == 0) bar_arrive(p_ready(k6));
+                last = k6, last_use = use;
+                k6 = k6 >= 4 ? k6 - 4 : k6 + 2;
+                use += k6 < 2;
             }
-            if (lost) break;
-            if (un.hi > un.lo) wait(pv_done(i), m - 1);
-            if (lost) break;
+            // (warps without rows meet nowhere in the loop)
+            if (!left && !lost) wait(pv_done(last), last_use);
+            *mine = l;
+            if (pair_any(pair, left || lost)) break;
+            l += *other;
             tc_fence_after();
-            // this row's sums out
-#pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-                uint32_t x[32];
-                if (un.hi > un.lo) {
-                    tc_load32(x, O + 32 * c);
-                    tc_wait_load(x);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) x[k] = 0;
-                }
-                if (r >= un.rows) continue;
+            // this row's sums out, 32 channels each half
+            uint32_t x[32];
+            tc_load32(x, O);
+            tc_wait_load(x);
+            if (r < un.rows) {
                 if (un.slot < 0) {
                     const float inv = a.out_unit / l;        // (every row sees itself)
                     uint4 *dst = reinterpret_cast<uint4 *>(
-                        a.out + (((int64_t)(un.node0 + un.first + r / g.H) * g.n_kv + un.head) * g.H + r % g.H) * D + 32 * c);
+                        a.out + (((int64_t)(un.node0 + un.first + r / g.H) * g.n_kv + un.head) * g.H + r % g.H) * D + 32 * h);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         uint32_t o[4];
@@ -534,10 +574,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
                     }
                 } else {
                     const int64_t at = (int64_t)un.slot * TL_ROWS + r;
-                    uint4 *dst = reinterpret_cast<uint4 *>(a.acc + at * 64 + 32 * c);
+                    uint4 *dst = reinterpret_cast<uint4 *>(a.acc + at * 64 + 32 * h);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) dst[k] = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
-                    if (c == 0) a.ml[at * 2] = ref, a.ml[at * 2 + 1] = l;
+                    if (h == 0) a.ml[at * 2] = ref, a.ml[at * 2 + 1] = l;
                 }
             }
             tc_fence_before();
@@ -546,7 +586,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
         }
     }
     __syncthreads();
-    if (warp == 8)
+    if (warp == 16)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
@@ -588,6 +628,7 @@ __global__ void __launch_bounds__(128) k_chunk_join(Geo g, TilesArgs a, ChunkVie
 #pragma unroll 8
         for (int s = 0; s < splits; ++s) {
             const float f = wt[r * splits + s];
+            if (f == 0.0f) continue;                 // (a piece of no tiles has written no sums)
             const float4 v = reinterpret_cast<const float4 *>(a.acc)[slot(s, r) * 16 + c4];
             o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
         }
