@@ -45,8 +45,10 @@ ChunkSeq walk_of(const ChunkView &v, int32_t seq, int64_t len, int32_t n, int64_
 
 // Row tiles, units and pieces of k_chunk_tiles. Units are whole row tiles unless
 // that leaves SMs idle: a row tile's KV tiles are then cut so that the units
-// fill rounds of one an SM evenly, counting two tiles' time for what a unit
-// costs besides its tiles.
+// fill rounds of one an SM evenly. Counted in KV tiles' times (1.26 us measured):
+// what a unit costs besides its tiles (4.5), and the join of pieces (1,024 units:
+// 44 us).
+constexpr double UNIT_TILES = 4.5, JOIN_TILES = 0.034;
 int cut_tiles(const Geo &g, const ChunkView &v, int sms, ChunkPlan &p) {
     std::sort(p.seqs.begin(), p.seqs.end(), [](const ChunkSeq &a, const ChunkSeq &b) {
         return a.context + a.nodes != b.context + b.nodes ? a.context + a.nodes > b.context + b.nodes : a.node0 < b.node0;
@@ -75,8 +77,8 @@ int cut_tiles(const Geo &g, const ChunkView &v, int sms, ChunkPlan &p) {
         double n = 0;
         for (size_t i = 0; i < p.seqs.size(); ++i)
             n += (double)p.seqs[i].rts * g.n_kv * (double)((most[i] + size - 1) / size);
-        const double rounds = std::ceil(n / sms), each = work / n + 2.0;
-        const double time = std::max(rounds * each, (double)(size + 2));
+        const double rounds = std::ceil(n / sms), each = work / n + UNIT_TILES;
+        const double time = std::max(rounds * each, size + UNIT_TILES) + (k > 1 ? n * JOIN_TILES : 0.0);
         if (k == 1 || time < 0.97 * best) best = time, piece = size;
     }
     for (size_t i = 0; i < p.seqs.size(); ++i) {

@@ -56,6 +56,8 @@ constexpr int TL_STAGES = 4, TL_THREADS = 20 * 32;
 constexpr int TL_Q_AT = 0, TL_KV_AT = 2 * 2 * TL_IMAGE, TL_UNIT_AT = TL_KV_AT + TL_STAGES * 2 * TL_IMAGE;
 constexpr int TL_HALVES_AT = TL_UNIT_AT + 128, TL_BARS_AT = TL_HALVES_AT + 2048, TL_SMEM = TL_BARS_AT + 256;
 
+constexpr int TL_POLY = 4;
+
 struct TilesArgs {
     const DevTables *tb;
     const uint8_t *pool;
@@ -196,16 +198,43 @@ struct TilesUnit {
     int32_t slot;                            // partial slot, -1: all of the row tile's KV tiles
 };
 
+// 2^v of two values by additions and multiplications: the special function unit
+// makes 16 exponentials a clock and SM, and bounds the kernel where it makes all.
+// With n the integer nearest to v and f = v - n, 2^f is a polynomial of degree
+// 3 (of least largest relative error on [-1/2, 1/2]: 2^-13.7, below P's rounding
+// to fp16, and the same in P and in its sum), and n is added to the exponent's
+// bits: for |v| up to 126.
+constexpr float POLY0 = 0.9999280571937561f, POLY1 = 0.6932609677314758f, POLY2 = 0.2426111251115799f,
+                POLY3 = 0.0551716685295105f, POLY_RANGE = 126.0f;
+__device__ __forceinline__ float2 exp2_pair(uint64_t v) {
+    auto both = [](float c) { return pair64(__float_as_uint(c), __float_as_uint(c)); };
+    const uint64_t t = add_pair(v, both(12582912.0f));           // 1.5 * 2^23: n in the low bits
+    const uint64_t f = fma_pair(add_pair(t, both(-12582912.0f)), both(-1.0f), v);
+    uint64_t r = fma_pair(f, both(POLY3), both(POLY2));
+    r = fma_pair(r, f, both(POLY1));
+    r = fma_pair(r, f, both(POLY0));
+    const float2 n = split64(t), y = split64(r);
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)),
+                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // P = exp2(S - ref) of 64 columns of a row in fp16 pairs, with a factor of 2^7
 // (as sum has). Under the row's own maximum they sum to 2^13 at most; true if
-// they exceed 2^15 (P and sum are then not valid: ref is too low). Up to there
-// every weight is inside fp16, which keeps them down to 2^-31 of the maximum,
-// and no comparison of scores is needed.
-template <bool MASKED, class Row>
+// they exceed 2^15, or a polynomial's range (P and sum are then not valid).
+// Up to there every weight is inside fp16, which keeps them down to 2^-31 of
+// the maximum, and no comparison of all scores is needed. POLY of 16 pairs go by
+// polynomials.
+template <bool MASKED, int POLY, class Row>
 __device__ __forceinline__ bool weigh_half(uint32_t S, float ref, float &sum, uint32_t (&p)[32], const Row &row, int t0) {
     const float sub = (ref > -INFINITY ? -ref : 0.0f) + 7.0f;
     const uint64_t sub2 = pair64(__float_as_uint(sub), __float_as_uint(sub));
     uint64_t acc[2] = {0, 0};
+    float far = 0.0f;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         uint32_t x[32];
@@ -218,15 +247,22 @@ __device__ __forceinline__ bool weigh_half(uint32_t S, float ref, float &sum, ui
         }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const float2 v = split64(add_pair(pair64(x[2 * j], x[2 * j + 1]), sub2));
-            const float e0 = ex2(v.x), e1 = ex2(v.y);
-            acc[j & 1] = add_pair(acc[j & 1], pair64(__float_as_uint(e0), __float_as_uint(e1)));
-            p[16 * c + j] = pack_half2(e0, e1);
+            const uint64_t v2 = add_pair(pair64(x[2 * j], x[2 * j + 1]), sub2);
+            const float2 v = split64(v2);
+            float2 e;
+            if (j * POLY / 16 != (j + 1) * POLY / 16) {
+                e = exp2_pair(v2);
+                far = max3(far, fabsf(v.x), fabsf(v.y));
+            } else {
+                e = make_float2(ex2(v.x), ex2(v.y));
+            }
+            acc[j & 1] = add_pair(acc[j & 1], pair64(__float_as_uint(e.x), __float_as_uint(e.y)));
+            p[16 * c + j] = pack_half2(e.x, e.y);
         }
     }
     const float2 v = split64(add_pair(acc[0], acc[1]));
     sum = v.x + v.y;
-    return sum > 32768.0f;
+    return sum > 32768.0f || (POLY && far > POLY_RANGE);
 }
 // The largest of a row's 64 columns that it sees, and of `m`.
 template <class Row>
@@ -496,24 +532,27 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
             const ChunkView::Row sees{p, p + 1 - view.window, view.sinks};
             float ref = -INFINITY, l = 0.0f;
             bool left = false;
+            // KV tiles that all rows see whole: those below `held` (of sinks), and from
+            // `whole0` to below `whole1`
+            const int held = min(view.sinks / TL_TILE, un.early), at_hi = un.p_hi - view.window;
+            const int whole0 = max(at_hi < 0 ? 0 : at_hi / TL_TILE + 1 - un.jump, un.early);
+            const int whole1 = (un.p_lo + 1) / TL_TILE - un.jump;
             for (int j = un.lo; j < un.hi; ++j) {
-                const int tile = (j < un.early ? j : j + un.jump) * TL_TILE, t0 = tile + 64 * h;
-                const bool whole = tile + TL_TILE - 1 <= un.p_lo &&
-                                   (tile > un.p_hi - view.window || tile + TL_TILE <= view.sinks);
-                const uint32_t S = tmem + lanes + 128 * (k6 % 3);
+                const int t0 = (j < un.early ? j : j + un.jump) * TL_TILE + 64 * h;
+                const bool whole = j < held || (j >= whole0 && j < whole1);
+                const uint32_t S = tmem + lanes + 128 * (k6 >= 3 ? k6 - 3 : k6);
                 wait(s_ready(k6), use);
                 tc_fence_after();
                 if (any_row) {
                     float sum = 0.0f;
                     uint32_t w[32];
                     bool over = lost || j == un.lo;
-                    auto weigh = [&] {
-                        if (whole) over |= weigh_half<false>(S + 64 * h, ref, sum, w, sees, t0);
-                        else over |= weigh_half<true>(S + 64 * h, ref, sum, w, sees, t0);
-                    };
                     // the exponentials are taken under the maximum so far, and again in
                     // the rare case that it was too low
-                    if (!over) weigh();
+                    if (!over) {
+                        if (whole) over = weigh_half<false, TL_POLY>(S + 64 * h, ref, sum, w, sees, t0);
+                        else over = weigh_half<true, 0>(S + 64 * h, ref, sum, w, sees, t0);
+                    }
                     if (pair_any(pair, over)) {
                         // O is this stream's once its last value product is done
                         if (j > un.lo && !lost) wait(pv_done(last), last_use);
@@ -528,7 +567,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
                         ref = now;
                         l *= f;
                         if (j > un.lo) scale_half(O, f);
-                        weigh();
+                        weigh_half<true, 0>(S + 64 * h, ref, sum, w, sees, t0);
                         pair_any(pair, false);               // all scores have been read: P may replace them
                     }
                     l += sum;
