@@ -55,6 +55,7 @@ struct AttendSeq {
 //     .sees(p)               whether it attends position p
 //     .bits(p)               the same of positions p to p + 31, a bit each
 //   whole(sq, p, n)          every new token attends positions p to p + n - 1
+//   SHARES                   k_attend_few may take four units a CTA
 struct AttendArgs {
     const DevTables *tb;
     const uint8_t *pool;
@@ -63,10 +64,11 @@ struct AttendArgs {
     __nv_bfloat16 *out;
     float *acc, *ml;                         // partials: [unit][rows][64], [unit][rows][2]
     int32_t *status;
-    int32_t n_seqs, chunk, row_tiles_rows;
+    int32_t n_seqs, units, chunk, row_tiles_rows;
     int32_t poll_limit, hold_cta, hold_tile; // tests: the tile whose copies are announced too large
     // what the products' fixed units leave to the formats: for the scores (k_attend_many: its two factors), the outputs
     float score_unit, q_scale, k_scale, out_unit;
+    float k_unit, v_unit;                    // factors of the centroids before their rounding to fp16 (the others undo them)
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
@@ -228,8 +230,14 @@ struct FewLayout {
     }
 };
 
-template <int KB, int VB, int MT, bool HALF, int NW, class View, class Src>
+// A CTA's warps work on one unit, or (SHARE) on four, a quarter of them each:
+// where there are more units than SMs, the tables, the start and the join are
+// then paid for once for four. 64 sequences of 4,224 tokens, one token each (512
+// units): 84 us by one unit a CTA, 46 by four.
+template <int KB, int VB, int MT, bool HALF, int NW, int SHARE, class View, class Src>
 __global__ void __launch_bounds__(NW * 32, 1) k_attend_few(Geo g, AttendArgs a, View view, const __grid_constant__ Src src) {
+    constexpr int UW = NW / SHARE;                   // warps of a unit
+    static_assert(UW * SHARE == NW, "every unit has as many warps");
     using L = FewLayout<KB, VB>;
     constexpr int R = 16 * MT;                       // rows of this CTA's tile
     constexpr int HR = HALF ? 1 : 2;                 // of a query fragment's two row halves, those that hold queries
@@ -246,8 +254,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attend_few(Geo g, AttendArgs a, 
     const float cunit = exp2f((float)-g.centroid_frac);
     if (L::PAIRS) {
         float *cent = reinterpret_cast<float *>(sm + L::stages_at(NW));
-        if (tid < (1 << KB)) cent[tid] = (float)a.tb->k_cent[tid] * cunit;
-        if (tid >= 32 && tid < 32 + (1 << VB)) cent[tid] = (float)a.tb->v_cent[tid - 32] * cunit;
+        if (tid < (1 << KB)) cent[tid] = (float)a.tb->k_cent[tid] * cunit * a.k_unit;
+        if (tid >= 32 && tid < 32 + (1 << VB)) cent[tid] = (float)a.tb->v_cent[tid - 32] * cunit * a.v_unit;
         __syncthreads();
         for (int e = warp; e < L::K_ENTRIES; e += NW)
             reinterpret_cast<uint32_t *>(sm)[e * (L::WIDE ? 64 : 32) + lane] =
@@ -264,7 +272,8 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attend_few(Geo g, AttendArgs a, 
     } else {
         __half *tab = reinterpret_cast<__half *>(sm);
         for (int i = tid; i < 512; i += NW * 32)
-            tab[i] = __float2half_rn((float)(i < 256 ? a.tb->k_cent[i] : a.tb->v_cent[i - 256]) * cunit);
+            tab[i] = __float2half_rn(i < 256 ? (float)a.tb->k_cent[i] * cunit * a.k_unit
+                                           : (float)a.tb->v_cent[i - 256] * cunit * a.v_unit);
     }
     if (lane == 0)
         for (int i = 0; i < STAGES; ++i) bar_init(bars + i * 8, 1);
@@ -275,15 +284,18 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attend_few(Geo g, AttendArgs a, 
 
     using Seq = typename View::Seq;
     const Seq *seqs = reinterpret_cast<const Seq *>(src.data());
-    const Seq sq = seqs[find_seq<false>(seqs, a.n_seqs, blockIdx.x)];
+    const int uw = SHARE > 1 ? warp % UW : warp, unit_at = (int)blockIdx.x * SHARE + (SHARE > 1 ? warp / UW : 0);
+    const bool idle = SHARE > 1 && unit_at >= a.units;       // (of the last CTA)
+    const int the_unit = idle ? a.units - 1 : unit_at;
+    const Seq sq = seqs[find_seq<false>(seqs, a.n_seqs, the_unit)];
     const int G = g.H, rows_all = sq.nodes * G, tiles = (rows_all + R - 1) / R;
-    int unit = blockIdx.x - sq.unit0;
+    int unit = the_unit - sq.unit0;
     const int head = unit % g.n_kv;
     unit /= g.n_kv;
     const int rt = unit % tiles, split = unit / tiles;
     const int row0 = rt * R, len = view.span(sq);
     const int lo = split * a.chunk, hi = min(len, lo + a.chunk);
-    const int n_tiles = (hi - lo + FEW_TILE - 1) / FEW_TILE;
+    const int n_tiles = idle ? 0 : (hi - lo + FEW_TILE - 1) / FEW_TILE;
 
     // query fragments: rows g8 and g8 + 8 of each 16; k pairs (2 t4, +1) and
     // (+8, +9) of step ks hold channels 16 t4 + 4 ks + {0, 1} and + {2, 3}
@@ -307,7 +319,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attend_few(Geo g, AttendArgs a, 
 
     // copies of tile j of this CTA into the ring slot of this warp's n-th tile
     auto issue = [&](int n) {
-        const int j = warp + n * NW;
+        const int j = uw + n * UW;
         if (j >= n_tiles) return;
         const int i0 = lo + j * FEW_TILE, p0 = view.at(sq, i0), rows16 = (min(FEW_TILE, hi - i0) + 15) & ~15;
         const uint32_t bar = bars + (n % STAGES) * 8, dst = ring + (n % STAGES) * stage;
@@ -347,7 +359,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attend_few(Geo g, AttendArgs a, 
     int issued = 0;
     for (; issued < STAGES - 1; ++issued) issue(issued);
     int n = 0;
-    for (int j = warp; j < n_tiles; j += NW, ++n) {
+    for (int j = uw; j < n_tiles; j += UW, ++n) {
         __syncwarp();                                 // every lane has read the slot's previous tile
         issue(issued++);
         // the lanes poll one by one: the warp gives up as one, as what follows
@@ -611,7 +623,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attend_few(Geo g, AttendArgs a, 
         // report it, and let the copies in flight land before the CTA goes
         if (lane == 0) atomicOr(a.status, ST_TIMEOUT);
         for (int k = n; k < issued; ++k)
-            if (warp + k * NW < n_tiles) bar_wait(bars + (k % STAGES) * 8, (k / STAGES) & 1, a.poll_limit);
+            if (uw + k * UW < n_tiles) bar_wait(bars + (k % STAGES) * 8, (k / STAGES) & 1, a.poll_limit);
     }
 
     // join the warps: each row's maximum, then the scaled sums
@@ -650,20 +662,20 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attend_few(Geo g, AttendArgs a, 
     }
     __syncthreads();
     constexpr int ROWS = HALF ? 8 : R;
-    const int used = min(NW, n_tiles);
-    for (int i = tid; i < ROWS * 16; i += NW * 32) {
+    const int used = min(UW, n_tiles), warp0 = warp - uw;    // the unit's warps with sums, from warp0 on
+    for (int i = tid - 32 * warp0; i < ROWS * 16 && !idle; i += UW * 32) {
         const int r = i / 16, c4 = i % 16;
         if (row0 + r >= rows_all) continue;
         float M = -INFINITY;
-        for (int w = 0; w < used; ++w) M = fmaxf(M, jml[(w * R + r) * 2]);
+        for (int w = 0; w < used; ++w) M = fmaxf(M, jml[((warp0 + w) * R + r) * 2]);
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         float sum = 0.0f;
         if (M > -INFINITY)
             for (int w = 0; w < used; ++w) {
-                const float f = ex2(jml[(w * R + r) * 2] - M);
-                const float4 v = reinterpret_cast<const float4 *>(jacc)[(w * R + r) * 16 + c4];
+                const float f = ex2(jml[((warp0 + w) * R + r) * 2] - M);
+                const float4 v = reinterpret_cast<const float4 *>(jacc)[((warp0 + w) * R + r) * 16 + c4];
                 o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
-                sum += f * jml[(w * R + r) * 2 + 1];
+                sum += f * jml[((warp0 + w) * R + r) * 2 + 1];
             }
         if (sq.splits == 1) {
             const float inv = sum > 0.0f ? a.out_unit / sum : 0.0f;   // a row that sees nothing is zero
@@ -673,7 +685,7 @@ __global__ void __launch_bounds__(NW * 32, 1) k_attend_few(Geo g, AttendArgs a, 
             dst[0] = __floats2bfloat162_rn(o.x * inv, o.y * inv);
             dst[1] = __floats2bfloat162_rn(o.z * inv, o.w * inv);
         } else {
-            const int64_t at = (int64_t)blockIdx.x * a.row_tiles_rows + r;
+            const int64_t at = (int64_t)the_unit * a.row_tiles_rows + r;
             reinterpret_cast<float4 *>(a.acc)[at * 16 + c4] = o;
             if (c4 == 0) a.ml[at * 2] = M, a.ml[at * 2 + 1] = sum;
         }
@@ -991,8 +1003,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) k_attend_many(Geo g, AttendAr
     const float cunit = exp2f((float)-g.centroid_frac);
     {
         float *cent = reinterpret_cast<float *>(sm + MANY_K_AT);
-        if (tid < (1 << KB)) cent[tid] = (float)a.tb->k_cent[tid] * cunit;
-        if (tid >= 32 && tid < 32 + (1 << VB)) cent[tid] = (float)a.tb->v_cent[tid - 32] * cunit;
+        if (tid < (1 << KB)) cent[tid] = (float)a.tb->k_cent[tid] * cunit * a.k_unit;
+        if (tid >= 32 && tid < 32 + (1 << VB)) cent[tid] = (float)a.tb->v_cent[tid - 32] * cunit * a.v_unit;
         __syncthreads();
         for (int e = warp; e < (1 << (2 * KB)); e += MANY_THREADS / 32)
             reinterpret_cast<uint32_t *>(sm)[e * 64 + lane] = pack_half2(cent[e & ((1 << KB) - 1)], cent[e >> KB]);
@@ -1473,6 +1485,7 @@ struct AttendPlan {
     using Seq = typename View::Seq;
     int rows = 16;
     bool many = false;                       // k_attend_many's runs, else k_attend_few's units
+    bool share = false;                      // four of them a CTA
     int64_t chunk = FEW_TILE, units = 0, groups = 0;
     int ctas = 0;                            // many: runs
     int max_splits = 1;
@@ -1535,17 +1548,31 @@ int cut_plan(const Geo &g, const View &view, int sms, AttendPlan<View> &p) {
     // chunk whose units still fit one wave; else a quarter of an SM's share of
     // all tokens, so that the last wave's unevenness stays small.
     const int64_t least = 4 * FEW_TILE;
-    int64_t chunk;
-    if (units_at(INT32_MAX) <= sms) {
-        int64_t lo = 1, hi = 1 << 25;                // in units of `least`
+    // the smallest chunk whose units are at most `n` (which one split per item has to be)
+    int64_t longest = 0;
+    for (const typename View::Seq &s : p.seqs) longest = std::max<int64_t>(longest, view.span(s));
+    auto fitting = [&](int64_t n) {
+        int64_t lo = 1, hi = (longest + least - 1) / least;      // in units of `least`
         while (lo < hi) {
             const int64_t mid = (lo + hi) / 2;
-            if (units_at(mid * least) <= sms) hi = mid;
+            if (units_at(mid * least) <= n) hi = mid;
             else lo = mid + 1;
         }
-        chunk = lo * least;
-    } else {
-        chunk = std::max<int64_t>(least, (total / (4 * sms) + least - 1) / least * least);
+        return lo * least;
+    };
+    const int64_t items = units_at(INT32_MAX);
+    int64_t chunk;
+    if (items <= sms) chunk = fitting(sms);
+    else chunk = std::max<int64_t>(least, (total / (4 * sms) + least - 1) / least * least);
+    if (View::SHARES) {
+        // Four units a CTA, of a quarter of its warps each: where there are more
+        // items than SMs, and where quarters of chunks fill the SMs more evenly.
+        const int64_t quarter = items <= sms ? fitting(4 * sms)
+                                             : std::max<int64_t>(least, (total * 3 / (8 * sms) + least - 1) / least * least);
+        p.share = items > sms || 10 * 4 * std::min(quarter, longest) < 9 * std::min(chunk, longest);
+        if (p.share) chunk = quarter;
+        // no join for a short rest (64 sequences of 768 tokens: 16 us whole, 33 cut)
+        if (2 * longest <= 3 * chunk) chunk = std::max(chunk, (longest + least - 1) / least * least);
     }
     chunk = std::min<int64_t>(chunk, INT32_MAX - least);
     p.chunk = chunk;
@@ -1567,16 +1594,16 @@ inline int device_sms(int dev, int *sms) {
     return INS_OK;
 }
 
-template <int KB, int VB, int MT, bool HALF, int NW, class View>
+template <int KB, int VB, int MT, bool HALF, int NW, int SHARE, class View>
 int launch_few(CacheBase *c, const AttendPlan<View> &p, const Plan &plan, const AttendArgs &a, const View &v,
                cudaStream_t s) {
     const size_t smem = FewLayout<KB, VB>::bytes(c->g, NW, 16 * MT);
     return plan.run(c, s, [&](const auto &src) -> cudaError_t {
-        auto fn = k_attend_few<KB, VB, MT, HALF, NW, View, std::decay_t<decltype(src)>>;
+        auto fn = k_attend_few<KB, VB, MT, HALF, NW, SHARE, View, std::decay_t<decltype(src)>>;
         const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return e;
         *c->launches += 1;
-        return launch_after(fn, (unsigned)p.units, NW * 32u, smem, s, c->g, a, v, src);
+        return launch_after(fn, (unsigned)((p.units + SHARE - 1) / SHARE), NW * 32u, smem, s, c->g, a, v, src);
     });
 }
 
@@ -1588,9 +1615,15 @@ int launch_few_rows(CacheBase *c, const AttendPlan<View> &p, bool half, const Pl
     // three where 32 rows take 168 (8 nodes of 1M: 12 warps 302 us, 14 spill:
     // 468). 8-bit rows make a stage 8.4 KB: 8 warps of them fit.
     constexpr int N1 = KB ? 20 : 8, N2 = KB ? 12 : 8;
-    if (p.rows == 32) return launch_few<KB, VB, 2, false, N2>(c, p, plan, a, v, s);
-    if (half) return launch_few<KB, VB, 1, true, N1>(c, p, plan, a, v, s);
-    return launch_few<KB, VB, 1, false, N1>(c, p, plan, a, v, s);
+    if constexpr (View::SHARES)
+        if (p.share) {
+            if (p.rows == 32) return launch_few<KB, VB, 2, false, N2, 4>(c, p, plan, a, v, s);
+            if (half) return launch_few<KB, VB, 1, true, N1, 4>(c, p, plan, a, v, s);
+            return launch_few<KB, VB, 1, false, N1, 4>(c, p, plan, a, v, s);
+        }
+    if (p.rows == 32) return launch_few<KB, VB, 2, false, N2, 1>(c, p, plan, a, v, s);
+    if (half) return launch_few<KB, VB, 1, true, N1, 1>(c, p, plan, a, v, s);
+    return launch_few<KB, VB, 1, false, N1, 1>(c, p, plan, a, v, s);
 }
 
 template <int KB, int VB, bool ROWS, class View>
@@ -1626,6 +1659,7 @@ AttendArgs attend_args(const CacheBase *c, const AttendPlan<View> &p, const int3
     a.ml = a.acc + (size_t)p.slots() * p.rows * 64;
     a.status = c->d_status;
     a.n_seqs = (int32_t)p.seqs.size();
+    a.units = (int32_t)p.units;
     a.chunk = (int32_t)p.chunk;
     a.row_tiles_rows = p.rows;
     a.poll_limit = std::min(c->wait.poll_limit, WAIT_POLLS);
@@ -1635,6 +1669,7 @@ AttendArgs attend_args(const CacheBase *c, const AttendPlan<View> &p, const int3
     a.q_scale = std::min(a.score_unit, 1.0f);
     a.k_scale = std::max(a.score_unit, 1.0f);
     a.out_unit = std::ldexp(1.0f, 9 - c->g.norm_frac);
+    a.k_unit = a.v_unit = 1.0f;
     return a;
 }
 

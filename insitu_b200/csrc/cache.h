@@ -146,6 +146,8 @@ struct CacheBase {
     std::vector<int32_t> split_seq;
     bool split_armed = false;
     double cent_max = 0.0;              // the largest centroid's magnitude, of keys and values
+    // factors in [1, 2) under which the centroids' roundings to fp16 are smallest
+    float k_unit = 1.0f, v_unit = 1.0f;
 
     int64_t capacity() const { return (int64_t)cfg.max_pages_per_seq * cfg.page_tokens; }
     int32_t *table_row(int32_t seq) const { return h_page_table + (size_t)seq * (size_t)cfg.max_pages_per_seq; }

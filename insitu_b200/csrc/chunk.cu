@@ -208,7 +208,13 @@ int chunk_body(CacheBase *c, int32_t B, const int32_t *seq, const int32_t *count
     if (bytes > workspace_bytes || (bytes && (!workspace || ((uintptr_t)workspace & 127u))))
         return fail(INS_EINVAL, "chunk scan: a 128-byte aligned workspace of " + std::to_string(bytes) + " bytes is needed");
     if (p.tiles) return run_tiles(c, p, v, q, out, workspace, sms, s);
-    return run_plan(c, p.few, attend_args(c, p.few, q, out, workspace), v, s);
+    AttendArgs a = attend_args(c, p.few, q, out, workspace);
+    a.k_unit = c->k_unit;
+    a.v_unit = c->v_unit;
+    a.score_unit /= a.k_unit;
+    a.k_scale /= a.k_unit;
+    a.out_unit /= a.v_unit;
+    return run_plan(c, p.few, a, v, s);
 }
 
 }  // namespace

@@ -32,6 +32,7 @@ struct ChunkSeq : AttendSeq {
 
 struct ChunkView {
     using Seq = ChunkSeq;
+    static constexpr bool SHARES = true;
     int32_t window, sinks;                   // no window: one larger than any position
     struct Row {
         int32_t p, from, sinks;              // sees `from` to p, and what is below sinks

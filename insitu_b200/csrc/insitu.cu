@@ -6,6 +6,8 @@
 // (cache/compressed.py:42-86). Kernels read device mirrors of it that every
 // mutating call refreshes with stream-ordered copies before its launch.
 
+#include <cuda_fp16.h>
+
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -126,6 +128,25 @@ int push_mirrors(ins_cache *c, cudaStream_t s, int32_t seq_lo, int32_t seq_hi) {
                        sizeof(int32_t) * row * (size_t)(seq_hi - seq_lo), cudaMemcpyHostToDevice, s));
     CK(cudaEventRecord(c->mirror_done, s));
     return INS_OK;
+}
+
+// The factor in [1, 2), of 512, under which the centroids' roundings to fp16 sum
+// to the least square. A codebook has few values, so their errors do not
+// average out: those of 3-bit ones go from 4e-4 of a centroid to 1e-4 at most.
+float fp16_unit(const int64_t *cent, int n, int frac) {
+    double best = 0.0;
+    float unit = 1.0f;
+    for (int i = 0; i < 512; ++i) {
+        const float u = 1.0f + (float)i / 512.0f;
+        double sum = 0.0;
+        for (int k = 0; k < n; ++k) {
+            const float x = (float)std::ldexp((double)cent[k], -frac) * u;
+            const double e = ((double)__half2float(__float2half_rn(x)) - x) / u;
+            sum += e * e;
+        }
+        if (i == 0 || sum < best) best = sum, unit = u;
+    }
+    return unit;
 }
 
 int64_t capacity_of(const ins_cache *c) {
@@ -281,6 +302,8 @@ int ins_cache_create(const ins_config *cfg, const ins_tables *tb, int32_t device
     for (int i = 0; i < nk; ++i) c->cent_max = std::max(c->cent_max, std::fabs((double)tb->k_centroids[i]));
     for (int i = 0; i < nv; ++i) c->cent_max = std::max(c->cent_max, std::fabs((double)tb->v_centroids[i]));
     c->cent_max = std::ldexp(c->cent_max, -cfg->centroid_frac);
+    c->k_unit = fp16_unit(tb->k_centroids, nk, cfg->centroid_frac);
+    c->v_unit = fp16_unit(tb->v_centroids, nv, cfg->centroid_frac);
     c->device = device;
     auto cleanup = [&](int rc) {
         ins_cache_destroy(c);

@@ -24,6 +24,7 @@ __device__ __forceinline__ uint32_t seen32(const uint64_t *mk, int nodes, int d)
 
 struct TreeView {
     using Seq = AttendSeq;
+    static constexpr bool SHARES = false;
     const uint64_t *mask;
     int32_t words;
     struct Row {

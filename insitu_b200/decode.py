@@ -61,6 +61,14 @@ class DecodeAttention:
         q_rot = self.pc.ingress([seq] * n, k, v, q)
         return self.pc.scan([seq] * n, q_rot, lengths=base + 1 + np.arange(n), mode=mode)
 
+    def chunk_attend(self, seq: int, q, k, v, *, window: int | None = None, sinks: int = 0):
+        """``prefill_attend`` in floating point (``PagedCache.chunk_scan``), under
+        a window and sinks if asked: append the n tokens, then every one attends.
+        Returns out (n, Hq, d) bfloat16 in real units, in the rotated basis."""
+        n = k.shape[0]
+        q_rot = self.pc.ingress([seq] * n, k, v, q)
+        return self.pc.chunk_scan([seq], q_rot, n, window=window, sinks=sinks)
+
     @staticmethod
     def merge_heads(out: torch.Tensor) -> torch.Tensor:
         """(B, heads, d) -> (B, heads*d), ops/project.py:67-74."""

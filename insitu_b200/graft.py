@@ -99,9 +99,11 @@ def _rope(config):
 def build_from_layer(attn_module, config, *, quant: QuantConfig | None = None,
                      fmt: FixedFormat | None = None, capacity: int = 4096, layer_idx: int = 0,
                      device=None, decoder=None, seq: int = 0,
-                     softmax: str = "two_pass") -> GpuKernelAttention:
+                     softmax: str = "two_pass", window: int | None = None,
+                     sinks: int = 0) -> GpuKernelAttention:
     """A GpuKernelAttention from an attention module's weights (W_o is folded).
-    ``decoder``/``seq`` place its cache in a shared DecodeAttention's slot."""
+    ``decoder``/``seq`` place its cache in a shared DecodeAttention's slot;
+    ``softmax``, ``window`` and ``sinks`` are AttentionLayer's."""
     w = lambda n: getattr(attn_module, f"{n}_proj").weight.detach().float().cpu().numpy()
 
     def b(n):
@@ -122,7 +124,7 @@ def build_from_layer(attn_module, config, *, quant: QuantConfig | None = None,
                            max_position=getattr(config, "max_position_embeddings", 4096),
                            rope_scaling=scaling, q_norm=gain("q_norm"), k_norm=gain("k_norm"),
                            norm_eps=eps, biases=(b("q"), b("k"), b("v"), b("o")), capacity=capacity,
-                           device=device, decoder=decoder, seq=seq, softmax=softmax)
+                           device=device, decoder=decoder, seq=seq, softmax=softmax, window=window, sinks=sinks)
     return GpuKernelAttention(layer, layer_idx, hk, d)
 
 

@@ -38,18 +38,28 @@ def fold_o_proj(o_proj, rotation: Rotation, num_heads: int, head_dim: int) -> np
 class AttentionLayer:
     """One layer: x (tokens, hidden) fp32 in, y (tokens, hidden) fp32 out,
     its compressed cache on the GPU. ``w_o`` is the checkpoint's W_o; pass
-    ``o_folded=True`` when it already carries the fold."""
+    ``o_folded=True`` when it already carries the fold. ``softmax``: "two_pass"
+    and "online" are the reference's fixed-point scans, "float" is
+    ``PagedCache.chunk_scan``, which is what a long prompt wants; it alone takes
+    a ``window`` (of cached tokens, a token's own among them) and ``sinks``."""
 
     def __init__(self, w_q, w_k, w_v, w_o, *, hidden: int, num_heads: int, num_kv_heads: int,
                  head_dim: int = 64, quant: QuantConfig | None = None, fmt: FixedFormat | None = None,
                  rope_theta: float = 10000.0, max_position: int = 4096,
                  rope_scaling: RopeScaling | None = None, q_norm=None, k_norm=None,
                  norm_eps: float = 1e-6, biases=(None, None, None, None), o_folded: bool = False,
-                 cast_after_rope: bool = True, softmax: str = "two_pass", capacity: int = 4096,
-                 device=None, decoder: DecodeAttention | None = None, seq: int = 0):
+                 cast_after_rope: bool = True, softmax: str = "two_pass", window: int | None = None,
+                 sinks: int = 0, capacity: int = 4096, device=None, decoder: DecodeAttention | None = None, seq: int = 0):
         # "two_pass" is AttentionKernel's default (kernel.py:117-124); the
         # board runs "online"
-        self.softmax = softmax
+        if softmax not in ("two_pass", "online", "float"):
+            raise ValueError(f"softmax={softmax!r}; expected two_pass, online or float")
+        if softmax != "float" and (window is not None or sinks):
+            raise ValueError("a window and sinks need softmax=\"float\"")
+        if (window is not None and window < 1) or sinks < 0:
+            raise ValueError(f"window={window} must be at least 1 or None, sinks={sinks} at least 0")
+        self.softmax, self.window, self.sinks = softmax, window, sinks
+        self.last_stats = None         # of the fixed-point scans
         self.quant = quant or QuantConfig(key_bits=4, value_bits=2)
         self.fmt = fmt or FixedFormat()
         self.hidden, self.hq, self.hk, self.d = hidden, num_heads, num_kv_heads, head_dim
@@ -97,7 +107,8 @@ class AttentionLayer:
     def forward(self, x, positions=None):
         """Rows of x are decode tokens, in order (a prefill when there are
         several). Returns y (tokens, hidden) fp32 on the device and the
-        attention output (tokens, num_heads * head_dim) int64 Q(acc_frac).
+        attention output (tokens, num_heads * head_dim), int64 Q(acc_frac) or
+        (softmax "float") bfloat16.
         Nodes of a ``verify`` that no ``accept`` kept are dropped first."""
         pc = self.dec.pc
         self._drop_drafted()
@@ -113,6 +124,10 @@ class AttentionLayer:
         else:
             pos = np.asarray(positions, np.int64)
         wq, wk, wv = self._qkv_wire(x, pos)
+        if self.softmax == "float":
+            merged = self.dec.chunk_attend(self.seq, wq, wk, wv, window=self.window, sinks=self.sinks)
+            merged = merged.reshape(n, self.hq * self.d)
+            return project(self.w_o, merged.to(torch.float32), self.b_o, rounded=True), merged
         out, self.last_stats = self.dec.prefill_attend(self.seq, wq, wk, wv, mode=self.softmax)
         merged = out.reshape(n, self.hq * self.d)
         acc = merged.to(torch.float64) / float(1 << self.fmt.qk_frac)      # Q.to_float
@@ -152,6 +167,8 @@ class AttentionLayer:
         keeps none. Returns y (nodes, hidden) fp32 and the
         attention output (nodes, num_heads, head_dim) bf16."""
         pc = self.dec.pc
+        if self.window is not None:
+            raise ValueError("verify attends the whole context; this layer has a window")
         if len(tree.counts) != 1 or tree.depths is None:
             raise ValueError("verify takes one tree with parents")
         x = torch.as_tensor(x).to(pc.device, torch.float32)
