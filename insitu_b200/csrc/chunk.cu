@@ -24,24 +24,8 @@ struct ChunkPlan {
     }
 };
 
-// Walks are cut at multiples of this.
-constexpr int WALK = 128;
 // Positions, and ends of tiles beyond them, stay well inside 32 bits.
 constexpr int32_t MAX_LENGTH = 1 << 30;
-static_assert(WALK % FEW_TILE == 0 && WALK % MANY_TILE == 0, "a tile of a walk is a run of positions");
-
-ChunkSeq walk_of(const ChunkView &v, int32_t seq, int64_t len, int32_t n, int64_t node0) {
-    ChunkSeq s{};
-    s.seq = seq;
-    s.context = (int32_t)(len - n);
-    s.nodes = n;
-    s.node0 = (int32_t)node0;
-    s.splits = 1;
-    const int32_t first = std::max(0, s.context + 1 - v.window) / WALK * WALK;
-    const int32_t early = (int32_t)(((int64_t)std::min(v.sinks, s.context + n) + WALK - 1) / WALK * WALK);
-    if (first > early) s.early = early, s.skip = first - early;
-    return s;
-}
 
 // Row tiles, units and pieces of k_chunk_tiles. Units are whole row tiles unless
 // that leaves SMs idle: a row tile's KV tiles are then cut so that the units
@@ -93,8 +77,13 @@ int cut_tiles(const Geo &g, const ChunkView &v, int sms, ChunkPlan &p) {
     return INS_OK;
 }
 
-// The expanded tiles' kernel takes over where a KV head has more than TILES_FROM
-// query rows in some sequence.
+// k_chunk_tiles takes over where a KV head has more than TILES_FROM query rows in
+// some sequence: 8 KV heads of 4 query heads, k_attend_many (or few) against it, of
+// 32,768 tokens and of 16 x 8,192: 64 tokens 53 : 60 us and 139 : 164, 96 tokens
+// 71 : 76 and 227 : 241, 128 tokens 77 : 77 and 247 : 248, 160 tokens 97 : 92 and
+// 345 : 318, 256 tokens 123 : 118 and 479 : 410. Not where its images would take
+// more than TILES_MOST bytes, nor in formats whose scores need a factor above 2^5
+// (k_attend_few takes those, at any number of rows).
 constexpr int64_t TILES_FROM = 512, TILES_MOST = (int64_t)8 << 30;
 
 int make_plan(const CacheBase *c, int32_t B, const int32_t *seq, const int32_t *counts, int sms, const ChunkView &v,

@@ -15,6 +15,16 @@
 // P V. P replaces S in tensor memory, so that there is room for three score buffers
 // of 128 columns next to two outputs of 64: while both streams work on a buffer
 // each, the third already holds the scores of the one that finishes first.
+//
+// 2,048 tokens on each of 4 sequences of 34,816 in all (8 KV heads of 4 query
+// heads, 2.27 TFLOP) take 2.36 ms, 0.96 PFLOP/s (2.68 ms in a run long enough for
+// the power cap). Bound by the exponentials and what surrounds them: of 2,200 clocks
+// a KV tile the special function unit works 70 %, the issue slots 61 %, the tensor
+// pipe 47 %. The steps there: one thread a row and one warp that issued all
+// products 2,814 us, as that warp's waits and issues (some 200 clocks each) followed
+// one another; two threads a row then 2,999, with a warp for the score products and
+// one a stream for the value products 2,565. Steps of 64 columns with three score
+// buffers a stream: 3,332 to 4,453, each step's fixed 700 clocks counting twice.
 #pragma once
 
 #include "attend.cuh"
@@ -36,18 +46,18 @@ struct ChunkView {
     int32_t window, sinks;                   // no window: one larger than any position
     struct Row {
         int32_t p, from, sinks;              // sees `from` to p, and what is below sinks
-        __device__ __forceinline__ bool sees(int t) const { return t <= p && (t >= from || t < sinks); }
-        __device__ __forceinline__ uint32_t bits(int t) const {
+        __host__ __device__ __forceinline__ bool sees(int t) const { return t <= p && (t >= from || t < sinks); }
+        __host__ __device__ __forceinline__ uint32_t bits(int t) const {
             auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? FULL : (1u << n) - 1u; };
             return below(p + 1 - t) & (~below(from - t) | below(sinks - t));
         }
     };
     __host__ __device__ __forceinline__ int span(const Seq &s) const { return s.context + s.nodes - s.skip; }
-    __device__ __forceinline__ int at(const Seq &s, int i) const { return i < s.early ? i : i + s.skip; }
-    __device__ __forceinline__ Row row(const Seq &s, int node) const {
+    __host__ __device__ __forceinline__ int at(const Seq &s, int i) const { return i < s.early ? i : i + s.skip; }
+    __host__ __device__ __forceinline__ Row row(const Seq &s, int node) const {
         return Row{s.context + node, s.context + node + 1 - window, sinks};
     }
-    __device__ __forceinline__ bool whole(const Seq &s, int t, int n) const {
+    __host__ __device__ __forceinline__ bool whole(const Seq &s, int t, int n) const {
         return t + n - 1 <= s.context && (t >= s.context + s.nodes - window || t + n <= sinks);
     }
 };
@@ -57,6 +67,9 @@ constexpr int TL_STAGES = 4, TL_THREADS = 20 * 32;
 constexpr int TL_Q_AT = 0, TL_KV_AT = 2 * 2 * TL_IMAGE, TL_UNIT_AT = TL_KV_AT + TL_STAGES * 2 * TL_IMAGE;
 constexpr int TL_HALVES_AT = TL_UNIT_AT + 128, TL_BARS_AT = TL_HALVES_AT + 2048, TL_SMEM = TL_BARS_AT + 256;
 
+// Pairs of 16 whose exponentials are polynomials, where no mask applies: 2,048
+// tokens of 4 x 34,816 take 2,539 us with none, 2,369, 2,341, 2,356 and 2,409 with
+// 3, 4, 5 and 6.
 constexpr int TL_POLY = 4;
 
 struct TilesArgs {
@@ -92,6 +105,33 @@ __host__ __device__ __forceinline__ RowTile row_tile(const ChunkView &v, const C
     t.jump = from > early ? from - early : 0;
     t.tiles = hi / TL_TILE + 1 - t.jump;
     return t;
+}
+
+// The KV tiles j of a row tile that all its rows see whole: those below `held` (of
+// sinks), and from `from` to below `to`.
+struct WholeTiles {
+    int32_t held, from, to;
+    __host__ __device__ __forceinline__ bool operator()(int j) const { return j < held || (j >= from && j < to); }
+};
+__host__ __device__ __forceinline__ WholeTiles whole_tiles(const ChunkView &v, int p_lo, int p_hi, int early, int jump) {
+    const int sunk = v.sinks / TL_TILE, left = p_hi - v.window, from = left < 0 ? 0 : left / TL_TILE + 1 - jump;
+    return WholeTiles{sunk < early ? sunk : early, from > early ? from : early, (p_lo + 1) / TL_TILE - jump};
+}
+
+// The walk of a sequence of `len` tokens whose last n are the chunk.
+constexpr int WALK = 128;
+static_assert(WALK % FEW_TILE == 0 && WALK % MANY_TILE == 0 && WALK % TL_TILE == 0, "a tile of a walk is a run of positions");
+inline ChunkSeq walk_of(const ChunkView &v, int32_t seq, int64_t len, int32_t n, int64_t node0) {
+    ChunkSeq s{};
+    s.seq = seq;
+    s.context = (int32_t)(len - n);
+    s.nodes = n;
+    s.node0 = (int32_t)node0;
+    s.splits = 1;
+    const int32_t first = std::max(0, s.context + 1 - v.window) / WALK * WALK;
+    const int32_t early = (int32_t)(((int64_t)std::min(v.sinks, s.context + n) + WALK - 1) / WALK * WALK);
+    if (first > early) s.early = early, s.skip = first - early;
+    return s;
 }
 
 // ---------------------------------------------------------------------------
@@ -533,14 +573,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
             const ChunkView::Row sees{p, p + 1 - view.window, view.sinks};
             float ref = -INFINITY, l = 0.0f;
             bool left = false;
-            // KV tiles that all rows see whole: those below `held` (of sinks), and from
-            // `whole0` to below `whole1`
-            const int held = min(view.sinks / TL_TILE, un.early), at_hi = un.p_hi - view.window;
-            const int whole0 = max(at_hi < 0 ? 0 : at_hi / TL_TILE + 1 - un.jump, un.early);
-            const int whole1 = (un.p_lo + 1) / TL_TILE - un.jump;
+            const WholeTiles is_whole = whole_tiles(view, un.p_lo, un.p_hi, un.early, un.jump);
             for (int j = un.lo; j < un.hi; ++j) {
                 const int t0 = (j < un.early ? j : j + un.jump) * TL_TILE + 64 * h;
-                const bool whole = j < held || (j >= whole0 && j < whole1);
+                const bool whole = is_whole(j);
                 const uint32_t S = tmem + lanes + 128 * (k6 >= 3 ? k6 - 3 : k6);
                 wait(s_ready(k6), use);
                 tc_fence_after();

@@ -153,6 +153,37 @@ def test_nodes_of_trees_add_their_paths():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("history", [1400, 12_289])
+def test_many_rows_of_shared_sequences(dtype, history):
+    """Sequences' own tokens, drafted ones among them and beside them, repeated;
+    sequences that no row names; rows aligned and not; more tokens of a slice
+    than its list holds."""
+    from insitu_b200 import Penalties
+    rng = np.random.default_rng(history)
+    for rows, vocab, pad, m in ((48, 30_001, 0, 5), (50, 9000, 3, 0), (64, 40_960, 0, 256)):
+        x, _, settings = setup(rng, rows, vocab, dtype, 1, pad)
+        tokens = torch.from_numpy((vocab * rng.random((5, history)) ** 3).astype(np.int64)).cuda()
+        tokens[1] = 7
+        tokens[2, ::2] = -1
+        kw = dict(tokens=tokens, lengths=ints(history, history, history - 1, 0, history), prompts=ints(0, 9, history, 4, -2),
+                  of=torch.from_numpy(rng.integers(0, 4, rows).astype(np.int32)).cuda())
+        if m:
+            drafted = torch.from_numpy((vocab * rng.random((rows, m)) ** 6).astype(np.int64)).cuda()
+            drafted[:, m // 2] = drafted[:, 0]
+            drafted[::3, 1:] = -1
+            kw["drafted"] = drafted
+        p = Penalties(**settings)
+        want = p(x, **kw)
+        check(want, x, settings, **kw)
+        more = dict(bias=torch.from_numpy(rng.standard_normal((1, vocab)).astype(np.float32)).cuda(),
+                    mask=some_mask(rng, rows, vocab))
+        check(p(x, **kw, **more), x, settings, **kw, **more)
+        y = x.contiguous()
+        assert torch.equal(p(y, **kw, out=y), want)
+
+
+@pytest.mark.gpu
 def test_ids_that_are_no_tokens_and_rows_that_are_no_sequences():
     from insitu_b200 import Penalties
     rng = np.random.default_rng(2)
