@@ -197,8 +197,12 @@ struct DenseLayout {
 
 // A warp takes 32 rows of a KV head, a thread a row, in turn with the next
 // task's codes already on their way. A thread holds its whole vector, so the
-// butterfly needs no exchange; the finished vectors go through shared memory
-// (rows padded by 16 bytes) so that eight lanes write each 128 bytes.
+// butterfly needs no exchange (four threads a vector, with exchanges and single
+// codes, took 115 us where this takes 67); the finished vectors go through shared
+// memory (rows padded by 16 bytes) so that eight lanes write each 128 bytes.
+//
+// Bound by the bytes, 52 read and 256 or 512 written a row and head: 131,072 rows
+// of 8 heads (4b/2b) in bf16 take 67 us, 4.8 TB/s, in fp32 124, 4.8 TB/s.
 template <int KB, int VB, typename T, class Src>
 __global__ void __launch_bounds__(DENSE_THREADS, sizeof(T) == 4 ? 1 : 2)
     k_dense(Geo g, const DevTables *__restrict__ tb, const uint8_t *__restrict__ pool,

@@ -9,7 +9,14 @@
 //
 // One pass: a CTA owns a slice of a row's vocabulary, counts the row's tokens
 // that fall into it in shared memory (a bit says which tokens have a count at
-// all), then reads, changes and writes its logits. Bound by the logits' bytes.
+// all), then changes and writes its logits, which it has read meanwhile. 256 rows
+// of 128,000 in bf16 with a mask take 30 us without tokens, 4.6 TB/s of reads and
+// writes; with 2,048 tokens a row 47, of 8,000 70 (12 us of a chain of loads and
+// atomics, then 3 us for each 1,000 tokens a row: each slice reads all of them).
+// 256 threads a CTA take 50 us, 1,024 77. Tried: a cluster that counts a row's
+// tokens once in distributed shared memory (79 us), equal tokens of a warp merged
+// before they are added (60), a kernel that lists each sequence's tokens once
+// (67; where 24 rows share a sequence of 9,000 tokens 77 us, this way 35).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -21,7 +28,7 @@
 
 namespace ins {
 
-constexpr int PEN_THREADS = 256, PEN_BYTES = 32768;      // logits of a slice, at most
+constexpr int PEN_THREADS = 512, PEN_BYTES = 32768;      // logits of a slice, at most
 constexpr int PEN_MAX_VOCAB = 1 << 18;
 constexpr int PEN_LIST = 4096;               // tokens with a count that a slice can list
 constexpr uint32_t PEN_ASKED = 1u << 31;     // in a count: the token is in the prompt
@@ -104,10 +111,9 @@ __device__ __forceinline__ Eight<T> load_eight(const T *from, uint32_t off) {
     return e;
 }
 
-// A thread changes PEN_GROUPS groups of eight logits, the groups where its
-// result's rows are aligned to 16 bytes, and single ones at a slice's ends. It
-// loads them before the tokens are counted, so that their latency passes
-// meanwhile.
+// A thread changes GROUPS groups of eight logits, the groups where its result's
+// rows are aligned to 16 bytes, and single ones at a slice's ends. It loads them
+// before the tokens are counted, so that their latency passes meanwhile.
 template <typename T>
 __global__ void __launch_bounds__(PEN_THREADS) k_penalize(const PenaltyArgs a) {
     // [slice] counts, then values; a bit each; up to PEN_LIST tokens that have one
