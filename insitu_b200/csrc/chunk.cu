@@ -31,9 +31,10 @@ constexpr int32_t MAX_LENGTH = 1 << 30;
 // that leaves SMs idle: a row tile's KV tiles are then cut so that the units
 // fill rounds of one an SM evenly. Counted in KV tiles' times (1.26 us measured):
 // what a unit costs besides its tiles (4.5), and the join of pieces (1,024 units:
-// 44 us).
+// 44 us). False: the images would take too much.
+constexpr int64_t TILES_MOST = (int64_t)8 << 30;
 constexpr double UNIT_TILES = 4.5, JOIN_TILES = 0.034;
-int cut_tiles(const Geo &g, const ChunkView &v, int sms, ChunkPlan &p) {
+bool cut_tiles(const Geo &g, const ChunkView &v, int sms, ChunkPlan &p) {
     std::sort(p.seqs.begin(), p.seqs.end(), [](const ChunkSeq &a, const ChunkSeq &b) {
         return a.context + a.nodes != b.context + b.nodes ? a.context + a.nodes > b.context + b.nodes : a.node0 < b.node0;
     });
@@ -53,6 +54,7 @@ int cut_tiles(const Geo &g, const ChunkView &v, int sms, ChunkPlan &p) {
         longest = std::max(longest, most[i]);
         work += 0.5 * (double)(first + last) * s.rts * g.n_kv;
     }
+    if (p.image_bytes(g) > TILES_MOST) return false;
     double best = 0;
     int64_t piece = longest;
     for (int k = 1; k <= 64; ++k) {
@@ -72,9 +74,7 @@ int cut_tiles(const Geo &g, const ChunkView &v, int sms, ChunkPlan &p) {
         p.units += (int64_t)s.rts * g.n_kv * s.splits;
         p.splits = std::max(p.splits, (int)s.splits);
     }
-    if (p.units > INT32_MAX || (p.row_tiles + p.walk_tiles) * g.n_kv > INT32_MAX)
-        return fail(INS_EBADLEN, "too much work in one call");
-    return INS_OK;
+    return p.units <= INT32_MAX;
 }
 
 // k_chunk_tiles takes over where a KV head has more than TILES_FROM query rows in
@@ -84,7 +84,7 @@ int cut_tiles(const Geo &g, const ChunkView &v, int sms, ChunkPlan &p) {
 // 345 : 318, 256 tokens 123 : 118 and 479 : 410. Not where its images would take
 // more than TILES_MOST bytes, nor in formats whose scores need a factor above 2^5
 // (k_attend_few takes those, at any number of rows).
-constexpr int64_t TILES_FROM = 512, TILES_MOST = (int64_t)8 << 30;
+constexpr int64_t TILES_FROM = 512;
 
 int make_plan(const CacheBase *c, int32_t B, const int32_t *seq, const int32_t *counts, int sms, const ChunkView &v,
               ChunkPlan &p) {
@@ -106,13 +106,11 @@ int make_plan(const CacheBase *c, int32_t B, const int32_t *seq, const int32_t *
     }
     if (all > INT32_MAX / (g.n_kv * g.H)) return fail(INS_EBADLEN, "too many tokens in one call");
     if (p.seqs.empty()) return INS_OK;
-    if (most > TILES_FROM && score_shift(g) <= MANY_SHIFT) {
-        p.tiles = true;
-        if (int rc = cut_tiles(g, v, sms, p)) return rc;
-        if (p.image_bytes(g) <= TILES_MOST) return INS_OK;
-        p.tiles = false;
-    }
     p.few.seqs = p.seqs;
+    if (most > TILES_FROM && score_shift(g) <= MANY_SHIFT) {
+        p.tiles = cut_tiles(g, v, sms, p);
+        if (p.tiles) return INS_OK;
+    }
     return cut_plan(g, v, sms, p.few);
 }
 
