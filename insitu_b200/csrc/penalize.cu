@@ -16,7 +16,11 @@
 // 256 threads a CTA take 50 us, 1,024 77. Tried: a cluster that counts a row's
 // tokens once in distributed shared memory (79 us), equal tokens of a warp merged
 // before they are added (60), a kernel that lists each sequence's tokens once
-// (67; where 24 rows share a sequence of 9,000 tokens 77 us, this way 35).
+// (67; where 24 rows share a sequence of 9,000 tokens 77 us, this way 30), the
+// next tokens loaded while the last are added (a CTA an SM: 80), logits loaded
+// after the count so that three CTAs fit an SM (47, and 29). All rows' first
+// slices come first: common tokens fall into them, and such a CTA as the last one
+// holds the call up (33 -> 30 us at those 24 rows a sequence).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -29,7 +33,7 @@
 namespace ins {
 
 constexpr int PEN_THREADS = 512, PEN_BYTES = 32768;      // logits of a slice, at most
-constexpr int PEN_MAX_VOCAB = 1 << 18;
+constexpr int PEN_MAX_VOCAB = 1 << 18, PEN_MAX_HISTORY = 1 << 30;
 constexpr int PEN_LIST = 4096;               // tokens with a count that a slice can list
 constexpr uint32_t PEN_ASKED = 1u << 31;     // in a count: the token is in the prompt
 
@@ -44,7 +48,7 @@ struct PenaltyArgs {
     const float *bias;
     const uint32_t *mask;
     int64_t bias_stride, mask_stride;
-    int32_t vocab, slices, slice_log2;       // CTAs a row, each for 2^slice_log2 tokens
+    int32_t rows, vocab, slice_log2;         // a CTA: 2^slice_log2 tokens of a row
     int32_t history, histories, n_drafted;
 };
 
@@ -121,8 +125,8 @@ __global__ void __launch_bounds__(PEN_THREADS) k_penalize(const PenaltyArgs a) {
     __shared__ int listed;
     constexpr int GROUPS = PEN_BYTES / (8 * (int)sizeof(T)) / PEN_THREADS;
     wait_prior_grid();
-    const int64_t row = blockIdx.x / a.slices;
-    const int slice = 1 << a.slice_log2, first = (int)(blockIdx.x % a.slices) << a.slice_log2;
+    const int64_t row = blockIdx.x % a.rows;
+    const int slice = 1 << a.slice_log2, first = (int)(blockIdx.x / a.rows) << a.slice_log2;
     const int n = min(slice, a.vocab - first);
     const int tid = threadIdx.x;
     const T *x = static_cast<const T *>(a.logits) + row * a.stride + first;
@@ -269,12 +273,12 @@ int launch_penalize(PenaltyArgs a, int32_t rows, cudaStream_t s) {
     const int64_t least = 4 * (int64_t)sms;
     a.slice_log2 = sizeof(T) == 4 ? 13 : 14;
     while (a.slice_log2 > 11 && (int64_t)rows * ((a.vocab - 1 >> a.slice_log2) + 1) < least) --a.slice_log2;
-    a.slices = (a.vocab - 1 >> a.slice_log2) + 1;
-    if ((int64_t)rows * a.slices > INT32_MAX) return fail(INS_EBADLEN, "penalties: too many rows in one call");
+    const int64_t slices = (a.vocab - 1 >> a.slice_log2) + 1;
+    if (rows * slices > INT32_MAX) return fail(INS_EBADLEN, "penalties: too many rows in one call");
     const size_t slice = (size_t)1 << a.slice_log2;
     const size_t smem = (slice + slice / 32) * sizeof(uint32_t) + PEN_LIST * sizeof(uint16_t);
     CK(cudaFuncSetAttribute(k_penalize<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    CK(launch_after(k_penalize<T>, (unsigned)(rows * a.slices), (unsigned)PEN_THREADS, smem, s, a));
+    CK(launch_after(k_penalize<T>, (unsigned)(rows * slices), (unsigned)PEN_THREADS, smem, s, a));
     return INS_OK;
 }
 
@@ -299,13 +303,15 @@ extern "C" int ins_penalize(int32_t rows, int32_t vocab, const void *logits, int
         if (p->history < 0 || p->histories < 0 || p->n_drafted < 0 || p->tokens_stride < 0 || p->drafted_stride < 0 ||
             p->bias_stride < 0 || p->mask_stride < 0)
             return fail(INS_EINVAL, "penalties: a negative size or stride");
+        if (p->history > PEN_MAX_HISTORY || p->n_drafted > PEN_MAX_HISTORY)
+            return fail(INS_EBADLEN, "penalties: more than 2^30 tokens a row");
         if (p->tokens && !p->of && p->histories != rows)
             return fail(INS_EINVAL, "penalties: " + std::to_string(p->histories) + " rows of tokens for " +
                                         std::to_string(rows) + " rows of logits");
         const PenaltyArgs a{logits, out, stride, out_stride, p->tokens, p->drafted, p->tokens_stride,
                             p->drafted_stride, p->lengths, p->prompts, p->of, p->repetition, p->presence,
                             p->frequency, p->bias, reinterpret_cast<const uint32_t *>(p->mask), p->bias_stride,
-                            p->mask_stride, vocab, 0, 0, p->history, p->histories, p->drafted ? p->n_drafted : 0};
+                            p->mask_stride, rows, vocab, 0, p->history, p->histories, p->drafted ? p->n_drafted : 0};
         cudaStream_t s = (cudaStream_t)stream;
         if (dtype == INS_F32) return launch_penalize<float>(a, rows, s);
         if (dtype == INS_F16) return launch_penalize<__half>(a, rows, s);

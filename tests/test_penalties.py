@@ -341,3 +341,13 @@ def test_the_c_entry_checks_its_arguments():
                  (1, 5, None, 0, 5, None, 5), (1, (1 << 18) + 1, None, 0, 5, None, 5)):
         assert L.ins_penalize(*args, C.byref(p), None) == _lib.INS_EINVAL
     assert L.ins_penalize(0, 5, None, 0, 5, None, 5, None, None) == _lib.INS_OK
+
+
+def test_histories_whose_indexes_would_wrap_are_refused():
+    import ctypes as C
+    from insitu_b200 import _lib
+    L, x = _lib.lib(), C.create_string_buffer(64)              # refused before any of it is read
+    at = C.cast(x, C.c_void_p)
+    for sizes in (dict(history=(1 << 30) + 1, histories=1), dict(n_drafted=(1 << 30) + 1), dict(history=2 ** 31 - 1)):
+        p = _lib.PenaltiesArgs(**sizes)
+        assert L.ins_penalize(1, 5, at, 0, 5, at, 5, C.byref(p), None) == _lib.INS_EBADLEN
