@@ -265,11 +265,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // P = exp2(S - ref) of 64 columns of a row in fp16 pairs, with a factor of 2^7
-// (as sum has). Under the row's own maximum they sum to 2^13 at most; true if
-// they exceed 2^15, or a polynomial's range (P and sum are then not valid).
-// Up to there every weight is inside fp16, which keeps them down to 2^-31 of
-// the maximum, and no comparison of all scores is needed. POLY of 16 pairs go by
-// polynomials.
+// (as sum has). ref is the largest score of some that the row has seen: under
+// the row's own maximum the weights sum to 2^13 at most; true if they exceed
+// 2^15, or a polynomial's range (P and sum are then not valid). Up to there
+// every weight is inside fp16, which keeps them down to 2^-31 of the maximum,
+// and no comparison of all scores is needed. A row that has seen nothing yet
+// (-inf: a window leaves its unit's first tiles out) has no such ref, and its
+// sum says nothing: true too. POLY of 16 pairs go by polynomials.
 template <bool MASKED, int POLY, class Row>
 __device__ __forceinline__ bool weigh_half(uint32_t S, float ref, float &sum, uint32_t (&p)[32], const Row &row, int t0) {
     const float sub = (ref > -INFINITY ? -ref : 0.0f) + 7.0f;
@@ -303,7 +305,7 @@ __device__ __forceinline__ bool weigh_half(uint32_t S, float ref, float &sum, ui
     }
     const float2 v = split64(add_pair(acc[0], acc[1]));
     sum = v.x + v.y;
-    return sum > 32768.0f || (POLY && far > POLY_RANGE);
+    return !(ref > -INFINITY) || sum > 32768.0f || (POLY && far > POLY_RANGE);
 }
 // The largest of a row's 64 columns that it sees, and of `m`.
 template <class Row>
@@ -585,7 +587,7 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
                     uint32_t w[32];
                     bool over = lost || j == un.lo;
                     // the exponentials are taken under the maximum so far, and again in
-                    // the rare case that it was too low
+                    // the rare case that there is none, or it was too low
                     if (!over) {
                         if (whole) over = weigh_half<false, TL_POLY>(S + 64 * h, ref, sum, w, sees, t0);
                         else over = weigh_half<true, 0>(S + 64 * h, ref, sum, w, sees, t0);
@@ -667,8 +669,10 @@ __global__ void __launch_bounds__(TL_THREADS, 1) k_chunk_tiles(Geo g, TilesArgs 
 }
 
 // The pieces of a row tile, scaled to the largest of their maxima, added in
-// order and divided by the sum of weights. One CTA per 8 rows; a sequence
-// whose row tiles are whole has nothing to join.
+// order and divided by the sum of weights. A piece of which a row sees nothing
+// has a maximum of -inf and weighs nothing; the one that holds the row's own
+// token has a finite one. One CTA per 8 rows; a sequence whose row tiles are
+// whole has nothing to join.
 template <class Src>
 __global__ void __launch_bounds__(128) k_chunk_join(Geo g, TilesArgs a, ChunkView view, const __grid_constant__ Src src) {
     extern __shared__ float wt[];                    // [8][splits]
