@@ -193,19 +193,28 @@ void truncate(int64_t h, const at::Tensor &anchor, at::IntArrayRef seq_ids, at::
                              at::cuda::getCurrentCUDAStream().stream()));
 }
 
+// How many rows [t0, t0 + n) of the sequences are, all of which have to be
+// cached: known before a result of that size is allocated.
+int64_t cached_rows(int64_t h, const std::vector<int32_t> &seq, at::IntArrayRef t0, at::IntArrayRef n) {
+    int64_t total = 0;
+    for (size_t i = 0; i < seq.size(); ++i) {
+        const int64_t len = ins_cache_length(handle(h), seq[i]);
+        TORCH_CHECK_VALUE(len >= 0, "[status ", INS_EINVAL, "] sequence id ", seq[i], " out of range");
+        TORCH_CHECK_VALUE(t0[i] >= 0 && n[i] >= 0 && t0[i] <= len && n[i] <= len - t0[i], "[status ", INS_EBADLEN,
+                          "] rows outside sequence ", seq[i], "'s ", len, " cached tokens");
+        total += n[i];
+    }
+    return total;
+}
+
 // ins_cache_rows into a new (sum n, n_kv, row_bytes) uint8 tensor.
 at::Tensor rows(int64_t h, const at::Tensor &anchor, at::IntArrayRef seq_ids, at::IntArrayRef t0, at::IntArrayRef n,
                 int64_t n_kv, int64_t row_bytes) {
     c10::cuda::CUDAGuard guard(anchor.device());
     TORCH_CHECK_VALUE(t0.size() == seq_ids.size() && n.size() == seq_ids.size(),
                       "insitu: seq_ids, t0 and n disagree on their number");
-    int64_t total = 0;
-    for (const int64_t k : n) {
-        TORCH_CHECK_VALUE(k >= 0 && k <= INT32_MAX, "insitu: a row count out of range");
-        total += k;
-    }
-    at::Tensor out = at::empty({total, n_kv, row_bytes}, anchor.options().dtype(at::kByte));
     const std::vector<int32_t> s = ids32(seq_ids);
+    at::Tensor out = at::empty({cached_rows(h, s, t0, n), n_kv, row_bytes}, anchor.options().dtype(at::kByte));
     check(ins_cache_rows(handle(h), n_ids(seq_ids), s.data(), t0.data(), n.data(), out.data_ptr<uint8_t>(),
                          at::cuda::getCurrentCUDAStream().stream()));
     return out;
@@ -299,13 +308,8 @@ std::tuple<at::Tensor, at::Tensor> dense(int64_t h, const at::Tensor &anchor, at
     TORCH_CHECK_VALUE(t0.size() == seq_ids.size() && n.size() == seq_ids.size(),
                       "insitu: seq_ids, t0 and n disagree on their number");
     const int32_t dtype = element_type(type);
-    int64_t total = 0;
-    for (const int64_t x : n) {
-        TORCH_CHECK_VALUE(x >= 0 && x <= INT32_MAX, "insitu: a row count out of range");
-        total += x;
-    }
-    at::Tensor k = at::empty({total, n_kv, 64}, anchor.options().dtype(type)), v = at::empty_like(k);
     const std::vector<int32_t> s = ids32(seq_ids);
+    at::Tensor k = at::empty({cached_rows(h, s, t0, n), n_kv, 64}, anchor.options().dtype(type)), v = at::empty_like(k);
     check(ins_cache_dense(handle(h), n_ids(seq_ids), s.data(), t0.data(), n.data(), k.data_ptr(), v.data_ptr(), dtype,
                           rotated, at::cuda::getCurrentCUDAStream().stream()));
     return {k, v};
