@@ -298,8 +298,13 @@ extern "C" int ins_penalize(int32_t rows, int32_t vocab, const void *logits, int
         if (stride < 0 || (out_stride < vocab && rows > 1))
             return fail(INS_EINVAL, "penalties: a negative row stride, or rows of the result that overlap");
         const int size = dtype == INS_F32 ? 4 : 2;
-        if ((uintptr_t)logits % size || (uintptr_t)out % size || (uintptr_t)p->tokens % 8 || (uintptr_t)p->drafted % 8)
-            return fail(INS_EINVAL, "penalties: a buffer is not aligned to its elements");
+        bool aligned = (uintptr_t)logits % size == 0 && (uintptr_t)out % size == 0;
+        for (const void *of_8 : {p->tokens, p->drafted}) aligned &= (uintptr_t)of_8 % 8 == 0;
+        for (const void *of_4 : {(const void *)p->lengths, (const void *)p->prompts, (const void *)p->of,
+                                 (const void *)p->repetition, (const void *)p->presence, (const void *)p->frequency,
+                                 (const void *)p->bias, (const void *)p->mask})
+            aligned &= (uintptr_t)of_4 % 4 == 0;
+        if (!aligned) return fail(INS_EINVAL, "penalties: a buffer is not aligned to its elements");
         if (p->history < 0 || p->histories < 0 || p->n_drafted < 0 || p->tokens_stride < 0 || p->drafted_stride < 0 ||
             p->bias_stride < 0 || p->mask_stride < 0)
             return fail(INS_EINVAL, "penalties: a negative size or stride");

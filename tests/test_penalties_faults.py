@@ -1,0 +1,37 @@
+"""Calls of the penalties that their C entry has to refuse before it launches anything."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+
+from insitu_b200 import _lib
+
+
+def refused(rows=1, vocab=5, dtype=0, logits=0, out=0, **fields):
+    """ins_penalize's status over host memory, none of which a refused call reads; logits and out are `logits`
+    and `out` bytes from an aligned address."""
+    memory = C.create_string_buffer(512)
+    base = (C.addressof(memory) + 15) // 16 * 16
+    args = _lib.PenaltiesArgs(**{k: base + v if k not in SIZES else v for k, v in fields.items()})
+    return _lib.lib().ins_penalize(rows, vocab, base + logits, dtype, vocab, base + out, vocab, C.byref(args), None)
+
+
+SIZES = ("history", "histories", "n_drafted")
+OF_4 = ("lengths", "prompts", "of", "repetition", "presence", "frequency", "bias", "mask")
+
+
+@pytest.mark.parametrize("name", OF_4 + ("tokens", "drafted"))
+def test_buffers_that_are_not_aligned_to_their_elements_are_refused(name):
+    """The kernel loads whole elements; an address between two would be a fault on the device."""
+    for off in (1, 2, 3) if name in OF_4 else (1, 4, 7):
+        assert refused(history=1, histories=1, n_drafted=1, **{name: off}) == _lib.INS_EINVAL, off
+    assert b"aligned" in _lib.lib().ins_last_error()
+
+
+def test_logits_and_results_that_are_not_aligned_are_refused():
+    for dtype, offs in ((0, (1, 2, 3)), (1, (1, 3)), (2, (1, 3))):
+        for off in offs:
+            assert refused(dtype=dtype, logits=off) == _lib.INS_EINVAL
+            assert refused(dtype=dtype, out=off) == _lib.INS_EINVAL
