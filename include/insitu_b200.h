@@ -549,7 +549,7 @@ int ins_sample(int32_t rows, int32_t vocab, const void *logits, int32_t dtype, i
 typedef struct ins_penalties {
     const int64_t *tokens;                     /* [histories] rows of `history`, tokens_stride apart */
     int64_t tokens_stride;
-    int32_t history, histories;                /* history, n_drafted: up to 2^30 */
+    int32_t history, histories;                /* history, n_drafted: up to 2^30, below 2^31 in all */
     const int32_t *lengths, *prompts;          /* [histories] */
     const int32_t *of;                         /* [rows] */
     const int64_t *drafted;                    /* [rows] rows of n_drafted, drafted_stride apart */

@@ -310,6 +310,8 @@ extern "C" int ins_penalize(int32_t rows, int32_t vocab, const void *logits, int
             return fail(INS_EINVAL, "penalties: a negative size or stride");
         if (p->history > PEN_MAX_HISTORY || p->n_drafted > PEN_MAX_HISTORY)
             return fail(INS_EBADLEN, "penalties: more than 2^30 tokens a row");
+        if ((int64_t)p->history + p->n_drafted >= PEN_ASKED)
+            return fail(INS_EBADLEN, "penalties: a row's tokens and drafted ones are 2^31, which a count does not hold");
         if (p->tokens && !p->of && p->histories != rows)
             return fail(INS_EINVAL, "penalties: " + std::to_string(p->histories) + " rows of tokens for " +
                                         std::to_string(rows) + " rows of logits");

@@ -35,3 +35,8 @@ def test_logits_and_results_that_are_not_aligned_are_refused():
         for off in offs:
             assert refused(dtype=dtype, logits=off) == _lib.INS_EINVAL
             assert refused(dtype=dtype, out=off) == _lib.INS_EINVAL
+
+
+def test_tokens_that_together_would_reach_the_bit_beside_a_count_are_refused():
+    """A token said 2^31 times would read as one of the prompt, never said."""
+    assert refused(histories=1, tokens=0, drafted=0, history=1 << 30, n_drafted=1 << 30) == _lib.INS_EBADLEN
