@@ -64,10 +64,16 @@ class DecodeAttention:
     def chunk_attend(self, seq: int, q, k, v, *, window: int | None = None, sinks: int = 0):
         """``prefill_attend`` in floating point (``PagedCache.chunk_scan``), under
         a window and sinks if asked: append the n tokens, then every one attends.
-        Returns out (n, Hq, d) bfloat16 in real units, in the rotated basis."""
+        Returns out (n, Hq, d) bfloat16 in real units, in the rotated basis. Where
+        the scan is refused or has no room, the cache is left as it was."""
         n = k.shape[0]
+        base = self.pc.length(seq)
         q_rot = self.pc.ingress([seq] * n, k, v, q)
-        return self.pc.chunk_scan([seq], q_rot, n, window=window, sinks=sinks)
+        try:
+            return self.pc.chunk_scan([seq], q_rot, n, window=window, sinks=sinks)
+        except Exception:
+            self.pc.truncate([seq], [base])
+            raise
 
     @staticmethod
     def merge_heads(out: torch.Tensor) -> torch.Tensor:
