@@ -564,7 +564,7 @@ typedef struct ins_penalties {
 
 /* out (rows of vocab elements, out_stride >= vocab apart) is the changed
  * logits, of their type; it may be the logits themselves (the same pointer and
- * stride), and may not overlap them otherwise. vocab in [1, 262144]; stride as
+ * stride), and may not overlap them otherwise, nor any other buffer. vocab in [1, 262144]; stride as
  * in ins_sample. Runs on the device of the current context, stream-ordered. */
 int ins_penalize(int32_t rows, int32_t vocab, const void *logits, int32_t dtype, int64_t stride, void *out,
                  int64_t out_stride, const ins_penalties *penalties, void *stream);

@@ -393,15 +393,22 @@ void penalize(const at::Tensor &logits, const c10::optional<at::Tensor> &tokens,
                           out.sizes() == logits.sizes() && (vocab < 2 || out.stride(1) == 1) &&
                           (n < 2 || out.stride(0) >= vocab),
                       "insitu: out must be a tensor of logits' shape, type and device whose rows do not overlap");
-    if (n > 0 && (out.data_ptr() != logits.data_ptr() || (n > 1 && out.stride(0) != logits.stride(0)))) {
-        auto span = [&](const at::Tensor &t) {
-            const auto *from = static_cast<const char *>(t.data_ptr());
-            return std::make_pair(from, from + ((n - 1) * t.stride(0) + vocab) * t.element_size());
-        };
-        const auto a = span(out), b = span(logits);
-        TORCH_CHECK_VALUE(a.second <= b.first || b.second <= a.first,
-                          "insitu: out must be logits itself, or lie wholly before or after it in memory");
-    }
+    auto span = [](const at::Tensor &t) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        const auto *from = static_cast<const char *>(t.data_ptr());
+        return std::make_pair(from, t.numel() ? from + (last + 1) * t.element_size() : from);
+    };
+    const auto a = span(out);
+    auto apart = [&](const at::Tensor &t) {
+        const auto b = span(t);
+        return a.second <= b.first || b.second <= a.first;
+    };
+    TORCH_CHECK_VALUE((out.data_ptr() == logits.data_ptr() && (n < 2 || out.stride(0) == logits.stride(0))) || apart(logits),
+                      "insitu: out must be logits itself, or lie wholly before or after it in memory");
+    // (rows are written while others still read what is theirs, or all rows')
+    for (const auto *t : {&tokens, &lengths, &prompts, &of, &drafted, &repetition, &presence, &frequency, &bias, &mask})
+        TORCH_CHECK_VALUE(!t->has_value() || apart(**t), "insitu: out shares memory with an argument that is not logits");
     check(ins_penalize((int32_t)n, (int32_t)vocab, logits.data_ptr(), dtype, logits.stride(0), out.data_ptr(),
                        n > 1 ? out.stride(0) : vocab, &p, at::cuda::getCurrentCUDAStream().stream()));
 }

@@ -47,7 +47,7 @@ class Penalties(RowSettings):
                  out: torch.Tensor | None = None) -> torch.Tensor:
         """``logits`` (rows, vocab) float32, float16 or bfloat16 on the GPU, rows
         at any stride. Returns them changed, in a new tensor or ``out`` (which
-        may be ``logits``). All other tensors are on the same device:
+        may be ``logits``, and shares memory with no other argument). All other tensors are on the same device:
 
         ``tokens`` (sequences, n) int64, a sequence a row of logits, or row i's
         sequence ``of[i]`` (int32); ``lengths`` (sequences,) int32, how many of

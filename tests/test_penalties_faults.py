@@ -40,3 +40,23 @@ def test_logits_and_results_that_are_not_aligned_are_refused():
 def test_tokens_that_together_would_reach_the_bit_beside_a_count_are_refused():
     """A token said 2^31 times would read as one of the prompt, never said."""
     assert refused(histories=1, tokens=0, drafted=0, history=1 << 30, n_drafted=1 << 30) == _lib.INS_EBADLEN
+
+
+@pytest.mark.gpu
+def test_a_result_over_another_argument_is_refused():
+    """A row of the result that is another row's bias, or all rows', would be written while it is read."""
+    torch = pytest.importorskip("torch")
+    from insitu_b200 import Penalties
+    x, wide = torch.randn((4, 3001), device="cuda"), torch.randn((9, 3001), device="cuda")
+    tokens = torch.randint(0, 3001, (4, 20), device="cuda")
+    p = Penalties(repetition=[1.0, 1.5, 1.1, 1.2])
+    want = p(x, tokens, bias=wide[0])
+    for kw in (dict(bias=wide[0], out=wide[:4]), dict(bias=wide[3], out=wide[:4]), dict(bias=wide[1:5], out=wide[:4]),
+               dict(bias=wide[:4], out=wide[1:5]), dict(mask=wide.view(torch.int32)[2, :94], out=wide[:4])):
+        with pytest.raises(ValueError):
+            p(x, tokens, **kw)
+    long = torch.zeros((4, 6002), dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError):
+        p(x, long[:, :7], out=long.view(torch.float32)[:, :3001])
+    assert torch.equal(p(x, tokens, bias=wide[0], out=wide[1:5]), want)
+    assert Penalties()(x[:0], bias=wide[0], out=wide[:0]).shape == (0, 3001)
