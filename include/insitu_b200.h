@@ -484,8 +484,8 @@ int ins_tree_scan(ins_cache *cache, int32_t B, const int32_t *seq_ids, const int
  * ops/attention.py:517-871, which ins_scan does for a chunk). Sequence
  * seq_ids[i]'s last counts[i] cached tokens (0 up to all; already appended by
  * an ingress) are a chunk; each attends itself and the tokens before it, under
- * a window (window > 0; 0: none) only those of the last `window` positions,
- * its own among them, and the sequence's first `sinks` tokens. A position is a
+ * a window (window > 0; 0: none, whatever `sinks`) only those of the last
+ * `window` positions, its own among them, and the sequence's first `sinks` tokens. A position is a
  * row's place in the cache. Outputs, numerics, buffers and their alignment are
  * ins_tree_scan's; q_rot and out hold sum counts tokens, workspace (128-byte
  * aligned) ins_chunk_workspace bytes for the same cache and arguments (the

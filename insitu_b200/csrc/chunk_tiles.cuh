@@ -17,8 +17,8 @@
 // each, the third already holds the scores of the one that finishes first.
 //
 // 2,048 tokens on each of 4 sequences of 34,816 in all (8 KV heads of 4 query
-// heads, 2.27 TFLOP) take 2.36 ms, 0.96 PFLOP/s (2.68 ms in a run long enough for
-// the power cap). Bound by the exponentials and what surrounds them: of 2,200 clocks
+// heads, 2.27 TFLOP) take 2.69 ms, 0.84 PFLOP/s, in a run long enough for the power
+// cap, 2.35 ms, 0.97 PFLOP/s, in a short one (as the steps below). Bound by the exponentials and what surrounds them: of 2,200 clocks
 // a KV tile the special function unit works 70 %, the issue slots 61 %, the tensor
 // pipe 47 %. The steps there: one thread a row and one warp that issued all
 // products 2,814 us, as that warp's waits and issues (some 200 clocks each) followed
@@ -69,7 +69,7 @@ constexpr int TL_HALVES_AT = TL_UNIT_AT + 128, TL_BARS_AT = TL_HALVES_AT + 2048,
 
 // Pairs of 16 whose exponentials are polynomials, where no mask applies: 2,048
 // tokens of 4 x 34,816 take 2,539 us with none, 2,369, 2,341, 2,356 and 2,409 with
-// 3, 4, 5 and 6.
+// 3, 4, 5 and 6 (short runs, before the power cap).
 constexpr int TL_POLY = 4;
 
 struct TilesArgs {

@@ -201,8 +201,11 @@ struct DenseLayout {
 // codes, took 115 us where this takes 67); the finished vectors go through shared
 // memory (rows padded by 16 bytes) so that eight lanes write each 128 bytes.
 //
-// Bound by the bytes, 52 read and 256 or 512 written a row and head: 131,072 rows
-// of 8 heads (4b/2b) in bf16 take 67 us, 4.8 TB/s, in fp32 124, 4.8 TB/s.
+// 52 bytes read and 256 or 512 written a row and head: 131,072 rows of 8 heads
+// (4b/2b) in bf16 take 69 us, 4.7 TB/s, in fp32 124 to 128, 4.7 TB/s. Bound by L1 (81 %
+// busy, most of it shared memory: table entries, the vectors' stage) and by its
+// latency, which 15 warps an SM do not cover; 1,054 instructions a warp's 32 rows
+// fill half of the issue slots.
 template <int KB, int VB, typename T, class Src>
 __global__ void __launch_bounds__(DENSE_THREADS, sizeof(T) == 4 ? 1 : 2)
     k_dense(Geo g, const DevTables *__restrict__ tb, const uint8_t *__restrict__ pool,

@@ -11,8 +11,9 @@
 // that fall into it in shared memory (a bit says which tokens have a count at
 // all), then changes and writes its logits, which it has read meanwhile. 256 rows
 // of 128,000 in bf16 with a mask take 30 us without tokens, 4.6 TB/s of reads and
-// writes; with 2,048 tokens a row 47, of 8,000 70 (12 us of a chain of loads and
-// atomics, then 3 us for each 1,000 tokens a row: each slice reads all of them).
+// writes; with 2,048 tokens a row 47 to 49, of 8,000 70 (12 us of a chain of loads
+// and atomics, then 3 us for each 1,000 tokens a row: each slice reads all of them).
+// With 2,048 the issue slots are busy to 67 %, DRAM to 22 %.
 // 256 threads a CTA take 50 us, 1,024 77. Tried: a cluster that counts a row's
 // tokens once in distributed shared memory (79 us), equal tokens of a warp merged
 // before they are added (60), a kernel that lists each sequence's tokens once

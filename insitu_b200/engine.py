@@ -360,7 +360,8 @@ class PagedCache:
         sequence; 1 is a decode token), appended by ``ingress``, whose rotated
         queries ``q_rot`` (tokens, n_kv*groups, d) are. ``window``: a token
         attends the last ``window`` positions, its own among them, and the
-        sequence's first ``sinks`` tokens; None: every position up to its own.
+        sequence's first ``sinks`` tokens; None: every position up to its own,
+        whatever ``sinks`` says.
         Returns q_rot's shape in bfloat16."""
         g = self.geo
         q = self._dev_i32(q_rot, (g.num_heads, g.head_dim))

@@ -41,7 +41,8 @@ class AttentionLayer:
     ``o_folded=True`` when it already carries the fold. ``softmax``: "two_pass"
     and "online" are the reference's fixed-point scans, "float" is
     ``PagedCache.chunk_scan``, which is what a long prompt wants; it alone takes
-    a ``window`` (of cached tokens, a token's own among them) and ``sinks``."""
+    a ``window`` (of cached tokens, a token's own among them) and ``sinks``
+    (the first tokens, which a window leaves visible; without one all are)."""
 
     def __init__(self, w_q, w_k, w_v, w_o, *, hidden: int, num_heads: int, num_kv_heads: int,
                  head_dim: int = 64, quant: QuantConfig | None = None, fmt: FixedFormat | None = None,
