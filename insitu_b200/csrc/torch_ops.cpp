@@ -406,9 +406,17 @@ void penalize(const at::Tensor &logits, const c10::optional<at::Tensor> &tokens,
     };
     TORCH_CHECK_VALUE((out.data_ptr() == logits.data_ptr() && (n < 2 || out.stride(0) == logits.stride(0))) || apart(logits),
                       "insitu: out must be logits itself, or lie wholly before or after it in memory");
-    // (rows are written while others still read what is theirs, or all rows')
+    // Rows of out are written while others still read what is theirs, or all
+    // rows'. Other columns of the same wider rows are no overlap.
+    auto beside = [&](const at::Tensor &t) {
+        const int64_t size = t.element_size(), every = n > 1 ? out.stride(0) * out.element_size() : 0;
+        if (every == 0 || t.dim() == 0 || (t.dim() == 2 && t.size(0) > 1 && t.stride(0) * size != every)) return false;
+        const int64_t off = static_cast<const char *>(t.data_ptr()) - a.first, at = (off % every + every) % every;
+        return at >= vocab * out.element_size() && at + t.size(-1) * size <= every;
+    };
     for (const auto *t : {&tokens, &lengths, &prompts, &of, &drafted, &repetition, &presence, &frequency, &bias, &mask})
-        TORCH_CHECK_VALUE(!t->has_value() || apart(**t), "insitu: out shares memory with an argument that is not logits");
+        TORCH_CHECK_VALUE(!t->has_value() || apart(**t) || beside(**t),
+                          "insitu: out shares memory with an argument that is not logits");
     check(ins_penalize((int32_t)n, (int32_t)vocab, logits.data_ptr(), dtype, logits.stride(0), out.data_ptr(),
                        n > 1 ? out.stride(0) : vocab, &p, at::cuda::getCurrentCUDAStream().stream()));
 }

@@ -60,3 +60,20 @@ def test_a_result_over_another_argument_is_refused():
         p(x, long[:, :7], out=long.view(torch.float32)[:, :3001])
     assert torch.equal(p(x, tokens, bias=wide[0], out=wide[1:5]), want)
     assert Penalties()(x[:0], bias=wide[0], out=wide[:0]).shape == (0, 3001)
+
+
+@pytest.mark.gpu
+def test_arguments_beside_the_result_in_wider_rows_are_not_over_it():
+    """Columns [0, 3001) of a buffer's rows hold the result, others a bias of each row or of all."""
+    torch = pytest.importorskip("torch")
+    from insitu_b200 import Penalties
+    x = torch.randn((4, 3001), device="cuda")
+    tokens = torch.randint(0, 3001, (4, 20), device="cuda")
+    p = Penalties(repetition=[1.0, 1.5, 1.1, 1.2])
+    buffer = torch.randn((4, 6010), device="cuda")
+    for bias in (buffer[:, 3001:6002], buffer[:, 3009:], buffer[2, 3005:6006]):
+        want = p(x, tokens, bias=bias.clone())
+        assert torch.equal(p(x, tokens, bias=bias, out=buffer[:, :3001]), want)
+    for bias in (buffer[:, 3000:6001], buffer[1, 3000:6001], buffer.flatten()[3010:6011]):
+        with pytest.raises(ValueError):
+            p(x, tokens, bias=bias, out=buffer[:, :3001])
